@@ -11,7 +11,7 @@ sequence are left as they are.
 
 * append: q and k are rotated by the angles of position p + position_offset (tables cos and sin), k and v go into the page.  For
   every page and key head the cache keeps bounds of its keys, channel by channel: int8 (lowest, highest), outwards rounded multiples of
-  a power of two, the smallest one that 127 multiples of reach the largest magnitude with (2^-24 to 2^96).
+  a power of two, the smallest one that 127 multiples of reach the largest magnitude with (2^-24 to 2^40).
 * attend: softmax attention over the shared prefix and over the sequence's own keys up to p.
 * attend_selected: the query, rounded to int8 multiples of such a power of two, times whichever bound gives more, summed over the
   channels, bounds what any key of a page can score; the best over the query heads of a key head is the page's score.  The
@@ -27,7 +27,7 @@ import torch
 own = False
 
 _DTYPES = {"bf16": torch.bfloat16, "fp16": torch.float16}
-_E_MIN, _E_MAX = -24, 96
+_E_MIN, _E_MAX = -24, 40
 
 
 # ------------------------------------------------------------------------------------------------------------ the cases
@@ -154,7 +154,7 @@ def work(case):
 # ------------------------------------------------------------------------------------------------------------ inputs
 
 def _exponent(amax):
-    """Smallest e in [-24, 96] with amax <= 127 * 2^e."""
+    """Smallest e in [-24, 40] with amax <= 127 * 2^e."""
     m, x = torch.frexp(amax.float())
     e = x - 7 + (m > 127.0 / 128.0).to(x.dtype)
     return torch.where(amax > 0, e, torch.full_like(e, _E_MIN)).clamp(_E_MIN, _E_MAX)
@@ -403,7 +403,7 @@ def run(st):
 # ------------------------------------------------------------------------------------------------------------ in 64 bits
 
 def _step(top):
-    """Smallest of 2^-24 .. 2^96 that 127 multiples of reach `top` with."""
+    """Smallest of 2^-24 .. 2^40 that 127 multiples of reach `top` with."""
     steps = torch.tensor([2.0 ** e for e in range(_E_MIN, _E_MAX + 1)], dtype=torch.float64, device=top.device)
     return steps[torch.searchsorted(127 * steps, top.contiguous()).clamp(max=len(steps) - 1)]
 
