@@ -363,6 +363,77 @@ int tv_v7_plan_sync(size_t n_synced, size_t n, const size_t *pending, size_t n_p
                     size_t n_fresh, size_t *materialise_out, size_t *n_materialise, size_t *carried_out,
                     size_t *n_carried, size_t *append_from, size_t *append_to);
 
+/* ---- paged key/value cache (csrc/kv_*.cu).  No reference counterpart: the reference indexes the vectors that models give out;
+ * these calls keep the keys and values that a model's attention reads, and read them: vectors are appended, a cheap score
+ * in whole numbers picks the pages worth reading (ties to the lower page, as in tv_search), and many requests can share one
+ * long prefix, such as the documents a search found.
+ *
+ * Unlike the calls above these are asynchronous: everything is device memory of the cache's device, the work is enqueued on
+ * `stream` (a cudaStream_t, may be null), nothing is allocated or kept, and a call may be captured into a CUDA graph.  The
+ * caller's current device is left as it was.  Failures that the host can see are returned, with a message in
+ * tv_last_error(NULL).
+ *
+ * A pool has `pages` pages of page_size (16, 32, 64 or 128) tokens for each of kv_heads key heads; head_dim is 64 or 128; dtype
+ * holds for keys, values, queries and outputs.  K and V are views [page][key head][token][channel] with channels adjacent and
+ * the other strides in elements, positive multiples of 8; 16-byte aligned.  bounds [page][key head][lowest, highest][channel]
+ * and scales [page][key head] are contiguous (32-byte aligned), or both null when no pages are ever chosen by score.
+ *
+ * A batch: row t of a call is token j of sequence b, offsets[b] <= t < offsets[b + 1] (offsets: sequences + 1 ascending
+ * numbers), and stands at position p = lens[b] - (offsets[b + 1] - offsets[b]) + j of the sequence's own pages, so lens counts the
+ * tokens of the call.  table[b] lists the pages of sequence b.  Rows outside [offsets[0], offsets[sequences]) are left as they are.
+ * What the host cannot see is checked on the device: a page number outside the pool holds no keys and stores none, positions
+ * below 0 or behind the table do not exist, offsets are cut to the call's rows.  Two sequences may share pages that are
+ * read; no two tokens of one tv_kv_append may go into the same place, nor new tokens of two sequences into one page. ---- */
+enum { TV_KV_BF16 = 0, TV_KV_F16 = 1 };
+typedef struct tv_kv_cache {
+    int device, dtype, head_dim, kv_heads, page_size;
+    int64_t pages;
+    void *k, *v;
+    int64_t k_page_stride, k_head_stride, k_token_stride;
+    int64_t v_page_stride, v_head_stride, v_token_stride;
+    int8_t *bounds;
+    float *scales;
+} tv_kv_cache;
+typedef struct tv_kv_batch {
+    int64_t sequences, table_width, table_stride;   /* table: [sequences][table_width], rows table_stride apart */
+    const int32_t *table, *lens, *offsets;
+} tv_kv_batch;
+typedef struct tv_kv_rows {                         /* [row][head][channel]: strides in elements, multiples of 8, channels adjacent */
+    void *data;
+    int64_t token_stride, head_stride;
+} tv_kv_rows;
+/* Appends `tokens` keys and values (kv_heads heads each) to the pages of their sequences and rotates keys and, where q is given
+ * (heads heads, a multiple of kv_heads), queries into q_out (which may be q) by the angles of position p + position_offset: cos
+ * and sin are [positions][rotary / 2] floats (16-byte aligned); rotary is a multiple of 16 up to head_dim, 0 = no rotation.
+ * interleaved = 0 pairs channels i and i + rotary / 2, 1 pairs 2i and 2i + 1.  y1 = x1 cos - x2 sin, y2 = x2 cos + x1 sin in
+ * 32 bits.  A token whose angle is outside the tables, or whose position is below 0, is neither stored nor rotated.  Brings bounds
+ * and scales of the pages up to date: a page whose first token is appended starts anew, others are widened, also when
+ * tokens are overwritten. */
+int tv_kv_append(const tv_kv_cache *cache, const tv_kv_batch *batch, int64_t tokens, int heads, const tv_kv_rows *k_new,
+                 const tv_kv_rows *v_new, const tv_kv_rows *q, const tv_kv_rows *q_out, const float *cos, const float *sin,
+                 int64_t positions, int rotary, int interleaved, int64_t position_offset, void *stream);
+/* out = softmax(scale * q k) v over the first prefix_len keys of the pages prefix_pages (prefix_width of them; none: 0) and the
+ * keys of the row's own sequence at positions up to p.  lse (may be null): natural logarithm of the sum of exponentials,
+ * [token][head].  A row that sees no key gives zeros and -infinity.  The workspace needs tv_kv_attend_workspace bytes (256-byte
+ * aligned), belongs to the call until its work is done, and need not be cleared. */
+size_t tv_kv_attend_workspace(const tv_kv_cache *cache, const tv_kv_batch *batch, int64_t tokens, int heads, int64_t prefix_len);
+int tv_kv_attend(const tv_kv_cache *cache, const tv_kv_batch *batch, int64_t tokens, int heads, const tv_kv_rows *q,
+                 const int32_t *prefix_pages, int64_t prefix_width, int64_t prefix_len, float scale, const tv_kv_rows *out,
+                 float *lse, void *workspace, size_t workspace_bytes, void *stream);
+/* The same over `budget` pages of the row's sequence (all of them where it has no more): the first `first` and the last `recent`
+ * visible ones, and of the others those with the best score, equal scores by the lower page.  The score of a page for a key head is
+ * the largest over its query heads of s * sum over channels of max(q8 lo, q8 hi), times the page's scale: lo and hi its bounds, q8 =
+ * q / s to the nearest whole number (ties to even) and s the smallest of 2^-24 .. 2^40 with |q| <= 127 s.  A page outside the pool comes
+ * last.  pages_out [token][key head][budget] receives the chosen page numbers of the sequence, ascending, then -1.  first + recent <=
+ * budget; table_width <= 49,152. */
+size_t tv_kv_attend_selected_workspace(const tv_kv_cache *cache, const tv_kv_batch *batch, int64_t tokens, int heads, int64_t budget);
+int tv_kv_attend_selected(const tv_kv_cache *cache, const tv_kv_batch *batch, int64_t tokens, int heads, const tv_kv_rows *q,
+                          int64_t budget, int64_t first, int64_t recent, float scale, const tv_kv_rows *out, float *lse,
+                          int32_t *pages_out, void *workspace, size_t workspace_bytes, void *stream);
+/* Waits for the device and tells whether a kernel of these calls gave up a wait since the last time it was asked (its results are
+ * then worthless): TV_OK or TV_ERR_DEVICE_TIMEOUT.  Not for a stream that is being captured. */
+int tv_kv_status(int device);
+
 /* ---- TQ+ calibration: calibrate_2d (lib.rs:2599-2723); on a populated index every stored row is re-encoded from
  * its own codes under the new pair (reencode_stored_rows, lib.rs:2760-2832); tqplus_shift/scale (lib.rs:2535-2545) ---- */
 int tv_calibrate(tv_index *h, const float *sample, size_t n, size_t dim);

@@ -111,6 +111,41 @@ SIGNATURES = {
     "tv_last_main_kernel_ms": (C.c_float, [_H, _intp]),
 }
 
+
+
+class KvCacheView(C.Structure):
+    """tv_kv_cache"""
+    _fields_ = [("device", C.c_int), ("dtype", C.c_int), ("head_dim", C.c_int), ("kv_heads", C.c_int), ("page_size", C.c_int),
+                ("pages", C.c_int64), ("k", C.c_void_p), ("v", C.c_void_p),
+                ("k_page_stride", C.c_int64), ("k_head_stride", C.c_int64), ("k_token_stride", C.c_int64),
+                ("v_page_stride", C.c_int64), ("v_head_stride", C.c_int64), ("v_token_stride", C.c_int64),
+                ("bounds", C.c_void_p), ("scales", C.c_void_p)]
+
+
+class KvBatchView(C.Structure):
+    """tv_kv_batch"""
+    _fields_ = [("sequences", C.c_int64), ("table_width", C.c_int64), ("table_stride", C.c_int64),
+                ("table", C.c_void_p), ("lens", C.c_void_p), ("offsets", C.c_void_p)]
+
+
+class KvRowsView(C.Structure):
+    """tv_kv_rows"""
+    _fields_ = [("data", C.c_void_p), ("token_stride", C.c_int64), ("head_stride", C.c_int64)]
+
+
+_cachep, _batchp, _rowsp = C.POINTER(KvCacheView), C.POINTER(KvBatchView), C.POINTER(KvRowsView)
+SIGNATURES.update({
+    "tv_kv_append": (C.c_int, [_cachep, _batchp, C.c_int64, C.c_int, _rowsp, _rowsp, _rowsp, _rowsp, C.c_void_p, C.c_void_p, C.c_int64,
+                               C.c_int, C.c_int, C.c_int64, C.c_void_p]),
+    "tv_kv_attend_workspace": (C.c_size_t, [_cachep, _batchp, C.c_int64, C.c_int, C.c_int64]),
+    "tv_kv_attend": (C.c_int, [_cachep, _batchp, C.c_int64, C.c_int, _rowsp, C.c_void_p, C.c_int64, C.c_int64, C.c_float, _rowsp,
+                               C.c_void_p, C.c_void_p, C.c_size_t, C.c_void_p]),
+    "tv_kv_attend_selected_workspace": (C.c_size_t, [_cachep, _batchp, C.c_int64, C.c_int, C.c_int64]),
+    "tv_kv_attend_selected": (C.c_int, [_cachep, _batchp, C.c_int64, C.c_int, _rowsp, C.c_int64, C.c_int64, C.c_int64, C.c_float, _rowsp,
+                                        C.c_void_p, C.c_void_p, C.c_void_p, C.c_size_t, C.c_void_p]),
+    "tv_kv_status": (C.c_int, [C.c_int]),
+})
+
 _lib = None
 
 

@@ -1787,6 +1787,17 @@ void blocked_to_packed(const uint8_t *blocked, size_t n, int bits, int dim, uint
 // =====================================================================================================
 // C ABI
 // =====================================================================================================
+namespace tv {
+int set_create_error(int code, const char *message) {
+    try {
+        g_create_error = message;
+    } catch (const std::bad_alloc &) {
+        g_create_error.clear();
+    }
+    return code;
+}
+}  // namespace tv
+
 extern "C" {
 
 const char *tv_version(void) { return "turbovec_b200 0.1 (sm_100a)"; }

@@ -1,0 +1,596 @@
+// Attention of a few query rows over the keys of a paged cache: a shared prefix, a sequence's own pages, or chosen pages.
+//
+// An item is up to 16 query rows of one key head (the heads that share it, times the tokens of one sequence; for a prefix the
+// rows of all sequences) and the keys they read, in tiles of 64.  All items' tiles are laid end to end and every block takes an equal
+// run of them, so that batches of any lengths fill the device evenly: lengths are known on the device alone.  A run that begins or
+// ends inside an item leaves partial results, (largest logit, sum of weights, weighted sum of values), in slot
+// item + block, a number that is different for every pair of the two that meet; a second kernel joins them.
+//
+// Bound by memory: a tile of 128 channels is 32 KB and 4 * 64 * 128 * 16 multiply-adds of which 16 / rows are padding.  One warp keeps the
+// ring of tiles full by tensor copies; four warps take 16 keys of each tile: no exchange between warps until the end of a part.
+#include <cfloat>
+
+#include "kv_cache.cuh"
+#include "scan_tc_common.cuh"
+
+namespace tv {
+namespace {
+
+constexpr int kConsumers = 4;
+constexpr int kAttendThreads = (kConsumers + 1) * 32;
+constexpr int kNothing = INT_MAX - kKvTile;              // first position of a group of keys that nobody sees
+
+__device__ uint32_t g_kv_timeouts;
+
+template <int D>
+struct Geometry {
+    static constexpr int kStages = D == 128 ? 3 : 6;
+    static constexpr int kHalfBytes = kKvTile * 128;      // 64 channels of a tile
+    static constexpr int kOperandBytes = kHalfBytes * (D / 64);
+    static constexpr int kStageBytes = 2 * kOperandBytes;
+};
+template <int D>
+struct AttendShared {
+    float o[kKvRows][D];
+    float2 ml[kConsumers][kKvRows];
+    int first_key[Geometry<D>::kStages][kConsumers];
+    int64_t scratch[kAttendThreads / 32 + 2];
+    uint64_t full[Geometry<D>::kStages], empty[Geometry<D>::kStages];
+};
+
+// A run of tiles of one item.
+struct Part {
+    int item, row0, rows;          // rows of the call's q: (token, head of the group) pairs row0 .. row0 + rows of `first_token` on
+    int first_token, h, b;         // b = -1: prefix
+    int tile0, tile1, item_tiles;  // tiles of this part, and of the item
+    int64_t item_start;            // the item's first tile in the whole list
+};
+
+// Walks the parts of a block's run [at, end) of the list.  Order of items: prefix by (key head, rows); then by (sequence, key head,
+// rows).  With chosen pages: by (token, key head, rows).
+template <bool CHOSEN>
+struct Walk {
+    const KvAttendParams &p;
+    int64_t at, end, prefix_total;
+    int live_first, live;           // tokens that belong to a sequence
+    int prefix_tiles, prefix_mt;
+    int b, item_of_b;               // sequence, its first item
+    int64_t start_of_b;
+
+    __device__ __forceinline__ int tiles_of(int len) const {
+        const int64_t cap = kv_capacity(p.batch.table_width, p.page_shift);
+        const int keys = kv_visible(int64_t(len) - 1, cap);
+        return keys < 1 ? 1 : (keys + kKvTile - 1) / kKvTile;        // an item without keys is one empty tile
+    }
+    __device__ __forceinline__ int row_tiles(int count) const { return int((int64_t(count) * p.group + kKvRows - 1) / kKvRows); }
+    __device__ __forceinline__ KvSpan span(int i) const { return kv_span(p.batch.offsets[i], p.batch.offsets[i + 1], p.tokens); }
+    __device__ __forceinline__ int64_t cost(int i) const {
+        return int64_t(row_tiles(span(i).count)) * p.kv_heads * tiles_of(p.batch.lens[i]);
+    }
+    __device__ __forceinline__ int64_t items(int i) const { return int64_t(row_tiles(span(i).count)) * p.kv_heads; }
+
+    __device__ __forceinline__ bool next(Part &out) {
+        if (at >= end) return false;
+        if constexpr (CHOSEN) {
+            const int per_item = (((p.budget << p.page_shift) + kKvTile - 1) / kKvTile), mt = row_tiles(1);
+            const int item = int(at / per_item), tile = int(at - int64_t(item) * per_item);
+            const int m = item % mt, th = item / mt;
+            out.item = item; out.b = 0;
+            out.h = th % p.kv_heads; out.first_token = live_first + th / p.kv_heads;
+            out.row0 = m * kKvRows; out.rows = min(kKvRows, p.group - out.row0);
+            out.tile0 = tile; out.item_tiles = per_item; out.item_start = at - tile;
+        } else if (at < prefix_total) {
+            const int item = int(at / prefix_tiles), tile = int(at - int64_t(item) * prefix_tiles);
+            const int m = item % prefix_mt;
+            out.item = item; out.b = -1; out.h = item / prefix_mt; out.first_token = live_first;
+            out.row0 = m * kKvRows; out.rows = min(int64_t(kKvRows), int64_t(live) * p.group - out.row0);
+            out.tile0 = tile; out.item_tiles = prefix_tiles; out.item_start = at - tile;
+        } else {
+            KvSpan sp = span(b);
+            int mt = row_tiles(sp.count), tiles = tiles_of(p.batch.lens[b]);
+            while (at - start_of_b >= int64_t(mt) * p.kv_heads * tiles) {
+                if (b + 1 >= p.batch.sequences) return false;
+                start_of_b += int64_t(mt) * p.kv_heads * tiles;
+                item_of_b += mt * p.kv_heads;
+                ++b;
+                sp = span(b); mt = row_tiles(sp.count); tiles = tiles_of(p.batch.lens[b]);
+            }
+            const int64_t place = at - start_of_b;
+            const int item = int(place / tiles), tile = int(place - int64_t(item) * tiles);
+            const int m = item % mt;
+            out.item = item_of_b + item; out.b = b; out.h = item / mt; out.first_token = sp.first;
+            out.row0 = m * kKvRows; out.rows = min(int64_t(kKvRows), int64_t(sp.count) * p.group - out.row0);
+            out.tile0 = tile; out.item_tiles = tiles; out.item_start = at - tile;
+        }
+        const int64_t left = end - at;
+        out.tile1 = out.tile0 + int(left < out.item_tiles - out.tile0 ? left : out.item_tiles - out.tile0);
+        at += out.tile1 - out.tile0;
+        return true;
+    }
+    // keys that row `r` of the part sees: those before this position
+    __device__ __forceinline__ int limit(const Part &w, int r) const {
+        if constexpr (CHOSEN) return p.token_pos[w.first_token] + 1;
+        if (w.b < 0) return p.prefix_len;
+        const KvSpan sp = span(w.b);
+        return kv_visible(int64_t(p.batch.lens[w.b]) - sp.count + (w.row0 + r) / p.group, kv_capacity(p.batch.table_width, p.page_shift));
+    }
+    // one past the last tile of the part that some row sees a key of
+    __device__ __forceinline__ int last_tile(const Part &w) const {
+        if constexpr (CHOSEN) return w.tile1;
+        return min(w.tile1, (limit(w, w.rows - 1) + kKvTile - 1) / kKvTile);
+    }
+};
+
+// Sets the walk of this block up; `per` = tiles of a run.  All threads.
+template <bool CHOSEN>
+__device__ __forceinline__ void set_up(Walk<CHOSEN> &w, int64_t *scratch, int64_t &per) {
+    const KvAttendParams &p = w.p;
+    const KvSpan all = kv_span(p.batch.offsets[0], p.batch.offsets[p.batch.sequences], p.tokens);
+    w.live_first = all.first; w.live = all.count;
+    int64_t total;
+    w.b = w.item_of_b = 0;
+    w.start_of_b = 0;
+    if constexpr (CHOSEN) {
+        w.prefix_total = 0; w.prefix_tiles = w.prefix_mt = 1;
+        total = int64_t(w.live) * p.kv_heads * w.row_tiles(1) * (((p.budget << p.page_shift) + kKvTile - 1) / kKvTile);
+    } else {
+        w.prefix_tiles = max(1, (p.prefix_len + kKvTile - 1) / kKvTile);
+        w.prefix_mt = max(1, w.row_tiles(w.live));
+        w.prefix_total = p.prefix_len > 0 && w.live > 0 ? int64_t(w.prefix_mt) * p.kv_heads * w.prefix_tiles : 0;
+        // total cost of the sequences
+        int64_t sum = 0;
+        for (int i = threadIdx.x; i < p.batch.sequences; i += kAttendThreads) sum += w.cost(i);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(kFullMask, sum, o);
+        if ((threadIdx.x & 31) == 0) scratch[threadIdx.x >> 5] = sum;
+        __syncthreads();
+        total = w.prefix_total;
+#pragma unroll
+        for (int i = 0; i < kAttendThreads / 32; ++i) total += scratch[i];
+        w.item_of_b = w.prefix_total > 0 ? w.prefix_mt * p.kv_heads : 0;
+        w.start_of_b = w.prefix_total;
+    }
+    per = max(int64_t(1), (total + gridDim.x - 1) / gridDim.x);
+    w.at = min(total, int64_t(blockIdx.x) * per);
+    w.end = min(total, w.at + per);
+    if constexpr (!CHOSEN) {
+        if (w.at < w.end && w.at > w.prefix_total) {
+            int b;
+            int64_t place;
+            kv_locate<kAttendThreads>(w.at - w.prefix_total, p.batch.sequences, [&](int i) { return w.cost(i); }, scratch, b, place);
+            w.b = b < p.batch.sequences ? b : p.batch.sequences - 1;
+            // items before sequence b
+            int64_t before = 0;
+            for (int i = threadIdx.x; i < w.b; i += kAttendThreads) before += w.items(i);
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) before += __shfl_xor_sync(kFullMask, before, o);
+            __syncthreads();
+            if ((threadIdx.x & 31) == 0) scratch[threadIdx.x >> 5] = before;
+            __syncthreads();
+#pragma unroll
+            for (int i = 0; i < kAttendThreads / 32; ++i) w.item_of_b += int(scratch[i]);
+            w.start_of_b = w.at - place;
+        }
+    }
+}
+
+__device__ __forceinline__ void tma_load_page(void *dst, const CUtensorMap *map, int channel, int token, int head, int page, uint64_t *bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];"
+        ::"r"(smem_u32(dst)), "l"(map), "r"(smem_u32(bar)), "r"(channel), "r"(token), "r"(head), "r"(page) : "memory");
+}
+__device__ __forceinline__ void ldmatrix4(uint32_t addr, uint32_t (&r)[4]) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void ldmatrix4_trans(uint32_t addr, uint32_t (&r)[4]) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+template <typename T>
+__device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    if constexpr (std::is_same<T, __nv_bfloat16>::value)
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                     : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    else
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                     : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void consumers_sync() { asm volatile("bar.sync 1, %0;" ::"n"(kConsumers * 32) : "memory"); }
+// a value whose exponent is all ones (infinite or NaN) among the two
+template <typename T>
+__device__ __forceinline__ bool not_finite(uint32_t x) {
+    constexpr uint32_t e = KvType<T>::kExponents;
+    return (x & e & 0xffffu) == (e & 0xffffu) || (x & e & 0xffff0000u) == (e & 0xffff0000u);
+}
+
+template <typename T, int D, bool CHOSEN>
+__global__ void __launch_bounds__(kAttendThreads, 2) kv_attend_kernel(const KvAttendParams p, const __grid_constant__ KvMaps maps) {
+    using G = Geometry<D>;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t *ring = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    AttendShared<D> &sh = *reinterpret_cast<AttendShared<D> *>(ring + G::kStages * G::kStageBytes);
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+
+    asm volatile("griddepcontrol.launch_dependents;");
+    if constexpr (CHOSEN) asm volatile("griddepcontrol.wait;" ::: "memory");
+    if (tid == 0) {
+        for (int s = 0; s < G::kStages; ++s) { mbar_init(&sh.full[s], 1); mbar_init(&sh.empty[s], kConsumers); }
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    __syncthreads();
+    Walk<CHOSEN> walk{p};
+    int64_t per;
+    set_up<CHOSEN>(walk, sh.scratch, per);
+    if (walk.at >= walk.end) return;
+    Part w;
+    uint32_t n = 0;                                     // tiles since the beginning: stage n % kStages, round n / kStages
+
+    if (warp == kConsumers) {                           // ---- the producer
+        const int box = min(kKvTile, 1 << p.page_shift), boxes = kKvTile / box;
+        bool ok = true;
+        while (walk.next(w)) {
+            const int last = walk.last_tile(w);
+            int chosen_count = p.budget;
+            const int32_t *list = nullptr, *pool = nullptr;
+            if constexpr (CHOSEN) {
+                const int64_t row = (int64_t(w.first_token) * p.kv_heads + w.h) * p.budget;
+                list = p.chosen + row; pool = p.chosen_pool + row;
+            }
+            for (int tile = w.tile0; tile < last; ++tile, ++n) {
+                const int s = n % G::kStages;
+                const int64_t key = int64_t(tile) * kKvTile + lane * box;
+                const int64_t entry = key >> p.page_shift;
+                const int token = int(key & ((1 << p.page_shift) - 1));
+                int page = -1, first = kNothing;
+                if (lane < boxes) {
+                    if constexpr (CHOSEN) {
+                        const int logical = entry < chosen_count ? list[entry] : -1;
+                        if (logical >= 0) { page = pool[entry]; first = (logical << p.page_shift) + token; }
+                    } else if (w.b < 0) {
+                        if (entry < p.prefix_width) page = __ldg(p.prefix_pages + entry);
+                        first = int(key);
+                    } else {
+                        if (entry < p.batch.table_width) page = __ldg(p.batch.table + int64_t(w.b) * p.batch.table_stride + entry);
+                        first = int(key);
+                    }
+                }
+                const bool good = page >= 0 && page < p.pages;
+                if (!good) { page = p.pages; first = kNothing; }      // outside the pool: the copy fills with zeros
+                if (ok && n >= G::kStages) ok = mbar_wait(&sh.empty[s], ((n / G::kStages) - 1) & 1, p.timeouts);
+                ok = __all_sync(kFullMask, ok);
+                if (!ok) break;
+                const int of_group = __shfl_sync(kFullMask, first, (lane & 3) * 16 / box);
+                if (lane < kConsumers) sh.first_key[s][lane] = of_group == kNothing ? kNothing : of_group + ((lane * 16) & (box - 1));
+                __syncwarp();
+                if (lane == 0) mbar_arrive_expect_tx(&sh.full[s], G::kStageBytes);
+                __syncwarp();
+                if (lane < boxes) {
+                    uint8_t *k = ring + s * G::kStageBytes + lane * box * 128, *v = k + G::kOperandBytes;
+#pragma unroll
+                    for (int c = 0; c < D / 64; ++c) {
+                        tma_load_page(k + c * G::kHalfBytes, &maps.k, c * 64, token, w.h, page, &sh.full[s]);
+                        tma_load_page(v + c * G::kHalfBytes, &maps.v, c * 64, token, w.h, page, &sh.full[s]);
+                    }
+                }
+            }
+            if (!ok) break;
+        }
+        if (!ok)                                        // the copies in flight land before the block ends
+            for (uint32_t i = n > G::kStages ? n - G::kStages : 0; i < n; ++i) mbar_wait(&sh.full[i % G::kStages], (i / G::kStages) & 1, p.timeouts);
+        return;
+    }
+
+    // ---- the consumers: 16 keys of every tile each
+    bool ok = true;
+    const int r0 = lane >> 2, r1 = r0 + 8, c2 = (lane & 3) * 2;
+    const uint32_t ring_addr = smem_u32(ring);
+    // row of this lane's ldmatrix address, and its 16-byte chunk before the swizzle
+    const int k_row = warp * 16 + ((lane >> 4) & 1) * 8 + (lane & 7), k_chunk = (lane >> 3) & 1;
+    const int v_row = warp * 16 + ((lane >> 3) & 1) * 8 + (lane & 7), v_chunk = (lane >> 4) & 1;
+    while (walk.next(w)) {
+        const int last = walk.last_tile(w);
+        uint32_t qf[D / 16][4];
+        auto q_row = [&](int r) -> const T * {
+            const int row = w.row0 + r;
+            return static_cast<const T *>(p.q.data) + int64_t(w.first_token + row / p.group) * p.q.token_stride +
+                   int64_t(w.h * p.group + row % p.group) * p.q.head_stride;
+        };
+        const bool have0 = r0 < w.rows, have1 = r1 < w.rows;
+        const T *q0 = q_row(have0 ? r0 : 0), *q1 = q_row(have1 ? r1 : 0);
+#pragma unroll
+        for (int i = 0; i < D / 16; ++i) {
+            qf[i][0] = have0 ? *reinterpret_cast<const uint32_t *>(q0 + 16 * i + c2) : 0u;
+            qf[i][1] = have1 ? *reinterpret_cast<const uint32_t *>(q1 + 16 * i + c2) : 0u;
+            qf[i][2] = have0 ? *reinterpret_cast<const uint32_t *>(q0 + 16 * i + 8 + c2) : 0u;
+            qf[i][3] = have1 ? *reinterpret_cast<const uint32_t *>(q1 + 16 * i + 8 + c2) : 0u;
+        }
+        const int lim0 = have0 ? walk.limit(w, r0) : 0, lim1 = have1 ? walk.limit(w, r1) : 0;
+        const int lim_first = walk.limit(w, 0), lim_last = walk.limit(w, w.rows - 1);
+        float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.0f, l1 = 0.0f;
+        float o[D / 8][4];
+#pragma unroll
+        for (int j = 0; j < D / 8; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.0f;
+
+        for (int tile = w.tile0; tile < last; ++tile, ++n) {
+            const int s = n % G::kStages;
+            if (ok) ok = mbar_wait(&sh.full[s], (n / G::kStages) & 1, p.timeouts);
+            const uint32_t k_addr = ring_addr + s * G::kStageBytes, v_addr = k_addr + G::kOperandBytes;
+            const int first = sh.first_key[s][warp];
+            float sc[2][4] = {};
+#pragma unroll
+            for (int i = 0; i < D / 16; ++i) {
+                uint32_t kf[4];
+                const int chunk = 2 * i + k_chunk;
+                ldmatrix4(k_addr + (chunk >> 3) * G::kHalfBytes + k_row * 128 + (((chunk & 7) ^ (k_row & 7)) << 4), kf);
+                mma16816<T>(sc[0], qf[i], kf[0], kf[1]);
+                mma16816<T>(sc[1], qf[i], kf[2], kf[3]);
+            }
+            // logits in powers of two; keys that a row does not see count for nothing, whatever they hold
+            const bool border = first + 16 > lim_first;
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    sc[j][e] *= p.scale_log2;
+                    sc[j][2 + e] *= p.scale_log2;
+                    if (border) {
+                        const int key = first + 8 * j + c2 + e;
+                        if (key >= lim0) sc[j][e] = -INFINITY;
+                        if (key >= lim1) sc[j][2 + e] = -INFINITY;
+                    }
+                }
+            float t0 = fmaxf(fmaxf(sc[0][0], sc[0][1]), fmaxf(sc[1][0], sc[1][1])), t1 = fmaxf(fmaxf(sc[0][2], sc[0][3]), fmaxf(sc[1][2], sc[1][3]));
+            t0 = fmaxf(t0, __shfl_xor_sync(kFullMask, t0, 1)); t1 = fmaxf(t1, __shfl_xor_sync(kFullMask, t1, 1));
+            t0 = fmaxf(t0, __shfl_xor_sync(kFullMask, t0, 2)); t1 = fmaxf(t1, __shfl_xor_sync(kFullMask, t1, 2));
+            if (__any_sync(kFullMask, t0 > m0 || t1 > m1)) {
+                const float n0 = fmaxf(m0, t0), n1 = fmaxf(m1, t1);
+                const float a0 = n0 == -INFINITY ? 1.0f : kv_exp2(m0 - n0), a1 = n1 == -INFINITY ? 1.0f : kv_exp2(m1 - n1);
+                m0 = n0; m1 = n1;
+                l0 *= a0; l1 *= a1;
+#pragma unroll
+                for (int j = 0; j < D / 8; ++j) { o[j][0] *= a0; o[j][1] *= a0; o[j][2] *= a1; o[j][3] *= a1; }
+            }
+            const float s0 = m0 == -INFINITY ? 0.0f : m0, s1 = m1 == -INFINITY ? 0.0f : m1;
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    sc[j][e] = kv_exp2(sc[j][e] - s0);
+                    sc[j][2 + e] = kv_exp2(sc[j][2 + e] - s1);
+                    l0 += sc[j][e];
+                    l1 += sc[j][2 + e];
+                }
+            // weights to the type for the second product: half a step each, and the sum of weights keeps what was rounded off
+            uint32_t pf[4] = {KvType<T>::pack(sc[0][0], sc[0][1]), KvType<T>::pack(sc[0][2], sc[0][3]),
+                              KvType<T>::pack(sc[1][0], sc[1][1]), KvType<T>::pack(sc[1][2], sc[1][3])};
+            // values of keys that no row sees: zero, for 0 * NaN is not 0
+            auto live_mask = [&](int key, int limit) { return (key < limit ? 0xffffu : 0u) | (key + 1 < limit ? 0xffff0000u : 0u); };
+            auto values = [&](int i, uint32_t (&vf)[4]) {
+                const int chunk = 2 * i + v_chunk;
+                ldmatrix4_trans(v_addr + (chunk >> 3) * G::kHalfBytes + v_row * 128 + (((chunk & 7) ^ (v_row & 7)) << 4), vf);
+            };
+            auto product = [&](const uint32_t (&a)[4], int limit) {
+                const bool all = first + 16 <= limit;
+                const uint32_t x0 = all ? ~0u : live_mask(first + c2, limit), x1 = all ? ~0u : live_mask(first + 8 + c2, limit);
+#pragma unroll
+                for (int i = 0; i < D / 16; ++i) {
+                    uint32_t vf[4];
+                    values(i, vf);
+                    mma16816<T>(o[2 * i], a, vf[0] & x0, vf[1] & x1);
+                    mma16816<T>(o[2 * i + 1], a, vf[2] & x0, vf[3] & x1);
+                }
+            };
+            bool apart = false;
+            if (!CHOSEN && border && lim_first < lim_last && first < lim_last) {
+                // keys that some rows see and others do not: an infinite value there must not reach the others
+                bool odd = false;
+                const uint32_t x0 = live_mask(first + c2, lim_last), x1 = live_mask(first + 8 + c2, lim_last);
+#pragma unroll
+                for (int i = 0; i < D / 16; ++i) {
+                    uint32_t vf[4];
+                    values(i, vf);
+                    odd |= not_finite<T>(vf[0] & x0) | not_finite<T>(vf[1] & x1) | not_finite<T>(vf[2] & x0) | not_finite<T>(vf[3] & x1);
+                }
+                apart = __any_sync(kFullMask, odd);
+            }
+            if (!apart) {
+                product(pf, lim_last);
+            } else {
+#pragma unroll 1
+                for (int limit = lim_first; limit <= lim_last; ++limit) {   // one token's rows after the other
+                    const bool on0 = have0 && lim0 == limit, on1 = have1 && lim1 == limit;
+                    if (!__any_sync(kFullMask, on0 || on1)) continue;
+                    const uint32_t a[4] = {on0 ? pf[0] : 0u, on1 ? pf[1] : 0u, on0 ? pf[2] : 0u, on1 ? pf[3] : 0u};
+                    float keep[D / 8][4];
+#pragma unroll
+                    for (int j = 0; j < D / 8; ++j)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) keep[j][e] = o[j][e];
+                    product(a, limit);
+#pragma unroll
+                    for (int j = 0; j < D / 8; ++j) {
+                        if (!on0) { o[j][0] = keep[j][0]; o[j][1] = keep[j][1]; }
+                        if (!on1) { o[j][2] = keep[j][2]; o[j][3] = keep[j][3]; }
+                    }
+                }
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sh.empty[s]);
+        }
+
+        // ---- the four warps' results together
+        l0 += __shfl_xor_sync(kFullMask, l0, 1); l1 += __shfl_xor_sync(kFullMask, l1, 1);
+        l0 += __shfl_xor_sync(kFullMask, l0, 2); l1 += __shfl_xor_sync(kFullMask, l1, 2);
+        if ((lane & 3) == 0) { sh.ml[warp][r0] = make_float2(m0, l0); sh.ml[warp][r1] = make_float2(m1, l1); }
+        consumers_sync();
+        float big0 = -INFINITY, big1 = -INFINITY, sum0 = 0.0f, sum1 = 0.0f;
+#pragma unroll
+        for (int i = 0; i < kConsumers; ++i) { big0 = fmaxf(big0, sh.ml[i][r0].x); big1 = fmaxf(big1, sh.ml[i][r1].x); }
+        const float base0 = big0 == -INFINITY ? 0.0f : big0, base1 = big1 == -INFINITY ? 0.0f : big1;
+#pragma unroll
+        for (int i = 0; i < kConsumers; ++i) {
+            sum0 = fmaf(kv_exp2(sh.ml[i][r0].x - base0), sh.ml[i][r0].y, sum0);
+            sum1 = fmaf(kv_exp2(sh.ml[i][r1].x - base1), sh.ml[i][r1].y, sum1);
+        }
+        const float f0 = kv_exp2(m0 - base0), f1 = kv_exp2(m1 - base1);
+#pragma unroll
+        for (int j = 0; j < D / 8; ++j) { o[j][0] *= f0; o[j][1] *= f0; o[j][2] *= f1; o[j][3] *= f1; }
+#pragma unroll 1
+        for (int i = kConsumers - 1; i >= 0; --i) {
+            if (warp == i) {
+#pragma unroll
+                for (int j = 0; j < D / 8; ++j) {
+                    const int col = (8 * j + c2) ^ (r0 * 8);           // rows lie a multiple of 32 words apart: spread their banks
+                    float2 *a = reinterpret_cast<float2 *>(&sh.o[r0][col]), *b = reinterpret_cast<float2 *>(&sh.o[r1][col]);
+                    if (i < kConsumers - 1) {
+                        o[j][0] += a->x; o[j][1] += a->y;
+                        o[j][2] += b->x; o[j][3] += b->y;
+                    }
+                    if (i > 0) { *a = make_float2(o[j][0], o[j][1]); *b = make_float2(o[j][2], o[j][3]); }
+                }
+            }
+            consumers_sync();
+        }
+        if (warp != 0) continue;
+        const bool whole = w.tile0 == 0 && w.tile1 == w.item_tiles && p.prefix_len == 0;
+        const int64_t slot = int64_t(w.item) + blockIdx.x;
+        auto finish = [&](int r, bool have, float big, float sum, int e) {
+            if (!have) return;
+            const int row = w.row0 + r;
+            const int64_t token = w.first_token + row / p.group, head = w.h * p.group + row % p.group;
+            if (whole) {
+                const float inv = sum > 0.0f || sum != sum ? 1.0f / sum : 0.0f;            // no key: zero
+                T *dst = static_cast<T *>(p.out.data) + token * p.out.token_stride + head * p.out.head_stride;
+#pragma unroll
+                for (int j = 0; j < D / 8; ++j) *reinterpret_cast<uint32_t *>(dst + 8 * j + c2) = KvType<T>::pack(o[j][e] * inv, o[j][e + 1] * inv);
+                if (c2 == 0 && p.lse) p.lse[token * p.heads + head] = sum > 0.0f || sum != sum ? (big + log2f(sum)) * 0.6931471805599453f : -INFINITY;
+            } else if (slot < p.slots) {
+                float *dst = p.part_o + (slot * kKvRows + r) * D;
+#pragma unroll
+                for (int j = 0; j < D / 8; ++j) *reinterpret_cast<float2 *>(dst + 8 * j + c2) = make_float2(o[j][e], o[j][e + 1]);
+                if (c2 == 0) p.part_ml[slot * kKvRows + r] = make_float2(big, sum);
+            }
+            if (c2 == 0 && w.tile0 == 0) {                      // where the parts of the item lie, packed with the row within a slot
+                const int64_t begin = w.item_start / per, finish_at = (w.item_start + w.item_tiles - 1) / per;
+                KvPieces pc{int(w.item + begin), whole ? 0 : int(finish_at - begin + 1)};
+                (w.b < 0 ? p.prefix_pieces : p.own_pieces)[token * p.heads + head] = pc;
+            }
+        };
+        finish(r0, have0, big0, sum0, 0);
+        finish(r1, have1, big1, sum1, 2);
+    }
+}
+
+// Joins the parts of a row: one warp per (token, head).
+template <typename T, int D>
+__global__ void __launch_bounds__(128) kv_join_kernel(const KvAttendParams p) {
+    constexpr int kPer = D / 32;
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const int lane = threadIdx.x & 31;
+    const int64_t row = int64_t(blockIdx.x) * 4 + (threadIdx.x >> 5);
+    const int token = int(row / p.heads), head = int(row % p.heads);
+    const KvSpan all = kv_span(p.batch.offsets[0], p.batch.offsets[p.batch.sequences], p.tokens);
+    if (token < all.first || token >= all.first + all.count) return;       // behind the last sequence: as it was
+    float big = -INFINITY, sum = 0.0f, acc[kPer] = {};
+    auto add = [&](const KvPieces &pc, int in_item) {
+        if (pc.first_slot < 0 || pc.count < 0 || int64_t(pc.first_slot) + pc.count > p.slots) return;
+        for (int i0 = 0; i0 < pc.count; i0 += 32) {
+            const int left = min(32, pc.count - i0);
+            const int64_t slot = pc.first_slot + i0;
+            const float2 ml = lane < left ? p.part_ml[(slot + lane) * kKvRows + in_item] : make_float2(-INFINITY, 0.0f);
+            float top = ml.x;
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(kFullMask, top, o));
+            const float next = fmaxf(big, top), base = next == -INFINITY ? 0.0f : next;
+            const float old = kv_exp2(big - base), mine = kv_exp2(ml.x - base);
+            float part = mine * ml.y;
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) part += __shfl_xor_sync(kFullMask, part, o);
+            sum = fmaf(sum, old, part);
+            big = next;
+#pragma unroll
+            for (int j = 0; j < kPer; ++j) acc[j] *= old;
+#pragma unroll 4
+            for (int i = 0; i < left; ++i) {
+                const float f = __shfl_sync(kFullMask, mine, i);
+                const float *src = p.part_o + ((slot + i) * kKvRows + in_item) * D + lane * kPer;
+                float x[kPer];
+                if constexpr (kPer == 4) { const float4 y = *reinterpret_cast<const float4 *>(src); x[0] = y.x; x[1] = y.y; x[2] = y.z; x[3] = y.w; }
+                else { const float2 y = *reinterpret_cast<const float2 *>(src); x[0] = y.x; x[1] = y.y; }
+#pragma unroll
+                for (int j = 0; j < kPer; ++j) acc[j] = fmaf(f, x[j], acc[j]);
+            }
+        }
+    };
+    const KvPieces own = p.own_pieces[row];
+    if (own.count == 0 && p.prefix_len == 0) return;
+    // the row's place within its items: rows of a group lie together, token after token
+    const int h = head / p.group, g = head - h * p.group;
+    if (p.prefix_len > 0) add(p.prefix_pieces[row], int((int64_t(token - all.first) * p.group + g) % kKvRows));
+    int from = 0;
+    if (p.chosen == nullptr) {                       // first token of the row's sequence
+        int lo = 0, hi = p.batch.sequences;
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) >> 1;
+            if (p.batch.offsets[mid] <= token) lo = mid; else hi = mid;
+        }
+        from = kv_span(p.batch.offsets[lo], p.batch.offsets[lo + 1], p.tokens).first;
+        add(own, int((int64_t(token - from) * p.group + g) % kKvRows));
+    } else {
+        add(own, g % kKvRows);
+    }
+    const float inv = sum > 0.0f || sum != sum ? 1.0f / sum : 0.0f;
+    uint32_t *dst = reinterpret_cast<uint32_t *>(static_cast<T *>(p.out.data) + token * p.out.token_stride + head * p.out.head_stride + lane * kPer);
+#pragma unroll
+    for (int j = 0; j < kPer / 2; ++j) dst[j] = KvType<T>::pack(acc[2 * j] * inv, acc[2 * j + 1] * inv);
+    if (lane == 0 && p.lse) p.lse[row] = sum > 0.0f || sum != sum ? (big + log2f(sum)) * 0.6931471805599453f : -INFINITY;
+}
+
+template <typename T, int D, bool CHOSEN>
+cudaError_t launch(const KvAttendParams &p, const KvMaps &maps, int sm_count, cudaStream_t s) {
+    using G = Geometry<D>;
+    const size_t smem = size_t(G::kStages) * G::kStageBytes + sizeof(AttendShared<D>) + 1024;
+    auto *kern = kv_attend_kernel<T, D, CHOSEN>;
+    cudaError_t e = allow_dynamic_shared(kern);
+    if (e != cudaSuccess) return e;
+    cudaLaunchAttribute after;
+    after.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    after.val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(unsigned(kv_attend_grid(sm_count)));
+    cfg.blockDim = dim3(kAttendThreads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    cfg.attrs = &after;
+    cfg.numAttrs = CHOSEN ? 1 : 0;
+    e = cudaLaunchKernelEx(&cfg, kern, p, maps);
+    if (e != cudaSuccess) return e;
+    cfg.gridDim = dim3(unsigned((int64_t(p.tokens) * p.heads + 3) / 4));
+    cfg.blockDim = dim3(128);
+    cfg.dynamicSmemBytes = 0;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kv_join_kernel<T, D>, p);
+}
+
+}  // namespace
+
+int kv_attend_grid(int sm_count) { return 2 * sm_count; }
+
+uint32_t *kv_timeouts_symbol() {
+    void *ptr = nullptr;
+    return cudaGetSymbolAddress(&ptr, g_kv_timeouts) == cudaSuccess ? static_cast<uint32_t *>(ptr) : nullptr;
+}
+
+cudaError_t launch_kv_attend(const KvAttendParams &p, const KvMaps &maps, int dtype, int head_dim, bool chosen, int sm_count, cudaStream_t s) {
+    if (p.tokens == 0 || p.batch.sequences == 0) return cudaSuccess;
+    auto go = [&](auto t, auto d) {
+        using T = decltype(t);
+        constexpr int D = decltype(d)::value;
+        return chosen ? launch<T, D, true>(p, maps, sm_count, s) : launch<T, D, false>(p, maps, sm_count, s);
+    };
+    using D64 = std::integral_constant<int, 64>;
+    using D128 = std::integral_constant<int, 128>;
+    if (dtype == TV_KV_BF16) return head_dim == 128 ? go(__nv_bfloat16(), D128()) : go(__nv_bfloat16(), D64());
+    return head_dim == 128 ? go(__half(), D128()) : go(__half(), D64());
+}
+
+}  // namespace tv

@@ -1,0 +1,286 @@
+"""Paged key/value cache on one GPU: appending keys and values with their position rotation, attention for a batch that may share
+a long prefix, and attention over pages that a cheap score selects (tv_kv_* of include/turbovec_b200.h).
+
+    cache = PagedKVCache.empty(pages=4096, page_size=64, kv_heads=8, head_dim=128, dtype=torch.bfloat16, device="cuda:0")
+    batch = KVBatch(table, lens, offsets)            # int32 tensors; lens counts the tokens of the call
+    q = cache.append(batch, k, v, q=q, cos=cos, sin=sin)
+    out = cache.attend(batch, q, prefix_pages=document_pages, prefix_len=30_000)
+    out, pages = cache.attend_selected(batch, q, budget=64, first=1, recent=4)
+
+Row t of a call is token j of sequence b, offsets[b] <= t < offsets[b + 1]; it stands at position lens[b] - (offsets[b + 1] -
+offsets[b]) + j of the sequence's own pages, table[b][position // page_size].  Rows behind the last sequence are left as they are.
+
+Everything runs on torch's current stream of the cache's device, without a synchronisation, and may be captured into a CUDA graph;
+results and workspaces come from torch's allocator.  Tensors are read when the kernels run: table, lens and offsets may be changed
+in place between calls, and a captured graph sees the new values.  There is no CPU path.
+"""
+from __future__ import annotations
+
+import ctypes as C
+
+import torch
+
+from . import _native
+
+__all__ = ["PagedKVCache", "KVBatch"]
+
+_DTYPES = {torch.bfloat16: 0, torch.float16: 1}
+_ref = C.byref
+
+
+def _fail(lib, rc: int):
+    msg = lib.tv_last_error(None).decode()
+    raise (ValueError if rc == 90 else RuntimeError)(msg)
+
+
+def _tensor(name: str, t, dtype, ndim: int, device=None) -> torch.Tensor:
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name} must be a torch tensor, got {type(t).__name__}")
+    if t.dtype != dtype:
+        raise TypeError(f"{name} must be of {dtype}, got {t.dtype}")
+    if t.dim() != ndim:
+        raise ValueError(f"{name} must have {ndim} dimensions, got {t.dim()}")
+    if device is not None and t.device != device:
+        raise ValueError(f"{name} must be on {device}, got {t.device}")
+    return t
+
+
+def _last_adjacent(name: str, t: torch.Tensor) -> None:
+    if t.shape[-1] > 1 and t.stride(-1) != 1:
+        raise ValueError(f"{name}: the elements of the last dimension must be adjacent")
+
+
+class KVBatch:
+    """The sequences of a call: `table` int32 [sequences, width], page numbers of each; `lens` int32 [sequences], tokens in its own
+    pages, those of the call among them; `offsets` int32 [sequences + 1], first row of each (None: one row each).  The tensors
+    are kept and read when the kernels run."""
+
+    def __init__(self, table: torch.Tensor, lens: torch.Tensor, offsets: torch.Tensor | None = None):
+        _tensor("lens", lens, torch.int32, 1)
+        if not lens.is_contiguous():
+            raise ValueError("lens must be contiguous")
+        self.device = lens.device
+        n = lens.numel()
+        _tensor("table", table, torch.int32, 2, self.device)
+        if table.shape[0] != n:
+            raise ValueError(f"table must have a row for each of the {n} sequences, got {table.shape[0]}")
+        _last_adjacent("table", table)
+        if offsets is None:
+            offsets = torch.arange(n + 1, dtype=torch.int32, device=self.device)
+        _tensor("offsets", offsets, torch.int32, 1, self.device)
+        if offsets.numel() != n + 1 or not offsets.is_contiguous():
+            raise ValueError(f"offsets must hold {n + 1} adjacent numbers, got {offsets.numel()}")
+        self.table, self.lens, self.offsets = table, lens, offsets
+        width = table.shape[1]
+        stride = table.stride(0) if n > 1 else width
+        if stride < width:
+            raise ValueError("the rows of table must not overlap")
+        self._view = _native.KvBatchView(n, width, stride, table.data_ptr(), lens.data_ptr(), offsets.data_ptr())
+
+    def __len__(self) -> int:
+        return self.lens.numel()
+
+
+class PagedKVCache:
+    """A pool of pages over tensors that the caller owns: k and v [pages, kv_heads, page_size, head_dim] with any strides but adjacent
+    channels (a pool laid out [pages, page_size, kv_heads, head_dim] is passed as its transpose(1, 2)), bfloat16 or float16, head_dim
+    64 or 128, page_size 16, 32, 64 or 128.  bounds int8 [pages, kv_heads, 2, head_dim] and scales float32 [pages, kv_heads] hold
+    the lowest and highest key of every channel of a page, as multiples of scales; both None where no pages are selected by score."""
+
+    def __init__(self, k: torch.Tensor, v: torch.Tensor, bounds: torch.Tensor | None = None, scales: torch.Tensor | None = None):
+        if not isinstance(k, torch.Tensor):
+            raise TypeError(f"k must be a torch tensor, got {type(k).__name__}")
+        if k.dtype not in _DTYPES:
+            raise TypeError(f"k must be of bfloat16 or float16, got {k.dtype}")
+        _tensor("k", k, k.dtype, 4)
+        _tensor("v", v, k.dtype, 4, k.device)
+        if k.shape != v.shape:
+            raise ValueError("k and v must have the same shape")
+        _last_adjacent("k", k)
+        _last_adjacent("v", v)
+        pages, heads, page_size, dim = k.shape
+        if dim not in (64, 128):
+            raise ValueError(f"head_dim must be 64 or 128, got {dim}")
+        if page_size not in (16, 32, 64, 128):
+            raise ValueError(f"page_size must be 16, 32, 64 or 128, got {page_size}")
+        if pages < 1 or heads < 1:
+            raise ValueError("the pool must have at least one page and one key head")
+        if (bounds is None) != (scales is None):
+            raise ValueError("bounds and scales must be given together")
+        if bounds is not None:
+            _tensor("bounds", bounds, torch.int8, 4, k.device)
+            _tensor("scales", scales, torch.float32, 2, k.device)
+            if tuple(bounds.shape) != (pages, heads, 2, dim) or not bounds.is_contiguous():
+                raise ValueError(f"bounds must be contiguous with shape {(pages, heads, 2, dim)}, got {tuple(bounds.shape)}")
+            if tuple(scales.shape) != (pages, heads) or not scales.is_contiguous():
+                raise ValueError(f"scales must be contiguous with shape {(pages, heads)}, got {tuple(scales.shape)}")
+        self._lib = _native.load()
+        if k.device.type != "cuda":
+            raise RuntimeError("turbovec_b200 has no CPU path: the cache must be in the memory of a CUDA device")
+        self.k, self.v, self.bounds, self.scales = k, v, bounds, scales
+        self.device, self.dtype = k.device, k.dtype
+        self.pages, self.kv_heads, self.page_size, self.head_dim = pages, heads, page_size, dim
+
+        def stride(t, i, natural):                      # of a dimension of one, whatever it says
+            return t.stride(i) if t.shape[i] > 1 else natural
+        sk = [stride(k, i, heads * page_size * dim) for i in range(3)]
+        sv = [stride(v, i, heads * page_size * dim) for i in range(3)]
+        self._view = _native.KvCacheView(
+            k.device.index, _DTYPES[k.dtype], dim, heads, page_size, pages, k.data_ptr(), v.data_ptr(), *sk, *sv,
+            bounds.data_ptr() if bounds is not None else None, scales.data_ptr() if scales is not None else None)
+        for name, strides, t in (("k", sk, k), ("v", sv, v)):
+            if any(s <= 0 or s % 8 for s in strides) or t.data_ptr() % 16:
+                raise ValueError(f"{name}: strides must be positive multiples of 8 elements, and the tensor 16-byte aligned")
+
+    @classmethod
+    def empty(cls, pages: int, page_size: int, kv_heads: int, head_dim: int, *, dtype=torch.bfloat16, device="cuda", bounds: bool = True):
+        """A pool of its own, contiguous, without contents; bounds=False leaves out what attend_selected needs."""
+        shape = (pages, kv_heads, page_size, head_dim)
+        k, v = torch.zeros(shape, dtype=dtype, device=device), torch.zeros(shape, dtype=dtype, device=device)
+        b = torch.zeros(pages, kv_heads, 2, head_dim, dtype=torch.int8, device=device) if bounds else None
+        s = torch.full((pages, kv_heads), 2.0 ** -24, dtype=torch.float32, device=device) if bounds else None
+        return cls(k, v, b, s)
+
+    # ---- helpers ----
+    def _rows(self, name: str, t, tokens: int | None, heads: int | None) -> _native.KvRowsView:
+        _tensor(name, t, self.dtype, 3, self.device)
+        n, h, d = t.shape
+        if d != self.head_dim:
+            raise ValueError(f"{name} must have {self.head_dim} channels, got {d}")
+        if (tokens is not None and n != tokens) or (heads is not None and h != heads):
+            raise ValueError(f"{name} must have {tokens if tokens is not None else n} rows of {heads if heads is not None else h} heads, got {n} of {h}")
+        st = t.stride()
+        if st[2] != 1:
+            raise ValueError(f"{name}: the elements of the last dimension must be adjacent")
+        return _native.KvRowsView(t.data_ptr(), st[0] if n > 1 else h * d, st[1] if h > 1 else d)
+
+    def _batch(self, batch) -> _native.KvBatchView:
+        if not isinstance(batch, KVBatch):
+            raise TypeError(f"batch must be a KVBatch, got {type(batch).__name__}")
+        if batch.device != self.device:
+            raise ValueError(f"batch must be on {self.device}, got {batch.device}")
+        return batch._view
+
+    def _query(self, q):
+        _tensor("q", q, self.dtype, 3, self.device)
+        heads = q.shape[1]
+        if heads < 1 or heads % self.kv_heads:
+            raise ValueError(f"the number of query heads must be a positive multiple of {self.kv_heads}, got {heads}")
+        return q.shape[0], heads
+
+    def _stream(self) -> int:
+        return torch.cuda.current_stream(self.device).cuda_stream
+
+    def _lse(self, lse, tokens: int, heads: int):
+        if lse is None:
+            return None
+        _tensor("lse", lse, torch.float32, 2, self.device)
+        if tuple(lse.shape) != (tokens, heads) or not lse.is_contiguous():
+            raise ValueError(f"lse must be contiguous with shape {(tokens, heads)}, got {tuple(lse.shape)}")
+        return lse.data_ptr()
+
+    def _workspace(self, n: int) -> torch.Tensor:
+        if n == 0:
+            _fail(self._lib, 90)
+        return torch.empty(n, dtype=torch.uint8, device=self.device)
+
+    # ---- operators ----
+    def append(self, batch: KVBatch, k: torch.Tensor, v: torch.Tensor, *, q: torch.Tensor | None = None, q_out: torch.Tensor | None = None,
+               cos: torch.Tensor | None = None, sin: torch.Tensor | None = None, interleaved: bool = False, position_offset: int = 0):
+        """Writes the rows of k and v [tokens, kv_heads, head_dim] into the pages of their sequences, keys rotated by the angles of
+        position + position_offset; rotates q [tokens, heads, head_dim] into q_out (a new tensor by default; q itself is allowed) and
+        returns it.  cos and sin: float32 [positions, rotary / 2], rotary a multiple of 16 up to head_dim; None: no rotation.  Pairs are
+        channels i and i + rotary / 2, or 2i and 2i + 1 where `interleaved`.  Tokens at positions below 0 or without an angle are left out."""
+        b = self._batch(batch)
+        kr = self._rows("k", k, None, self.kv_heads)
+        tokens = k.shape[0]
+        vr = self._rows("v", v, tokens, self.kv_heads)
+        heads, qr, qo = self.kv_heads, None, None
+        if q is not None:
+            n, heads = self._query(q)
+            qr = self._rows("q", q, tokens, heads)
+            if q_out is None:
+                q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
+            qo = self._rows("q_out", q_out, tokens, heads)
+        elif q_out is not None:
+            raise ValueError("q_out must not be given without q")
+        positions = rotary = 0
+        if (cos is None) != (sin is None):
+            raise ValueError("cos and sin must be given together")
+        if cos is not None:
+            _tensor("cos", cos, torch.float32, 2, self.device)
+            _tensor("sin", sin, torch.float32, 2, self.device)
+            if cos.shape != sin.shape or not cos.is_contiguous() or not sin.is_contiguous():
+                raise ValueError("cos and sin must be contiguous and have the same shape")
+            positions, rotary = cos.shape[0], 2 * cos.shape[1]
+        rc = self._lib.tv_kv_append(self._view, b, tokens, heads, kr, vr, qr, qo, cos.data_ptr() if positions else None,
+                                    sin.data_ptr() if positions else None, positions, rotary if positions else 0, int(bool(interleaved)),
+                                    int(position_offset), self._stream())
+        if rc:
+            _fail(self._lib, rc)
+        return q_out
+
+    def attend(self, batch: KVBatch, q: torch.Tensor, *, prefix_pages: torch.Tensor | None = None, prefix_len: int = 0,
+               scale: float | None = None, out: torch.Tensor | None = None, lse: torch.Tensor | None = None) -> torch.Tensor:
+        """Attention of the rows of q [tokens, heads, head_dim] over the first prefix_len keys of prefix_pages (int32 [n], read once for the
+        whole batch) and the keys of their own sequence up to their position.  Returns out (a new tensor by default); lse, where given,
+        receives the logarithm of each row's sum of exponentials.  scale: head_dim ** -0.5 by default.  Rows that see no key: zeros
+        and -inf."""
+        b = self._batch(batch)
+        tokens, heads = self._query(q)
+        qr = self._rows("q", q, tokens, heads)
+        if out is None:
+            out = torch.empty_like(q, memory_format=torch.contiguous_format)
+        orow = self._rows("out", out, tokens, heads)
+        width = 0
+        if prefix_pages is not None:
+            _tensor("prefix_pages", prefix_pages, torch.int32, 1, self.device)
+            if not prefix_pages.is_contiguous():
+                raise ValueError("prefix_pages must be contiguous")
+            width = prefix_pages.numel()
+        prefix_len = int(prefix_len)
+        if not 0 <= prefix_len <= width * self.page_size:
+            raise ValueError(f"prefix_len must be between 0 and the {width * self.page_size} tokens of prefix_pages, got {prefix_len}")
+        ws = self._workspace(self._lib.tv_kv_attend_workspace(self._view, b, tokens, heads, prefix_len)) if tokens and len(batch) else None
+        rc = self._lib.tv_kv_attend(self._view, b, tokens, heads, qr, prefix_pages.data_ptr() if prefix_len else None, width, prefix_len,
+                                    self.head_dim ** -0.5 if scale is None else float(scale), orow, self._lse(lse, tokens, heads),
+                                    ws.data_ptr() if ws is not None else None, ws.numel() if ws is not None else 0, self._stream())
+        if rc:
+            _fail(self._lib, rc)
+        return out
+
+    def attend_selected(self, batch: KVBatch, q: torch.Tensor, *, budget: int, first: int = 1, recent: int = 1, scale: float | None = None,
+                        out: torch.Tensor | None = None, lse: torch.Tensor | None = None, pages: torch.Tensor | None = None):
+        """Attention of every row over at most `budget` pages of its sequence: the `first` and the `recent` ones and the best of the others by
+        the bound of what their keys can score (include/turbovec_b200.h), chosen for each token and key head.  Returns (out, pages): the
+        chosen page numbers within the sequence, int32 [tokens, kv_heads, budget], ascending, then -1."""
+        if self.bounds is None:
+            raise ValueError("the cache has no bounds to choose pages by")
+        b = self._batch(batch)
+        tokens, heads = self._query(q)
+        qr = self._rows("q", q, tokens, heads)
+        budget, first, recent = int(budget), int(first), int(recent)
+        if budget < 1 or first < 0 or recent < 0 or first + recent > budget:
+            raise ValueError(f"budget must be positive and first + recent at most budget, got {budget}, {first} and {recent}")
+        if out is None:
+            out = torch.empty_like(q, memory_format=torch.contiguous_format)
+        orow = self._rows("out", out, tokens, heads)
+        if pages is None:
+            pages = torch.empty(tokens, self.kv_heads, budget, dtype=torch.int32, device=self.device)
+        _tensor("pages", pages, torch.int32, 3, self.device)
+        if tuple(pages.shape) != (tokens, self.kv_heads, budget) or not pages.is_contiguous():
+            raise ValueError(f"pages must be contiguous with shape {(tokens, self.kv_heads, budget)}, got {tuple(pages.shape)}")
+        ws = self._workspace(self._lib.tv_kv_attend_selected_workspace(self._view, b, tokens, heads, budget)) if tokens and len(batch) else None
+        rc = self._lib.tv_kv_attend_selected(self._view, b, tokens, heads, qr, budget, first, recent,
+                                             self.head_dim ** -0.5 if scale is None else float(scale), orow, self._lse(lse, tokens, heads),
+                                             pages.data_ptr(), ws.data_ptr() if ws is not None else None, ws.numel() if ws is not None else 0,
+                                             self._stream())
+        if rc:
+            _fail(self._lib, rc)
+        return out, pages
+
+    def check(self) -> None:
+        """Waits for the device and raises RuntimeError if a kernel of the cache gave up a wait since the last check."""
+        rc = self._lib.tv_kv_status(self.device.index)
+        if rc:
+            _fail(self._lib, rc)
