@@ -64,6 +64,12 @@ ATTEND = [
     (BF, 128, 32, 8, 2, [2, 1, 5], [40, 1, 90], 1000, True, 0),
     (FP, 128, 128, 14, 2, [1] * 11, list(range(1, 12)), 257, False, 0),
     (BF, 64, 64, 4, 1, [40], [50], 0, False, 0),                            # a piece of a prompt
+    (BF, 128, 64, 8, 1, [1] * 4, [3] * 4, 128, False, 0),                   # a prefix on the tensor cores: one tile of keys
+    (BF, 128, 64, 8, 2, [1] * 9, [5] * 9, 1111, False, 2),                  # 36 rows a key head
+    (FP, 64, 16, 16, 2, [1] * 16, [2] * 16, 129, True, 0),                  # 128 rows; one key in the second tile
+    (BF, 128, 128, 16, 2, [1] * 17, [2] * 17, 900, False, 0),               # 136: two row tiles
+    (FP, 128, 32, 10, 1, [1, 3, 2] * 9, [4] * 27, 5000, True, 1),           # 540 rows, three pairs
+    (BF, 64, 64, 24, 8, [2] * 50, [70] * 50, 2050, False, 0),               # 300 rows, eight key heads
 ]
 
 

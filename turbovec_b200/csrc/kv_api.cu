@@ -120,8 +120,21 @@ struct Carver {
         return p;
     }
 };
-size_t carve_attend(KvAttendParams &p, char *base, int64_t slots, int64_t rows, int head_dim, bool prefix) {
+// Rows (tokens x heads of a key head) from which a prefix goes to the tensor cores.
+constexpr int64_t kTensorRows = 17;
+void plan_prefix(KvAttendParams &p, const tv_kv_cache *c, int64_t tokens, int heads, int64_t prefix_len, int sm_count) {
+    const int64_t rows = tokens * (heads / c->kv_heads);
+    p.tensor_prefix = prefix_len > 0 && rows >= kTensorRows;
+    if (p.tensor_prefix) p.plan = kv_prefix_plan(rows, c->kv_heads, int(prefix_len), sm_count);
+}
+size_t carve_attend(KvAttendParams &p, char *base, int64_t slots, int64_t rows, const tv_kv_cache *c, bool prefix) {
     Carver w{base};
+    const int head_dim = c->head_dim;
+    if (p.tensor_prefix) {
+        const int64_t blocks = int64_t(c->kv_heads + p.plan.groups) * p.plan.units * 2;
+        p.pre_o = w.take<float>(blocks * kKvPrefixRows * head_dim);
+        p.pre_ml = w.take<float2>(blocks * kKvPrefixRows);
+    }
     p.part_o = w.take<float>(slots * kKvRows * head_dim);
     p.part_ml = w.take<float2>(slots * kKvRows);
     p.own_pieces = w.take<KvPieces>(rows);
@@ -129,8 +142,8 @@ size_t carve_attend(KvAttendParams &p, char *base, int64_t slots, int64_t rows, 
     p.slots = int(slots);
     return w.used;
 }
-size_t carve_chosen(KvAttendParams &p, KvSelectParams &q, char *base, int64_t slots, int64_t tokens, int64_t rows, int64_t lists, int head_dim) {
-    const size_t first = carve_attend(p, base, slots, rows, head_dim, false);
+size_t carve_chosen(KvAttendParams &p, KvSelectParams &q, char *base, int64_t slots, int64_t tokens, int64_t rows, int64_t lists, const tv_kv_cache *c) {
+    const size_t first = carve_attend(p, base, slots, rows, c, false);
     Carver w{base, first};
     q.chosen_pool = w.take<int32_t>(lists);
     q.token_pos = w.take<int32_t>(tokens);
@@ -211,8 +224,12 @@ int tv_kv_append(const tv_kv_cache *c, const tv_kv_batch *b, int64_t tokens, int
 
 size_t tv_kv_attend_workspace(const tv_kv_cache *c, const tv_kv_batch *b, int64_t tokens, int heads, int64_t prefix_len) {
     if (check_common(c, b, tokens, heads) != TV_OK) return 0;
+    const int sms = sm_count_of(c->device);
+    if (sms == 0) return 0;
     KvAttendParams p{};
-    return carve_attend(p, nullptr, attend_slots(c, b, tokens, heads, prefix_len > 0, sm_count_of(c->device)), tokens * heads, c->head_dim, prefix_len > 0);
+    plan_prefix(p, c, tokens, heads, prefix_len, sms);
+    const bool items = prefix_len > 0 && !p.tensor_prefix;
+    return carve_attend(p, nullptr, attend_slots(c, b, tokens, heads, items, sms), tokens * heads, c, items);
 }
 
 int tv_kv_attend(const tv_kv_cache *c, const tv_kv_batch *b, int64_t tokens, int heads, const tv_kv_rows *q, const int32_t *prefix_pages,
@@ -229,9 +246,11 @@ int tv_kv_attend(const tv_kv_cache *c, const tv_kv_batch *b, int64_t tokens, int
     if (rc != TV_OK) return rc;
     const int sms = sm_count_of(c->device);
     if (sms == 0) return set_create_error(TV_ERR_CUDA, "no such CUDA device");
-    const int64_t slots = attend_slots(c, b, tokens, heads, prefix_len > 0, sms);
+    plan_prefix(p, c, tokens, heads, prefix_len, sms);
+    const bool items = prefix_len > 0 && !p.tensor_prefix;
+    const int64_t slots = attend_slots(c, b, tokens, heads, items, sms);
     if (slots > INT_MAX) return unsupported("too many rows for one call");
-    rc = check_workspace(workspace, workspace_bytes, carve_attend(p, static_cast<char *>(workspace), slots, tokens * heads, c->head_dim, prefix_len > 0));
+    rc = check_workspace(workspace, workspace_bytes, carve_attend(p, static_cast<char *>(workspace), slots, tokens * heads, c, items));
     if (rc != TV_OK) return rc;
     p.prefix_pages = prefix_pages; p.prefix_len = int(prefix_len); p.prefix_width = int(prefix_width);
     DeviceScope scope(c->device);
@@ -239,7 +258,14 @@ int tv_kv_attend(const tv_kv_cache *c, const tv_kv_batch *b, int64_t tokens, int
     p.timeouts = kv_timeouts_symbol();
     KvMaps maps;
     if (!p.timeouts || !make_maps(&maps, c, c->page_size < kKvTile ? c->page_size : kKvTile)) return set_create_error(TV_ERR_CUDA, "the tensor maps of the cache cannot be made");
-    const cudaError_t e = launch_kv_attend(p, maps, c->dtype, c->head_dim, false, sms, static_cast<cudaStream_t>(stream));
+    cudaError_t e;
+    if (p.tensor_prefix) {
+        KvMaps wide;
+        if (!make_maps(&wide, c, c->page_size)) return set_create_error(TV_ERR_CUDA, "the tensor maps of the cache cannot be made");
+        e = launch_kv_prefix(p, wide, c->dtype, c->head_dim, static_cast<cudaStream_t>(stream));
+        if (e != cudaSuccess) return cuda_error("prefix kernel", e);
+    }
+    e = launch_kv_attend(p, maps, c->dtype, c->head_dim, false, sms, static_cast<cudaStream_t>(stream));
     return e == cudaSuccess ? int(TV_OK) : cuda_error("attention kernel", e);
 }
 
@@ -247,7 +273,7 @@ size_t tv_kv_attend_selected_workspace(const tv_kv_cache *c, const tv_kv_batch *
     if (check_common(c, b, tokens, heads) != TV_OK || budget < 1 || budget > kKvMaxScored) return 0;
     KvAttendParams p{};
     KvSelectParams s{};
-    return carve_chosen(p, s, nullptr, chosen_slots(c, tokens, heads, sm_count_of(c->device)), tokens, tokens * heads, tokens * c->kv_heads * budget, c->head_dim);
+    return carve_chosen(p, s, nullptr, chosen_slots(c, tokens, heads, sm_count_of(c->device)), tokens, tokens * heads, tokens * c->kv_heads * budget, c);
 }
 
 int tv_kv_attend_selected(const tv_kv_cache *c, const tv_kv_batch *b, int64_t tokens, int heads, const tv_kv_rows *q, int64_t budget, int64_t first,
@@ -270,7 +296,7 @@ int tv_kv_attend_selected(const tv_kv_cache *c, const tv_kv_batch *b, int64_t to
     const int64_t slots = chosen_slots(c, tokens, heads, sms);
     if (slots > INT_MAX) return unsupported("too many rows for one call");
     rc = check_workspace(workspace, workspace_bytes,
-                         carve_chosen(p, s, static_cast<char *>(workspace), slots, tokens, tokens * heads, tokens * c->kv_heads * budget, c->head_dim));
+                         carve_chosen(p, s, static_cast<char *>(workspace), slots, tokens, tokens * heads, tokens * c->kv_heads * budget, c));
     if (rc != TV_OK) return rc;
     s.batch = p.batch; s.q = p.q; s.bounds = c->bounds; s.scales = c->scales; s.chosen = pages_out;
     s.tokens = p.tokens; s.group = p.group; s.kv_heads = p.kv_heads; s.page_shift = p.page_shift; s.pages = p.pages;

@@ -136,7 +136,7 @@ __device__ __forceinline__ void set_up(Walk<CHOSEN> &w, int64_t *scratch, int64_
     } else {
         w.prefix_tiles = max(1, (p.prefix_len + kKvTile - 1) / kKvTile);
         w.prefix_mt = max(1, w.row_tiles(w.live));
-        w.prefix_total = p.prefix_len > 0 && w.live > 0 ? int64_t(w.prefix_mt) * p.kv_heads * w.prefix_tiles : 0;
+        w.prefix_total = p.prefix_len > 0 && !p.tensor_prefix && w.live > 0 ? int64_t(w.prefix_mt) * p.kv_heads * w.prefix_tiles : 0;
         // total cost of the sequences
         int64_t sum = 0;
         for (int i = threadIdx.x; i < p.batch.sequences; i += kAttendThreads) sum += w.cost(i);
@@ -220,7 +220,11 @@ __global__ void __launch_bounds__(kAttendThreads, 2) kv_attend_kernel(const KvAt
     Walk<CHOSEN> walk{p};
     int64_t per;
     set_up<CHOSEN>(walk, sh.scratch, per);
-    if (walk.at >= walk.end) return;
+    // a prefix kernel before this one must have ended when this one has: the join waits for this one alone
+    if (walk.at >= walk.end) {
+        if (!CHOSEN && p.tensor_prefix) asm volatile("griddepcontrol.wait;" ::: "memory");
+        return;
+    }
     Part w;
     uint32_t n = 0;                                     // tiles since the beginning: stage n % kStages, round n / kStages
 
@@ -276,6 +280,7 @@ __global__ void __launch_bounds__(kAttendThreads, 2) kv_attend_kernel(const KvAt
         }
         if (!ok)                                        // the copies in flight land before the block ends
             for (uint32_t i = n > G::kStages ? n - G::kStages : 0; i < n; ++i) mbar_wait(&sh.full[i % G::kStages], (i / G::kStages) & 1, p.timeouts);
+        if (!CHOSEN && p.tensor_prefix) asm volatile("griddepcontrol.wait;" ::: "memory");
         return;
     }
 
@@ -491,20 +496,19 @@ __global__ void __launch_bounds__(128) kv_join_kernel(const KvAttendParams p) {
     const KvSpan all = kv_span(p.batch.offsets[0], p.batch.offsets[p.batch.sequences], p.tokens);
     if (token < all.first || token >= all.first + all.count) return;       // behind the last sequence: as it was
     float big = -INFINITY, sum = 0.0f, acc[kPer] = {};
-    auto add = [&](const KvPieces &pc, int in_item) {
-        if (pc.first_slot < 0 || pc.count < 0 || int64_t(pc.first_slot) + pc.count > p.slots) return;
-        for (int i0 = 0; i0 < pc.count; i0 += 32) {
-            const int left = min(32, pc.count - i0);
-            const int64_t slot = pc.first_slot + i0;
-            const float2 ml = lane < left ? p.part_ml[(slot + lane) * kKvRows + in_item] : make_float2(-INFINITY, 0.0f);
+    // parts at o + i * step, (largest logit, sum) at ml + i * step / D
+    auto add = [&](const float *o, const float2 *ml_at, int64_t step, int count) {
+        for (int i0 = 0; i0 < count; i0 += 32) {
+            const int left = min(32, count - i0);
+            const float2 ml = lane < left ? ml_at[(i0 + lane) * (step / D)] : make_float2(-INFINITY, 0.0f);
             float top = ml.x;
 #pragma unroll
-            for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(kFullMask, top, o));
+            for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(kFullMask, top, d));
             const float next = fmaxf(big, top), base = next == -INFINITY ? 0.0f : next;
             const float old = kv_exp2(big - base), mine = kv_exp2(ml.x - base);
             float part = mine * ml.y;
 #pragma unroll
-            for (int o = 16; o > 0; o >>= 1) part += __shfl_xor_sync(kFullMask, part, o);
+            for (int d = 16; d > 0; d >>= 1) part += __shfl_xor_sync(kFullMask, part, d);
             sum = fmaf(sum, old, part);
             big = next;
 #pragma unroll
@@ -512,20 +516,41 @@ __global__ void __launch_bounds__(128) kv_join_kernel(const KvAttendParams p) {
 #pragma unroll 4
             for (int i = 0; i < left; ++i) {
                 const float f = __shfl_sync(kFullMask, mine, i);
-                const float *src = p.part_o + ((slot + i) * kKvRows + in_item) * D + lane * kPer;
-                float x[kPer];
-                if constexpr (kPer == 4) { const float4 y = *reinterpret_cast<const float4 *>(src); x[0] = y.x; x[1] = y.y; x[2] = y.z; x[3] = y.w; }
-                else { const float2 y = *reinterpret_cast<const float2 *>(src); x[0] = y.x; x[1] = y.y; }
+                const float *src = o + (i0 + i) * step + lane * kPer;
+                float x[kPer] = {};
+                if (f != 0.0f) {                     // a part without keys may have no sums
+                    if constexpr (kPer == 4) { const float4 y = *reinterpret_cast<const float4 *>(src); x[0] = y.x; x[1] = y.y; x[2] = y.z; x[3] = y.w; }
+                    else { const float2 y = *reinterpret_cast<const float2 *>(src); x[0] = y.x; x[1] = y.y; }
+                }
 #pragma unroll
                 for (int j = 0; j < kPer; ++j) acc[j] = fmaf(f, x[j], acc[j]);
             }
         }
     };
+    auto add_items = [&](const KvPieces &pc, int in_item) {
+        if (pc.first_slot < 0 || pc.count < 0 || int64_t(pc.first_slot) + pc.count > p.slots) return;
+        const int64_t at = int64_t(pc.first_slot) * kKvRows + in_item;
+        add(p.part_o + at * D, p.part_ml + at, int64_t(kKvRows) * D, pc.count);
+    };
     const KvPieces own = p.own_pieces[row];
     if (own.count == 0 && p.prefix_len == 0) return;
     // the row's place within its items: rows of a group lie together, token after token
     const int h = head / p.group, g = head - h * p.group;
-    if (p.prefix_len > 0) add(p.prefix_pieces[row], int((int64_t(token - all.first) * p.group + g) % kKvRows));
+    const int64_t r = int64_t(token - all.first) * p.group + g;
+    if (p.tensor_prefix) {
+        const KvPrefixPlan &w = p.plan;
+        const int first = int(int64_t(h) * w.tiles / w.per), count = int((int64_t(h + 1) * w.tiles - 1) / w.per) - first + 1;
+        const int64_t block = int64_t(kKvPrefixRows) * D;
+        if (w.paired) {
+            const int64_t at = ((int64_t(h) + first) * w.units + r / (2 * kKvPrefixRows)) * 2 * kKvPrefixRows + r % (2 * kKvPrefixRows);
+            add(p.pre_o + at * D, p.pre_ml + at, 2 * w.units * block, count);
+        } else {
+            const int64_t at = (int64_t(h) + first) * 2 * kKvPrefixRows + r;
+            add(p.pre_o + at * D, p.pre_ml + at, block, 2 * count);
+        }
+    } else if (p.prefix_len > 0) {
+        add_items(p.prefix_pieces[row], int(r % kKvRows));
+    }
     int from = 0;
     if (p.chosen == nullptr) {                       // first token of the row's sequence
         int lo = 0, hi = p.batch.sequences;
@@ -534,9 +559,9 @@ __global__ void __launch_bounds__(128) kv_join_kernel(const KvAttendParams p) {
             if (p.batch.offsets[mid] <= token) lo = mid; else hi = mid;
         }
         from = kv_span(p.batch.offsets[lo], p.batch.offsets[lo + 1], p.tokens).first;
-        add(own, int((int64_t(token - from) * p.group + g) % kKvRows));
+        add_items(own, int((int64_t(token - from) * p.group + g) % kKvRows));
     } else {
-        add(own, g % kKvRows);
+        add_items(own, g % kKvRows);
     }
     const float inv = sum > 0.0f || sum != sum ? 1.0f / sum : 0.0f;
     uint32_t *dst = reinterpret_cast<uint32_t *>(static_cast<T *>(p.out.data) + token * p.out.token_stride + head * p.out.head_stride + lane * kPer);
@@ -561,7 +586,7 @@ cudaError_t launch(const KvAttendParams &p, const KvMaps &maps, int sm_count, cu
     cfg.dynamicSmemBytes = smem;
     cfg.stream = s;
     cfg.attrs = &after;
-    cfg.numAttrs = CHOSEN ? 1 : 0;
+    cfg.numAttrs = CHOSEN || p.tensor_prefix ? 1 : 0;
     e = cudaLaunchKernelEx(&cfg, kern, p, maps);
     if (e != cudaSuccess) return e;
     cfg.gridDim = dim3(unsigned((int64_t(p.tokens) * p.heads + 3) / 4));

@@ -148,6 +148,28 @@ cudaError_t launch_kv_append(const KvAppendParams &p, int dtype, int head_dim, c
 struct KvPieces {
     int first_slot, count;                   // count 0: the row was written where it belongs
 };
+// Partial results of the tensor-memory form for a prefix (kv_prefix.cu): blocks of 128 rows.
+constexpr int kKvPrefixRows = 128;           // M of tcgen05.mma
+constexpr int kKvPrefixTile = 128;           // keys of one step
+struct KvPrefixPlan {                        // the same on host and device but for `live_rows`
+    bool paired;                             // two row tiles to a block, which share its keys; else one, its keys dealt to two streams
+    int units;                               // row tiles (or pairs) of a key head
+    int tiles;                               // key tiles
+    int groups;                              // blocks of one unit: they share the (key head, tile) list
+    int64_t per;                             // steps of a block
+};
+__host__ __device__ inline KvPrefixPlan kv_prefix_plan(int64_t rows, int kv_heads, int prefix_len, int sm_count) {
+    KvPrefixPlan w;
+    w.paired = rows > kKvPrefixRows;
+    w.units = int(w.paired ? (rows + 2 * kKvPrefixRows - 1) / (2 * kKvPrefixRows) : 1);
+    w.tiles = (prefix_len + kKvPrefixTile - 1) / kKvPrefixTile;
+    const int64_t steps = int64_t(kv_heads) * w.tiles;
+    int64_t groups = w.units < sm_count ? sm_count / w.units : 1;
+    if (groups > steps) groups = steps;
+    w.groups = int(groups);
+    w.per = (steps + groups - 1) / groups;
+    return w;
+}
 struct KvAttendParams {
     KvBatch batch;
     KvRows q, out;
@@ -167,6 +189,11 @@ struct KvAttendParams {
     KvPieces *own_pieces, *prefix_pieces;    // [token][head]
     int slots;
     uint32_t *timeouts;
+    // prefix by the tensor-memory form: its results instead of prefix items
+    bool tensor_prefix;
+    KvPrefixPlan plan;
+    float *pre_o;                            // [key head + group][unit][2][kKvPrefixRows][head_dim]
+    float2 *pre_ml;                          // [key head + group][unit][2][kKvPrefixRows]
 };
 struct KvMaps {
     CUtensorMap k, v;                        // (channel, token, key head, page), boxes of 64 channels
@@ -180,6 +207,8 @@ inline int64_t kv_attend_slots(int64_t tokens, int64_t sequences, int group, int
 inline int64_t kv_chosen_slots(int64_t tokens, int group, int kv_heads, int grid) { return tokens * ((group + kKvRows - 1) / kKvRows) * kv_heads + grid; }
 int kv_attend_grid(int sm_count);
 cudaError_t launch_kv_attend(const KvAttendParams &p, const KvMaps &maps, int dtype, int head_dim, bool chosen, int sm_count, cudaStream_t s);
+// The prefix by tcgen05 (kv_prefix.cu); launched before launch_kv_attend with the same parameters.
+cudaError_t launch_kv_prefix(const KvAttendParams &p, const KvMaps &maps, int dtype, int head_dim, cudaStream_t s);
 uint32_t *kv_timeouts_symbol();              // address on the current device, null if it cannot be had
 
 constexpr int kKvMaxScored = 49152;          // pages of a sequence whose scores fit a block's shared memory

@@ -1,0 +1,392 @@
+// Attention of many query rows over a shared prefix, on the tensor cores (tcgen05, accumulators in tensor memory).
+//
+// All rows of a batch (tokens x heads of a key head) see all keys of the prefix, so the prefix is read once for 256 rows instead of
+// once for every sequence.  S = Q K^T and O += P V are MMAs of 128 rows by 128 keys; four warps turn a tile of S into P, a row
+// to a thread: running maximum, weights in powers of two, their sum.  O is rescaled only when a row's maximum grows by more than
+// 2^8 (weights then stay below 2^8, which neither type nor the sums mind).  P replaces S in tensor memory and is the A operand
+// of the second MMA.
+//
+// Two streams of such tiles keep the tensor cores busy while the other's weights are computed.  With more than 128 rows the streams
+// are two row tiles that share each tile of keys and values; with fewer they are one row tile over every other tile of keys.
+// 128 channels: 256 columns of S and 256 of O fill tensor memory.
+//
+// Blocks of one unit of rows share the list of (key head, tile) steps evenly; the units of one group of blocks go over the same keys at
+// the same time, so that the second and later ones find them in L2.  A step is 2 * 128 * 128 * 128 * 2 multiply-adds = 2,048 cycles
+// of the tensor cores and as many of the exponential unit: that is what bounds it.
+#include "kv_cache.cuh"
+#include "scan_tc_common.cuh"
+
+namespace tv {
+namespace {
+
+constexpr int kPrefixThreads = 10 * 32;          // 2 x 4 warps of weights, one of MMAs, one of copies
+constexpr int kMmaWarp = 8, kCopyWarp = 9;
+constexpr float kRescaleAt = 8.0f;
+
+template <int D>
+struct PrefixGeometry {
+    static constexpr int kHalfBytes = 128 * 128;                 // 128 rows of 64 channels
+    static constexpr int kTileBytes = kHalfBytes * (D / 64);
+    static constexpr int kSlots = D == 128 ? 5 : 8;              // tiles of keys or values in the ring
+    static constexpr int kQBytes = 2 * kTileBytes;
+    static constexpr int kOColumns = D;
+};
+template <int D>
+struct PrefixShared {
+    uint64_t full[PrefixGeometry<D>::kSlots], empty[PrefixGeometry<D>::kSlots];
+    uint64_t s_full[2], p_ready[2], o_done[2], q_ready;
+    uint32_t tmem_base;
+};
+
+__device__ __forceinline__ void tma_load_page(void *dst, const CUtensorMap *map, int channel, int token, int head, int page, uint64_t *bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];"
+        ::"r"(smem_u32(dst)), "l"(map), "r"(smem_u32(bar)), "r"(channel), "r"(token), "r"(head), "r"(page) : "memory");
+}
+// 128-byte swizzle, channels (values) or keys... of a row adjacent: the MMA's other dimension is the one that is adjacent in
+// memory.  64 adjacent elements by 8 rows are 1,024 bytes; further rows 1,024 apart, further 64 elements `next` bytes apart.
+__device__ __forceinline__ uint64_t desc_mn(uint32_t addr, uint32_t next) {
+    return umma_desc(addr) & ~(uint64_t(0x3fff) << 16) | uint64_t(next >> 4) << 16;
+}
+template <typename T>
+constexpr uint32_t idesc(int n, bool b_adjacent) {
+    return (1u << 4) | (std::is_same<T, __nv_bfloat16>::value ? (1u << 7) | (1u << 10) : 0u) | (b_adjacent ? 1u << 16 : 0u) | (uint32_t(n >> 3) << 17) | (128u >> 4 << 24);
+}
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t id, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+        ::"r"(d), "l"(a), "l"(b), "r"(id), "r"(accumulate) : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t id, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+        ::"r"(d), "r"(a), "l"(b), "r"(id), "r"(accumulate) : "memory");
+}
+__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t *r) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31};"
+        ::"r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
+          "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]),
+          "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]),
+          "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31]), "r"(taddr) : "memory");
+}
+__device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void fence_shared_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+
+// a block's steps [at, end) of the (key head, tile) list, a part per key head
+struct PrefixPart {
+    int h, tile0, count;
+};
+__device__ __forceinline__ bool next_part(const KvPrefixPlan &plan, int64_t &at, int64_t end, PrefixPart &w) {
+    if (at >= end) return false;
+    w.h = int(at / plan.tiles);
+    w.tile0 = int(at - int64_t(w.h) * plan.tiles);
+    w.count = int(min(end - at, int64_t(plan.tiles - w.tile0)));
+    at += w.count;
+    return true;
+}
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kPrefixThreads, 1) kv_prefix_kernel(const KvAttendParams p, const __grid_constant__ KvMaps maps) {
+    using G = PrefixGeometry<D>;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t *q_smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    uint8_t *ring = q_smem + G::kQBytes;
+    PrefixShared<D> &sh = *reinterpret_cast<PrefixShared<D> *>(ring + G::kSlots * G::kTileBytes);
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const KvPrefixPlan plan = p.plan;
+    const int unit = blockIdx.x % plan.units, group = blockIdx.x / plan.units;
+    asm volatile("griddepcontrol.launch_dependents;");
+
+    if (tid == 0) {
+        for (int s = 0; s < G::kSlots; ++s) { mbar_init(&sh.full[s], 1); mbar_init(&sh.empty[s], 1); }
+        for (int s = 0; s < 2; ++s) { mbar_init(&sh.s_full[s], 1); mbar_init(&sh.p_ready[s], 4); mbar_init(&sh.o_done[s], 1); }
+        mbar_init(&sh.q_ready, 8);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == kMmaWarp) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sh.tmem_base)), "r"(512u) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    fence_before();
+    __syncthreads();
+    fence_after();
+    const uint32_t tmem = sh.tmem_base;
+    const int64_t steps = int64_t(p.kv_heads) * plan.tiles;
+    int64_t at = min(steps, group * plan.per);
+    const int64_t end = min(steps, at + plan.per);
+    const int lookahead = plan.paired ? 1 : 2;                   // tiles of keys whose logits are under way
+    PrefixPart w;
+    bool ok = true;
+
+    if (warp == kCopyWarp) {
+        // ---- tiles in the order of their use: the keys `lookahead` tiles ahead of the values
+        const int box = min(kKvPrefixTile, 1 << p.page_shift), boxes = kKvPrefixTile / box;
+        uint32_t n = 0;
+        auto load = [&](const PrefixPart &part, int i, const CUtensorMap *map) {
+            if (!ok) return;
+            const int s = n % G::kSlots;
+            const int64_t key = int64_t(part.tile0 + i) * kKvPrefixTile + lane * box;
+            const int64_t entry = key >> p.page_shift;
+            int page = -1;
+            if (lane < boxes && entry < p.prefix_width && key < p.prefix_len) page = __ldg(p.prefix_pages + entry);
+            const bool good = page >= 0 && page < p.pages;
+            if (!good) page = p.pages;                           // outside the pool: the copy fills with zeros
+            if (n >= G::kSlots) ok = mbar_wait(&sh.empty[s], ((n / G::kSlots) - 1) & 1, p.timeouts);
+            ok = __all_sync(kFullMask, ok);
+            if (!ok) return;
+            if (lane == 0) mbar_arrive_expect_tx(&sh.full[s], G::kTileBytes);
+            __syncwarp();
+            if (lane < boxes)
+#pragma unroll
+                for (int c = 0; c < D / 64; ++c)
+                    tma_load_page(ring + s * G::kTileBytes + c * G::kHalfBytes + lane * box * 128, map, c * 64, int(key & ((1 << p.page_shift) - 1)), part.h, page, &sh.full[s]);
+            ++n;
+        };
+        while (next_part(plan, at, end, w)) {
+            for (int i = 0; i < min(lookahead, w.count); ++i) load(w, i, &maps.k);
+            for (int i = 0; i < w.count; ++i) {
+                load(w, i, &maps.v);
+                if (i + lookahead < w.count) load(w, i + lookahead, &maps.k);
+            }
+        }
+        if (!ok)                                                 // the copies in flight land before the block ends
+            for (uint32_t i = n > G::kSlots ? n - G::kSlots : 0; i < n; ++i) mbar_wait(&sh.full[i % G::kSlots], (i / G::kSlots) & 1, p.timeouts);
+    } else if (warp == kMmaWarp) {
+        uint32_t n = 0, parts = 0, p_count[2] = {0, 0};
+        constexpr uint32_t kIdS = idesc<T>(128, false), kIdO = idesc<T>(D, true);
+        const uint32_t ring_addr = smem_u32(ring), q_addr = smem_u32(q_smem);
+        auto wait = [&](uint64_t *bar, uint32_t parity) {
+            if (ok) ok = mbar_wait(bar, parity, p.timeouts);
+        };
+        auto logits = [&](int s, uint32_t k_addr) {              // S_s = Q_s K^T
+            if (lane == 0) {
+                const uint32_t a = q_addr + (plan.paired ? s * G::kTileBytes : 0);
+#pragma unroll
+                for (int i = 0; i < D / 16; ++i) {
+                    const uint32_t off = (i >> 2) * G::kHalfBytes + (i & 3) * 32;
+                    mma_ss(tmem + 128 * s, umma_desc(a + off), umma_desc(k_addr + off), kIdS, i > 0);
+                }
+                umma_commit(&sh.s_full[s]);
+            }
+            __syncwarp();
+        };
+        auto sums = [&](int s, uint32_t v_addr, bool first) {    // O_s += P_s V
+            if (lane == 0) {
+#pragma unroll
+                for (int i = 0; i < kKvPrefixTile / 16; ++i)
+                    mma_ts(tmem + 256 + G::kOColumns * s, tmem + 128 * s + 8 * i, desc_mn(v_addr + i * 2048, G::kHalfBytes), kIdO, !first || i > 0);
+                umma_commit(&sh.o_done[s]);
+            }
+            __syncwarp();
+        };
+        auto release = [&](uint32_t slot) {
+            if (lane == 0) umma_commit(&sh.empty[slot]);
+            __syncwarp();
+        };
+        auto next_tile = [&](uint32_t &slot) {                   // waits for the next tile of the ring
+            slot = n % G::kSlots;
+            wait(&sh.full[slot], (n / G::kSlots) & 1);
+            fence_after();
+            ++n;
+            return ring_addr + slot * G::kTileBytes;
+        };
+        while (next_part(plan, at, end, w)) {
+            wait(&sh.q_ready, parts & 1);
+            fence_after();
+            ++parts;
+            uint32_t slot;
+            auto begin = [&](int i) {                            // logits of tile i
+                const uint32_t k_addr = next_tile(slot);
+                if (plan.paired) { logits(0, k_addr); logits(1, k_addr); }
+                else logits(i & 1, k_addr);
+                release(slot);
+            };
+            for (int i = 0; i < min(lookahead, w.count); ++i) begin(i);
+            for (int i = 0; i < w.count; ++i) {
+                uint32_t v_slot;
+                const uint32_t v_addr = next_tile(v_slot);
+                const int64_t left = int64_t(p.prefix_len) - int64_t(w.tile0 + i) * kKvPrefixTile;
+                if (left < kKvPrefixTile) {                      // places behind the prefix may hold anything, and 0 * NaN is not 0
+                    uint8_t *v = ring + v_slot * G::kTileBytes;
+                    for (int row = int(left); row < kKvPrefixTile; ++row)
+                        if (lane < D / 8) *reinterpret_cast<uint4 *>(v + (lane >> 3) * G::kHalfBytes + row * 128 + (lane & 7) * 16) = make_uint4(0, 0, 0, 0);
+                    fence_shared_async();
+                    __syncwarp();
+                }
+                if (plan.paired) {
+                    uint32_t k_slot = 0, k_addr = 0;
+                    const bool more = i + 1 < w.count;
+#pragma unroll
+                    for (int s = 0; s < 2; ++s) {
+                        wait(&sh.p_ready[s], p_count[s]++ & 1);
+                        fence_after();
+                        sums(s, v_addr, i == 0);
+                        if (s == 1) release(v_slot);
+                        if (more) {
+                            if (s == 0) k_addr = next_tile(k_slot);
+                            logits(s, k_addr);
+                            if (s == 1) release(k_slot);
+                        }
+                    }
+                } else {
+                    const int s = i & 1;
+                    wait(&sh.p_ready[s], p_count[s]++ & 1);
+                    fence_after();
+                    sums(s, v_addr, i < 2);
+                    release(v_slot);
+                    if (i + 2 < w.count) begin(i + 2);
+                }
+            }
+        }
+    } else {
+        // ---- weights: stream `s`, a row to a thread
+        const int s = warp >> 2, r = (warp & 3) * 32 + lane;
+        const uint32_t quarter = uint32_t((warp & 3) * 32) << 16, s_addr = tmem + 128 * s + quarter, o_addr = tmem + 256 + G::kOColumns * s + quarter;
+        uint32_t s_count = 0, o_count = 0;
+        const KvSpan all = kv_span(p.batch.offsets[0], p.batch.offsets[p.batch.sequences], p.tokens);
+        const int64_t live = int64_t(all.count) * p.group;
+        const int64_t row_base = int64_t(unit) * (plan.paired ? 2 * kKvPrefixRows : kKvPrefixRows) + (plan.paired ? s * kKvPrefixRows : 0);
+        auto wait = [&](uint64_t *bar, uint32_t parity) {
+            if (ok) ok = mbar_wait(bar, parity, p.timeouts);
+        };
+        while (next_part(plan, at, end, w)) {
+            if (plan.paired || s == 0) {                         // this stream's rows of Q, swizzled as a copy would
+                uint8_t *dst = q_smem + s * G::kTileBytes;
+                for (int i = tid & 127; i < kKvPrefixRows * (D / 8); i += 128) {
+                    const int row = i / (D / 8), c = i % (D / 8);
+                    const int64_t at_row = row_base + row;
+                    uint4 x = make_uint4(0, 0, 0, 0);
+                    if (at_row < live)
+                        x = *reinterpret_cast<const uint4 *>(static_cast<const T *>(p.q.data) + (all.first + at_row / p.group) * p.q.token_stride +
+                                                             (int64_t(w.h) * p.group + at_row % p.group) * p.q.head_stride + 8 * c);
+                    *reinterpret_cast<uint4 *>(dst + (c >> 3) * G::kHalfBytes + row * 128 + (((c & 7) ^ (row & 7)) << 4)) = x;
+                }
+                fence_shared_async();
+            }
+            fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sh.q_ready);
+            float m = -INFINITY, l = 0.0f;
+            int done = 0;                                        // tiles of this stream so far
+            for (int i = plan.paired ? 0 : s; i < w.count; i += plan.paired ? 1 : 2, ++done) {
+                // pages outside the pool hold no keys
+                const int64_t tile_key = int64_t(w.tile0 + i) * kKvPrefixTile, left = int64_t(p.prefix_len) - tile_key;
+                const int64_t first = tile_key + 16 * (lane & 7), entry = first >> p.page_shift;
+                int page = -1;
+                if (first < p.prefix_len && entry < p.prefix_width) page = __ldg(p.prefix_pages + entry);
+                const uint32_t good = __ballot_sync(kFullMask, page >= 0 && page < p.pages) & 0xffu;
+                wait(&sh.s_full[s], s_count++ & 1);
+                fence_after();
+                uint32_t x[128];
+#pragma unroll
+                for (int c = 0; c < 4; ++c) tmem_ld32(s_addr + 32 * c, reinterpret_cast<uint32_t (&)[32]>(x[32 * c]));
+                tmem_wait_ld();
+                if (good != 0xffu || left < kKvPrefixTile) {
+#pragma unroll
+                    for (int c = 0; c < 128; ++c)
+                        if (c >= left || !((good >> (c >> 4)) & 1u)) x[c] = 0xff800000u;
+                }
+                float top = -INFINITY;
+                {
+                    float t4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                    for (int c = 0; c < 128; ++c) t4[c & 3] = fmaxf(t4[c & 3], __uint_as_float(x[c]));
+                    top = fmaxf(fmaxf(t4[0], t4[1]), fmaxf(t4[2], t4[3])) * p.scale_log2;
+                }
+                if (done == 0) {
+                    m = top;
+                } else if (__any_sync(kFullMask, top > m + kRescaleAt)) {
+                    const float next = fmaxf(m, top), f = next == -INFINITY ? 1.0f : kv_exp2(m - next);
+                    m = next;
+                    l *= f;
+                    wait(&sh.o_done[s], (o_count + done - 1) & 1);
+                    fence_after();
+#pragma unroll 1
+                    for (int c = 0; c < D; c += 32) {
+                        uint32_t y[32];
+                        tmem_ld32(o_addr + c, y);
+                        tmem_wait_ld();
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) y[j] = __float_as_uint(__uint_as_float(y[j]) * f);
+                        tmem_st32(o_addr + c, y);
+                    }
+                    tmem_wait_st();
+                }
+                const float base = m == -INFINITY ? 0.0f : m;
+                float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                uint32_t pk[64];
+#pragma unroll
+                for (int c = 0; c < 64; ++c) {
+                    const float a = kv_exp2(fmaf(__uint_as_float(x[2 * c]), p.scale_log2, -base)), b = kv_exp2(fmaf(__uint_as_float(x[2 * c + 1]), p.scale_log2, -base));
+                    part[(2 * c) & 3] += a;
+                    part[(2 * c + 1) & 3] += b;
+                    pk[c] = KvType<T>::pack(a, b);
+                }
+                l += (part[0] + part[1]) + (part[2] + part[3]);
+                tmem_st32(s_addr, pk);
+                tmem_st32(s_addr + 32, pk + 32);
+                tmem_wait_st();
+                fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&sh.p_ready[s]);
+            }
+            // ---- the part's result
+            const int64_t block = ((int64_t(w.h) + group) * plan.units + unit) * 2 + s;
+            const bool have = row_base + r < live;
+            if (done > 0) {
+                wait(&sh.o_done[s], (o_count + done - 1) & 1);
+                fence_after();
+                float *dst = p.pre_o + (block * kKvPrefixRows + r) * D;
+#pragma unroll 1
+                for (int c = 0; c < D; c += 32) {
+                    uint32_t y[32];
+                    tmem_ld32(o_addr + c, y);
+                    tmem_wait_ld();
+                    if (have)
+#pragma unroll
+                        for (int j = 0; j < 8; ++j)
+                            *reinterpret_cast<uint4 *>(dst + c + 4 * j) = make_uint4(y[4 * j], y[4 * j + 1], y[4 * j + 2], y[4 * j + 3]);
+                }
+            }
+            o_count += done;
+            if (have) p.pre_ml[block * kKvPrefixRows + r] = make_float2(m, l);
+        }
+    }
+
+    fence_before();
+    __syncthreads();
+    if (warp == kMmaWarp) {
+        fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
+    }
+}
+
+template <typename T, int D>
+cudaError_t launch(const KvAttendParams &p, const KvMaps &maps, cudaStream_t s) {
+    using G = PrefixGeometry<D>;
+    const size_t smem = G::kQBytes + size_t(G::kSlots) * G::kTileBytes + sizeof(PrefixShared<D>) + 1024;
+    static_assert(G::kQBytes + G::kSlots * G::kTileBytes + sizeof(PrefixShared<D>) + 1024 <= kBlockSharedBytes, "more shared memory than a block can have");
+    cudaError_t e = allow_dynamic_shared(kv_prefix_kernel<T, D>);
+    if (e != cudaSuccess) return e;
+    kv_prefix_kernel<T, D><<<unsigned(p.plan.units * p.plan.groups), kPrefixThreads, smem, s>>>(p, maps);
+    return cudaGetLastError();
+}
+
+}  // namespace
+
+cudaError_t launch_kv_prefix(const KvAttendParams &p, const KvMaps &maps, int dtype, int head_dim, cudaStream_t s) {
+    if (dtype == TV_KV_BF16) return head_dim == 128 ? launch<__nv_bfloat16, 128>(p, maps, s) : launch<__nv_bfloat16, 64>(p, maps, s);
+    return head_dim == 128 ? launch<__half, 128>(p, maps, s) : launch<__half, 64>(p, maps, s);
+}
+
+}  // namespace tv
