@@ -53,32 +53,42 @@ __device__ __forceinline__ Unit unit_of(int u, int rotary, int interleaved) {
     return {16 * u, 16 * u + 8, u < turned};
 }
 
+struct Run16 {
+    uint4 a, b;
+};
 template <typename T>
-__device__ __forceinline__ void unit_through(const T *src, T *dst, const Unit &un, int u, bool turn, int interleaved, const float *cos_row,
-                                             const float *sin_row, uint4 &ya, uint4 &yb) {
-    const uint4 a = *reinterpret_cast<const uint4 *>(src + un.a), b = *reinterpret_cast<const uint4 *>(src + un.b);
-    ya = a; yb = b;
-    if (turn && un.turned) {
-        float c[8], s[8];
-        const float4 *pc = reinterpret_cast<const float4 *>(cos_row + 8 * u), *ps = reinterpret_cast<const float4 *>(sin_row + 8 * u);
-        *reinterpret_cast<float4 *>(c) = pc[0]; *reinterpret_cast<float4 *>(c + 4) = pc[1];
-        *reinterpret_cast<float4 *>(s) = ps[0]; *reinterpret_cast<float4 *>(s + 4) = ps[1];
-        if (interleaved) rotate_pairs<T>(a, b, c, s, ya, yb);
-        else rotate8<T>(a, b, c, s, ya, yb);
-    }
-    *reinterpret_cast<uint4 *>(dst + un.a) = ya;
-    *reinterpret_cast<uint4 *>(dst + un.b) = yb;
+__device__ __forceinline__ Run16 load_unit(const T *src, const Unit &un) {
+    return {*reinterpret_cast<const uint4 *>(src + un.a), *reinterpret_cast<const uint4 *>(src + un.b)};
 }
+template <typename T>
+__device__ __forceinline__ void store_unit(T *dst, const Unit &un, const Run16 &x) {
+    *reinterpret_cast<uint4 *>(dst + un.a) = x.a;
+    *reinterpret_cast<uint4 *>(dst + un.b) = x.b;
+}
+template <typename T>
+__device__ __forceinline__ Run16 turn(const Run16 &x, const Unit &un, int interleaved, const float (&c)[8], const float (&s)[8]) {
+    if (!un.turned) return x;
+    Run16 y;
+    if (interleaved) rotate_pairs<T>(x.a, x.b, c, s, y.a, y.b);
+    else rotate8<T>(x.a, x.b, c, s, y.a, y.b);
+    return y;
+}
+// lowest / highest of two values each; a NaN is left out
+__device__ __forceinline__ uint32_t low2(uint32_t x, uint32_t y, __nv_bfloat16) { uint32_t d; asm("min.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(x), "r"(y)); return d; }
+__device__ __forceinline__ uint32_t high2(uint32_t x, uint32_t y, __nv_bfloat16) { uint32_t d; asm("max.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(x), "r"(y)); return d; }
+__device__ __forceinline__ uint32_t low2(uint32_t x, uint32_t y, __half) { uint32_t d; asm("min.f16x2 %0, %1, %2;" : "=r"(d) : "r"(x), "r"(y)); return d; }
+__device__ __forceinline__ uint32_t high2(uint32_t x, uint32_t y, __half) { uint32_t d; asm("max.f16x2 %0, %1, %2;" : "=r"(d) : "r"(x), "r"(y)); return d; }
 
-template <typename T, int D>
-__global__ void __launch_bounds__(kAppendThreads) kv_append_kernel(const KvAppendParams p) {
+// HEADS key heads to a block: whole warps each.
+template <typename T, int D, int HEADS>
+__global__ void __launch_bounds__(kAppendThreads, 4) kv_append_kernel(const KvAppendParams p) {
     constexpr int kUnits = D / 16;                          // threads of one row, 16 channels each
-    constexpr int kLanes = kAppendThreads / kUnits;         // rows at a time
     constexpr int kWarps = kAppendThreads / 32;
+    constexpr int kWarpsPerHead = kWarps / HEADS;
+    constexpr int kLanes = kWarpsPerHead * 32 / kUnits;     // tokens of a head at a time
     __shared__ int64_t scratch[kWarps + 2];
-    __shared__ float lows[kWarps][D], highs[kWarps][D];
-    __shared__ float tops[D / 32];
-    const int tid = threadIdx.x, h = blockIdx.y, page_size = 1 << p.page_shift;
+    __shared__ uint32_t lows[kWarps][D / 2], highs[kWarps][D / 2];   // pairs of channels
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, page_size = 1 << p.page_shift;
 
     int b;
     int64_t place;
@@ -101,112 +111,126 @@ __global__ void __launch_bounds__(kAppendThreads) kv_append_kernel(const KvAppen
     const bool stored = page >= 0 && page < p.pages;
     const int count = int(end - begin), row0 = sp.first + int(begin - from), at0 = int(begin - page_from);
     const int half = p.rotary >> 1;
-    // a position outside the tables has no angle: its token is neither stored nor rotated
-    auto angled = [&](int i) {
-        const int64_t a = begin + i + p.position_offset;
-        return p.rotary == 0 || (a >= 0 && a < p.positions);
-    };
-
-    const int u = tid % kUnits, lane_row = tid / kUnits;
+    const int h = blockIdx.y * HEADS + warp / kWarpsPerHead;
+    const int in_head = tid % (kWarpsPerHead * 32), u = in_head % kUnits;
     const Unit un = unit_of(u, p.rotary, p.interleaved);
-    float lo[16], hi[16];
+    uint32_t lo[8], hi[8];
 #pragma unroll
-    for (int i = 0; i < 16; ++i) { lo[i] = INFINITY; hi[i] = -INFINITY; }
-    if (stored) {
-        T *dst = reinterpret_cast<T *>(p.k) + page * p.k_page + int64_t(h) * p.k_head;
-        const T *src = static_cast<const T *>(p.k_new.data) + int64_t(h) * p.k_new.head_stride;
-        for (int i = lane_row; i < count; i += kLanes) {
-            if (!angled(i)) continue;
-            const int64_t a = (begin + i + p.position_offset) * half;
-            uint4 ya, yb;
-            unit_through<T>(src + int64_t(row0 + i) * p.k_new.token_stride, dst + int64_t(at0 + i) * p.k_token, un, u, true, p.interleaved, p.cos + a, p.sin + a, ya, yb);
-            const uint32_t *wa = reinterpret_cast<const uint32_t *>(&ya), *wb = reinterpret_cast<const uint32_t *>(&yb);
+    for (int i = 0; i < 8; ++i) { lo[i] = KvType<T>::pack(INFINITY, INFINITY); hi[i] = KvType<T>::pack(-INFINITY, -INFINITY); }
+    if (h < p.kv_heads) {
+        for (int i = in_head / kUnits; i < count; i += kLanes) {
+            // a position outside the tables has no angle: its token is neither stored nor rotated
+            const int64_t angle = begin + i + p.position_offset;
+            if (p.rotary > 0 && (angle < 0 || angle >= p.positions)) continue;
+            const int64_t row = row0 + i;
+            Run16 k, v;
+            if (stored) {
+                k = load_unit(static_cast<const T *>(p.k_new.data) + row * p.k_new.token_stride + int64_t(h) * p.k_new.head_stride, un);
+                v = load_unit(static_cast<const T *>(p.v_new.data) + row * p.v_new.token_stride + int64_t(h) * p.v_new.head_stride, un);
+            }
+            float c[8] = {}, s[8] = {};
+            if (un.turned) {
+                const float4 *pc = reinterpret_cast<const float4 *>(p.cos + angle * half + 8 * u), *ps = reinterpret_cast<const float4 *>(p.sin + angle * half + 8 * u);
+                *reinterpret_cast<float4 *>(c) = pc[0]; *reinterpret_cast<float4 *>(c + 4) = pc[1];
+                *reinterpret_cast<float4 *>(s) = ps[0]; *reinterpret_cast<float4 *>(s + 4) = ps[1];
+            }
+            if (stored) {
+                k = turn<T>(k, un, p.interleaved, c, s);
+                store_unit(reinterpret_cast<T *>(p.k) + page * p.k_page + int64_t(h) * p.k_head + int64_t(at0 + i) * p.k_token, un, k);
+                store_unit(reinterpret_cast<T *>(p.v) + page * p.v_page + int64_t(h) * p.v_head + int64_t(at0 + i) * p.v_token, un, v);
+                const uint32_t *w = reinterpret_cast<const uint32_t *>(&k);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {                    // fminf and fmaxf leave NaN out
-                const float2 x = KvType<T>::unpack(wa[j]), y = KvType<T>::unpack(wb[j]);
-                lo[2 * j] = fminf(lo[2 * j], x.x); hi[2 * j] = fmaxf(hi[2 * j], x.x);
-                lo[2 * j + 1] = fminf(lo[2 * j + 1], x.y); hi[2 * j + 1] = fmaxf(hi[2 * j + 1], x.y);
-                lo[8 + 2 * j] = fminf(lo[8 + 2 * j], y.x); hi[8 + 2 * j] = fmaxf(hi[8 + 2 * j], y.x);
-                lo[9 + 2 * j] = fminf(lo[9 + 2 * j], y.y); hi[9 + 2 * j] = fmaxf(hi[9 + 2 * j], y.y);
+                for (int j = 0; j < 8; ++j) { lo[j] = low2(lo[j], w[j], T()); hi[j] = high2(hi[j], w[j], T()); }
+            }
+            if (p.q.data) {                                  // two heads at a time, so that their loads overlap
+                const T *src = static_cast<const T *>(p.q.data) + row * p.q.token_stride + int64_t(h) * p.group * p.q.head_stride;
+                T *dst = static_cast<T *>(p.q_out.data) + row * p.q_out.token_stride + int64_t(h) * p.group * p.q_out.head_stride;
+                int g = 0;
+                for (; g + 1 < p.group; g += 2) {
+                    const Run16 x = load_unit(src + g * p.q.head_stride, un), y = load_unit(src + (g + 1) * p.q.head_stride, un);
+                    store_unit(dst + g * p.q_out.head_stride, un, turn<T>(x, un, p.interleaved, c, s));
+                    store_unit(dst + (g + 1) * p.q_out.head_stride, un, turn<T>(y, un, p.interleaved, c, s));
+                }
+                if (g < p.group) store_unit(dst + g * p.q_out.head_stride, un, turn<T>(load_unit(src + g * p.q.head_stride, un), un, p.interleaved, c, s));
             }
         }
     }
-    // values and queries: rows of the same shape, G + 1 to a token
-    const int per_token = (p.q.data ? p.group : 0) + 1;
-    for (int i = lane_row; i < count * per_token; i += kLanes) {
-        const int t = i / per_token, r = i - t * per_token;
-        if (!angled(t)) continue;
-        const int64_t row = row0 + t;
-        uint4 ya, yb;
-        if (r == 0) {
-            if (stored)
-                unit_through<T>(static_cast<const T *>(p.v_new.data) + row * p.v_new.token_stride + int64_t(h) * p.v_new.head_stride,
-                                reinterpret_cast<T *>(p.v) + page * p.v_page + int64_t(h) * p.v_head + int64_t(at0 + t) * p.v_token, un, u, false, 0, nullptr, nullptr, ya, yb);
-        } else {
-            const int64_t head = int64_t(h) * p.group + r - 1, a = (begin + t + p.position_offset) * half;
-            unit_through<T>(static_cast<const T *>(p.q.data) + row * p.q.token_stride + head * p.q.head_stride,
-                            static_cast<T *>(p.q_out.data) + row * p.q_out.token_stride + head * p.q_out.head_stride, un, u, true, p.interleaved, p.cos + a, p.sin + a, ya, yb);
-        }
-    }
     if (p.bounds == nullptr || !stored) return;
-    const int64_t at = page * p.kv_heads + h;
-    const bool widen = at0 > 0;                             // the page holds earlier keys
-    const float old_scale = widen ? p.scales[at] : 0.0f;    // before a barrier that comes before its new value
 
-    // lowest and highest new key of every channel: over the rows of a warp, then over the warps
+    // lowest and highest new key of every channel: over the rows of a warp, then over the head's warps
 #pragma unroll
     for (int o = kUnits; o < 32; o <<= 1)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            lo[i] = fminf(lo[i], __shfl_xor_sync(kFullMask, lo[i], o));
-            hi[i] = fmaxf(hi[i], __shfl_xor_sync(kFullMask, hi[i], o));
+        for (int i = 0; i < 8; ++i) {
+            lo[i] = low2(lo[i], __shfl_xor_sync(kFullMask, lo[i], o), T());
+            hi[i] = high2(hi[i], __shfl_xor_sync(kFullMask, hi[i], o), T());
         }
-    const int warp = tid >> 5, lane = tid & 31;
     if (lane < kUnits)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            const int ch = i < 8 ? un.a + i : un.b + i - 8;
-            lows[warp][ch] = lo[i];
-            highs[warp][ch] = hi[i];
+        for (int i = 0; i < 8; ++i) {
+            const int at = (i < 4 ? un.a : un.b) / 2 + (i & 3);
+            lows[warp][at] = lo[i];
+            highs[warp][at] = hi[i];
         }
     __syncthreads();
-    float low = INFINITY, high = -INFINITY;
-    if (tid < D) {
+    // one warp per head: a lane takes D / 64 pairs of channels
+    const int mine = blockIdx.y * HEADS + warp;
+    if (warp >= HEADS || mine >= p.kv_heads) return;
+    constexpr int kPairs = D / 64;
+    float2 low[kPairs], high[kPairs];
+    float top = 0.0f;
 #pragma unroll
-        for (int w = 0; w < kWarps; ++w) { low = fminf(low, lows[w][tid]); high = fmaxf(high, highs[w][tid]); }
-        float top = low > high ? 0.0f : fmaxf(fabsf(low), fabsf(high));
+    for (int j = 0; j < kPairs; ++j) {
+        uint32_t l = lows[warp * kWarpsPerHead][lane + 32 * j], g = highs[warp * kWarpsPerHead][lane + 32 * j];
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(kFullMask, top, o));
-        if (lane == 0) tops[warp] = top;
+        for (int w = 1; w < kWarpsPerHead; ++w) {
+            l = low2(l, lows[warp * kWarpsPerHead + w][lane + 32 * j], T());
+            g = high2(g, highs[warp * kWarpsPerHead + w][lane + 32 * j], T());
+        }
+        low[j] = KvType<T>::unpack(l);
+        high[j] = KvType<T>::unpack(g);
+        if (low[j].x <= high[j].x) top = fmaxf(top, fmaxf(fabsf(low[j].x), fabsf(high[j].x)));
+        if (low[j].y <= high[j].y) top = fmaxf(top, fmaxf(fabsf(low[j].y), fabsf(high[j].y)));
     }
-    __syncthreads();
-    if (tid >= D) return;
-    float top = tops[0];
 #pragma unroll
-    for (int w = 1; w < D / 32; ++w) top = fmaxf(top, tops[w]);
+    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(kFullMask, top, o));
+    const int64_t at = page * p.kv_heads + mine;
+    const bool widen = at0 > 0;                             // the page holds earlier keys
+    const float old_scale = widen ? p.scales[at] : 0.0f;
+    const float scale = fmaxf(kv_pow2(kv_exponent(top)), old_scale), ratio = old_scale / scale;
     int8_t *row = p.bounds + at * 2 * D;
-    const float scale = fmaxf(kv_pow2(kv_exponent(top)), old_scale);
-    const bool none = low > high;                           // no new key with a value in this channel
-    float qlo = none ? 127.0f : fminf(fmaxf(floorf(low / scale), -127.0f), 127.0f);
-    float qhi = none ? -127.0f : fminf(fmaxf(ceilf(high / scale), -127.0f), 127.0f);
-    if (widen) {
-        const float ratio = old_scale / scale;
-        qlo = fminf(qlo, floorf(float(row[tid]) * ratio));
-        qhi = fmaxf(qhi, ceilf(float(row[D + tid]) * ratio));
-    } else if (none) {
-        qlo = qhi = 0.0f;
+    auto low8 = [&](float x, float y, int8_t old) {         // x <= y unless no new key has a value in the channel
+        const float q = x > y ? 127.0f : fminf(fmaxf(floorf(x / scale), -127.0f), 127.0f);
+        return widen ? fminf(q, floorf(float(old) * ratio)) : x > y ? 0.0f : q;
+    };
+    auto high8 = [&](float x, float y, int8_t old) {
+        const float q = x > y ? -127.0f : fminf(fmaxf(ceilf(y / scale), -127.0f), 127.0f);
+        return widen ? fmaxf(q, ceilf(float(old) * ratio)) : x > y ? 0.0f : q;
+    };
+#pragma unroll
+    for (int j = 0; j < kPairs; ++j) {
+        char2 *pl = reinterpret_cast<char2 *>(row) + lane + 32 * j, *ph = reinterpret_cast<char2 *>(row + D) + lane + 32 * j;
+        const char2 ol = widen ? *pl : make_char2(0, 0), oh = widen ? *ph : make_char2(0, 0);
+        *pl = make_char2(int8_t(int(low8(low[j].x, high[j].x, ol.x))), int8_t(int(low8(low[j].y, high[j].y, ol.y))));
+        *ph = make_char2(int8_t(int(high8(low[j].x, high[j].x, oh.x))), int8_t(int(high8(low[j].y, high[j].y, oh.y))));
     }
-    row[tid] = int8_t(int(qlo));
-    row[D + tid] = int8_t(int(qhi));
-    if (tid == 0) p.scales[at] = scale;
+    __syncwarp();                                           // every lane has read the old scale
+    if (lane == 0) p.scales[at] = scale;
 }
 
 template <typename T, int D>
 cudaError_t launch(const KvAppendParams &p, cudaStream_t s) {
     // pages touched: at most one per token, and at most two partial ones beside the full ones of a sequence
     const int64_t most = (int64_t(p.tokens) >> p.page_shift) + 2 * int64_t(p.batch.sequences);
-    const int64_t blocks = most < p.tokens ? most : p.tokens;
-    kv_append_kernel<T, D><<<dim3(unsigned(blocks), unsigned(p.kv_heads)), kAppendThreads, 0, s>>>(p);
+    const unsigned blocks = unsigned(most < p.tokens ? most : p.tokens);
+    // a block with few tokens takes several heads, so that finding its page is not most of its work
+    const int64_t tokens_of_page = p.tokens / blocks;
+    const int heads = tokens_of_page >= 16 || p.kv_heads == 1 ? 1 : tokens_of_page >= 8 || p.kv_heads == 2 ? 2 : tokens_of_page >= 4 || p.kv_heads <= 4 ? 4 : 8;
+    const dim3 grid(blocks, unsigned((p.kv_heads + heads - 1) / heads));
+    if (heads == 1) kv_append_kernel<T, D, 1><<<grid, kAppendThreads, 0, s>>>(p);
+    else if (heads == 2) kv_append_kernel<T, D, 2><<<grid, kAppendThreads, 0, s>>>(p);
+    else if (heads == 4) kv_append_kernel<T, D, 4><<<grid, kAppendThreads, 0, s>>>(p);
+    else kv_append_kernel<T, D, 8><<<grid, kAppendThreads, 0, s>>>(p);
     return cudaGetLastError();
 }
 
