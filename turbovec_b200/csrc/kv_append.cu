@@ -81,7 +81,7 @@ __device__ __forceinline__ uint32_t high2(uint32_t x, uint32_t y, __half) { uint
 
 // HEADS key heads to a block: whole warps each.
 template <typename T, int D, int HEADS>
-__global__ void __launch_bounds__(kAppendThreads, 4) kv_append_kernel(const KvAppendParams p) {
+__global__ void __launch_bounds__(kAppendThreads, 3) kv_append_kernel(const KvAppendParams p) {
     constexpr int kUnits = D / 16;                          // threads of one row, 16 channels each
     constexpr int kWarps = kAppendThreads / 32;
     constexpr int kWarpsPerHead = kWarps / HEADS;
