@@ -307,7 +307,7 @@ int tv_kv_attend_selected(const tv_kv_cache *c, const tv_kv_batch *b, int64_t to
     p.timeouts = kv_timeouts_symbol();
     KvMaps maps;
     if (!p.timeouts || !make_maps(&maps, c, c->page_size < kKvTile ? c->page_size : kKvTile)) return set_create_error(TV_ERR_CUDA, "the tensor maps of the cache cannot be made");
-    cudaError_t e = launch_kv_select(s, c->dtype, c->head_dim, static_cast<cudaStream_t>(stream));
+    cudaError_t e = launch_kv_select(s, c->dtype, c->head_dim, sms, static_cast<cudaStream_t>(stream));
     if (e != cudaSuccess) return cuda_error("selection kernel", e);
     e = launch_kv_attend(p, maps, c->dtype, c->head_dim, true, sms, static_cast<cudaStream_t>(stream));
     return e == cudaSuccess ? int(TV_OK) : cuda_error("attention kernel", e);

@@ -183,6 +183,7 @@ struct KvAttendParams {
     const int32_t *chosen, *chosen_pool;
     const int32_t *token_pos;
     int budget;
+    int item_cost;                           // what an item costs beside its tiles, in tiles
     // partial results: unnormalised sums, and (largest logit, sum of weights) in powers of two
     float *part_o;                           // [slot][kKvRows][head_dim]
     float2 *part_ml;                         // [slot][kKvRows]
@@ -220,6 +221,6 @@ struct KvSelectParams {
     int32_t *chosen, *chosen_pool, *token_pos;
     int tokens, group, kv_heads, page_shift, pages, budget, first, recent;
 };
-cudaError_t launch_kv_select(const KvSelectParams &p, int dtype, int head_dim, cudaStream_t s);
+cudaError_t launch_kv_select(const KvSelectParams &p, int dtype, int head_dim, int sm_count, cudaStream_t s);
 
 }  // namespace tv

@@ -6,12 +6,14 @@
 // with (lo, hi), exact in whole numbers below 2^22, times powers of two (2^-24 to 2^40 each): no rounding anywhere, so the choice does not depend on the
 // order of any sum, and equal scores go to the lower page.
 //
-// A block takes one token and key head.  Scores: int8 MMAs, query heads on the M side, 8 pages on the N side; a lane's 16-byte
+// A cluster of blocks takes one token and key head: all of them score pages, into the shared memory of the first, which chooses.
+// Scores: int8 MMAs, query heads on the M side, 8 pages on the N side; a lane's 16-byte
 // loads of a page's bounds feed four register operands, with the queries' channels permuted to match.  Choice: the k-th largest
 // score digit by digit (four counts of 8 bits), then one pass that keeps the pages' order.
 #include <cfloat>
 
 #include "kv_cache.cuh"
+#include "scan_tc_common.cuh"
 
 namespace tv {
 namespace {
@@ -28,17 +30,27 @@ __device__ __forceinline__ void mma_s8(int (&d)[4], uint32_t a0, uint32_t a1, ui
                  : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
+__device__ __forceinline__ void store_cluster(uint32_t addr, uint32_t x) { asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(addr), "r"(x) : "memory"); }
+__device__ __forceinline__ uint32_t load_cluster(uint32_t addr) {
+    uint32_t x;
+    asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(x) : "r"(addr) : "memory");
+    return x;
+}
+
 template <typename T, int D>
-__global__ void __launch_bounds__(kSelectThreads) kv_select_kernel(const KvSelectParams p) {
+__global__ void __launch_bounds__(kSelectThreads, 2) kv_select_kernel(const KvSelectParams p, int blocks) {
     extern __shared__ uint32_t keys[];                    // scores in ascending order of their bits; 0: no such page in the pool
     __shared__ __align__(16) int8_t q8[kKvRows][2 * D];
     __shared__ float q_scale[kKvRows];
     __shared__ uint32_t counts[256];
     __shared__ uint32_t found[2];
     __shared__ uint32_t sums[kSelectWarps];
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, token = blockIdx.x, h = blockIdx.y;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, token = blockIdx.x / blocks, h = blockIdx.y;
+    const int rank = blocks > 1 ? int(cluster_ctarank()) : 0;              // clusters lie along x
 
     asm volatile("griddepcontrol.launch_dependents;");
+    if (blocks > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");   // this block has begun: others may write into it
+    auto others_begun = [&] { if (blocks > 1) asm volatile("barrier.cluster.wait.aligned;" ::: "memory"); };
     int b = 0;
     {
         int hi = p.batch.sequences;
@@ -48,11 +60,14 @@ __global__ void __launch_bounds__(kSelectThreads) kv_select_kernel(const KvSelec
         }
     }
     const KvSpan sp = kv_span(p.batch.offsets[b], p.batch.offsets[b + 1], p.tokens);
-    if (token < sp.first || token >= sp.first + sp.count) return;          // behind the last sequence
+    if (token < sp.first || token >= sp.first + sp.count) {                // behind the last sequence
+        others_begun();
+        return;
+    }
     const int64_t pos = int64_t(p.batch.lens[b]) - sp.count + (token - sp.first);
     const int seen = kv_visible(pos, kv_capacity(p.batch.table_width, p.page_shift));
     const int n = int((int64_t(seen) + (1 << p.page_shift) - 1) >> p.page_shift);
-    if (h == 0 && tid == 0) p.token_pos[token] = seen - 1;
+    if (h == 0 && rank == 0 && tid == 0) p.token_pos[token] = seen - 1;
     const int32_t *table = p.batch.table + int64_t(b) * p.batch.table_stride;
     int32_t *list = p.chosen + (int64_t(token) * p.kv_heads + h) * p.budget, *pool = p.chosen_pool + (int64_t(token) * p.kv_heads + h) * p.budget;
     auto put = [&](int at, int page) {
@@ -60,13 +75,21 @@ __global__ void __launch_bounds__(kSelectThreads) kv_select_kernel(const KvSelec
         pool[at] = page >= 0 ? table[page] : -1;
     };
     if (n <= p.budget) {
-        for (int i = tid; i < p.budget; i += kSelectThreads) put(i, i < n ? i : -1);
+        if (rank == 0)
+            for (int i = tid; i < p.budget; i += kSelectThreads) put(i, i < n ? i : -1);
+        others_begun();
         return;
     }
     const int begin = p.first, end = n - p.recent, want = p.budget - p.first - p.recent;
-    for (int i = tid; i < p.first; i += kSelectThreads) put(i, i);
-    for (int i = tid; i < p.recent; i += kSelectThreads) put(p.budget - p.recent + i, end + i);
-    if (want == 0) return;
+    if (rank == 0) {
+        for (int i = tid; i < p.first; i += kSelectThreads) put(i, i);
+        for (int i = tid; i < p.recent; i += kSelectThreads) put(p.budget - p.recent + i, end + i);
+    }
+    if (want == 0) {
+        others_begun();
+        return;
+    }
+    const uint32_t keys_at = blocks > 1 ? map_to_cta(smem_u32(keys), 0) : smem_u32(keys);
 
     for (int g0 = 0; g0 < p.group; g0 += kKvRows) {
         __syncthreads();
@@ -103,36 +126,60 @@ __global__ void __launch_bounds__(kSelectThreads) kv_select_kernel(const KvSelec
             a0[i] = *reinterpret_cast<const uint4 *>(&q8[r0][64 * i + 16 * c]);
             a1[i] = *reinterpret_cast<const uint4 *>(&q8[r0 + 8][64 * i + 16 * c]);
         }
-        for (int p0 = begin + warp * 8; p0 < end; p0 += kSelectWarps * 8) {
-            const int mine = p0 + r0;
-            const int page = mine < end ? table[mine] : -1;
-            const bool good = page >= 0 && page < p.pages;
-            const int64_t at = (good ? int64_t(page) : 0) * p.kv_heads + h;
-            const uint4 *row = reinterpret_cast<const uint4 *>(p.bounds + at * 2 * D) + c;
-            int d[4] = {0, 0, 0, 0};
+        if (g0 == 0) others_begun();
+        // two runs of 8 pages at a time: their loads overlap
+        constexpr int kRuns = 2;
+        const int step = kSelectWarps * 8 * blocks;
+        for (int p0 = begin + (rank * kSelectWarps + warp) * 8; p0 < end; p0 += kRuns * step) {
+            bool good[kRuns];
+            int64_t at[kRuns];
+            uint4 w[kRuns][D / 32];
 #pragma unroll
-            for (int i = 0; i < D / 32; ++i) {
-                const uint4 w = row[4 * i];
-                mma_s8(d, a0[i].x, a1[i].x, a0[i].y, a1[i].y, w.x, w.y);
-                mma_s8(d, a0[i].z, a1[i].z, a0[i].w, a1[i].w, w.z, w.w);
+            for (int k = 0; k < kRuns; ++k) {
+                const int mine = p0 + k * step + r0;
+                const int page = mine < end ? __ldg(table + mine) : -1;
+                good[k] = page >= 0 && page < p.pages;
+                at[k] = (good[k] ? int64_t(page) : 0) * p.kv_heads + h;
             }
-            float s0 = -FLT_MAX, s1 = -FLT_MAX;
-            if (have0) { s0 = float(d[0]) * f0; s1 = float(d[1]) * f0; }
-            if (have1) { s0 = fmaxf(s0, float(d[2]) * f1); s1 = fmaxf(s1, float(d[3]) * f1); }
+            float scale[kRuns];
 #pragma unroll
-            for (int o = 4; o < 32; o <<= 1) {
-                s0 = fmaxf(s0, __shfl_xor_sync(kFullMask, s0, o));
-                s1 = fmaxf(s1, __shfl_xor_sync(kFullMask, s1, o));
+            for (int k = 0; k < kRuns; ++k) {
+                const uint4 *row = reinterpret_cast<const uint4 *>(p.bounds + at[k] * 2 * D) + c;
+#pragma unroll
+                for (int i = 0; i < D / 32; ++i) w[k][i] = __ldg(row + 4 * i);
+                scale[k] = __ldg(p.scales + at[k]);
             }
-            // lanes 0 .. 3 hold pages 2 lane and 2 lane + 1; hand page r0 to lane 4 r0
-            const float from0 = __shfl_sync(kFullMask, s0, r0 >> 1), from1 = __shfl_sync(kFullMask, s1, r0 >> 1);
-            if (c == 0 && mine < end) {
-                const float score = ((r0 & 1) ? from1 : from0) * (good ? p.scales[at] : 0.0f);
-                uint32_t key = good ? max(ascending(score), 1u) : 0u;
-                if (g0 > 0) key = max(key, keys[mine - begin]);
-                keys[mine - begin] = key;
+#pragma unroll
+            for (int k = 0; k < kRuns; ++k) {
+                int d[4] = {0, 0, 0, 0};
+#pragma unroll
+                for (int i = 0; i < D / 32; ++i) {
+                    mma_s8(d, a0[i].x, a1[i].x, a0[i].y, a1[i].y, w[k][i].x, w[k][i].y);
+                    mma_s8(d, a0[i].z, a1[i].z, a0[i].w, a1[i].w, w[k][i].z, w[k][i].w);
+                }
+                float s0 = -FLT_MAX, s1 = -FLT_MAX;
+                if (have0) { s0 = float(d[0]) * f0; s1 = float(d[1]) * f0; }
+                if (have1) { s0 = fmaxf(s0, float(d[2]) * f1); s1 = fmaxf(s1, float(d[3]) * f1); }
+#pragma unroll
+                for (int o = 4; o < 32; o <<= 1) {
+                    s0 = fmaxf(s0, __shfl_xor_sync(kFullMask, s0, o));
+                    s1 = fmaxf(s1, __shfl_xor_sync(kFullMask, s1, o));
+                }
+                // lanes 0 .. 3 hold pages 2 lane and 2 lane + 1; hand page r0 to lane 4 r0
+                const float from0 = __shfl_sync(kFullMask, s0, r0 >> 1), from1 = __shfl_sync(kFullMask, s1, r0 >> 1);
+                const int mine = p0 + k * step + r0;
+                if (c == 0 && mine < end) {
+                    const uint32_t to = keys_at + 4 * (mine - begin);
+                    uint32_t key = good[k] ? max(ascending(((r0 & 1) ? from1 : from0) * scale[k]), 1u) : 0u;
+                    if (g0 > 0) key = max(key, load_cluster(to));          // this lane wrote it for the heads before
+                    store_cluster(to, key);
+                }
             }
         }
+    }
+    if (blocks > 1) {
+        cluster_sync_all();
+        if (rank > 0) return;
     }
     __syncthreads();
 
@@ -202,21 +249,34 @@ __global__ void __launch_bounds__(kSelectThreads) kv_select_kernel(const KvSelec
 }
 
 template <typename T, int D>
-cudaError_t launch(const KvSelectParams &p, cudaStream_t s) {
+cudaError_t launch(const KvSelectParams &p, int sm_count, cudaStream_t s) {
     constexpr int kStatic = 8 * 1024;
-    cudaError_t e = allow_dynamic_shared(kv_select_kernel<T, D>, kStatic);
+    auto *kern = kv_select_kernel<T, D>;
+    cudaError_t e = allow_dynamic_shared(kern, kStatic);
     if (e != cudaSuccess) return e;
-    const size_t smem = size_t(p.batch.table_width) * 4;
-    kv_select_kernel<T, D><<<dim3(unsigned(p.tokens), unsigned(p.kv_heads)), kSelectThreads, smem, s>>>(p);
-    return cudaGetLastError();
+    // as many blocks to a token and key head as the device holds at once (two to a multiprocessor), none with less than a round of pages
+    const int64_t items = int64_t(p.tokens) * p.kv_heads;
+    int blocks = 1;
+    while (blocks < 8 && items * blocks * 2 <= 2 * sm_count && blocks * kSelectWarps * 8 < p.batch.table_width) blocks *= 2;
+    cudaLaunchAttribute cluster;
+    cluster.id = cudaLaunchAttributeClusterDimension;
+    cluster.val.clusterDim.x = unsigned(blocks); cluster.val.clusterDim.y = 1; cluster.val.clusterDim.z = 1;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(unsigned(p.tokens) * unsigned(blocks), unsigned(p.kv_heads));
+    cfg.blockDim = dim3(kSelectThreads);
+    cfg.dynamicSmemBytes = size_t(p.batch.table_width) * 4;
+    cfg.stream = s;
+    cfg.attrs = &cluster;
+    cfg.numAttrs = blocks > 1 ? 1 : 0;
+    return cudaLaunchKernelEx(&cfg, kern, p, blocks);
 }
 
 }  // namespace
 
-cudaError_t launch_kv_select(const KvSelectParams &p, int dtype, int head_dim, cudaStream_t s) {
+cudaError_t launch_kv_select(const KvSelectParams &p, int dtype, int head_dim, int sm_count, cudaStream_t s) {
     if (p.tokens == 0 || p.batch.sequences == 0) return cudaSuccess;
-    if (dtype == TV_KV_BF16) return head_dim == 128 ? launch<__nv_bfloat16, 128>(p, s) : launch<__nv_bfloat16, 64>(p, s);
-    return head_dim == 128 ? launch<__half, 128>(p, s) : launch<__half, 64>(p, s);
+    if (dtype == TV_KV_BF16) return head_dim == 128 ? launch<__nv_bfloat16, 128>(p, sm_count, s) : launch<__nv_bfloat16, 64>(p, sm_count, s);
+    return head_dim == 128 ? launch<__half, 128>(p, sm_count, s) : launch<__half, 64>(p, sm_count, s);
 }
 
 }  // namespace tv
