@@ -173,6 +173,7 @@ int fill_attend(KvAttendParams &p, const tv_kv_cache *c, const tv_kv_batch *b, i
     p.page_shift = shift_of(c->page_size);
     p.pages = int(c->pages);
     p.scale_log2 = scale * 1.4426950408889634f;
+    p.item_cost = 3;
     return TV_OK;
 }
 int check_workspace(const void *ws, size_t have, size_t need) {

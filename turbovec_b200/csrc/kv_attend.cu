@@ -18,6 +18,7 @@ namespace {
 
 constexpr int kConsumers = 4;
 constexpr int kAttendThreads = (kConsumers + 1) * 32;
+constexpr int kLeastTiles = 3;                           // tiles of a run: joining more parts takes longer than these
 constexpr int kNothing = INT_MAX - kKvTile;              // first position of a group of keys that nobody sees
 
 __device__ uint32_t g_kv_timeouts;
@@ -38,13 +39,19 @@ struct AttendShared {
     uint64_t full[Geometry<D>::kStages], empty[Geometry<D>::kStages];
 };
 
-// A run of tiles of one item.
+// A run of tiles of one item.  In the list an item is p.item_cost places without tiles, which stand for what an item costs beside them
+// (its rows of Q, and joining the warps' results), and then its tiles.
 struct Part {
     int item, row0, rows;          // rows of the call's q: (token, head of the group) pairs row0 .. row0 + rows of `first_token` on
     int first_token, h, b;         // b = -1: prefix
     int tile0, tile1, item_tiles;  // tiles of this part, and of the item
-    int64_t item_start;            // the item's first tile in the whole list
+    int64_t item_start;            // place of the item's first tile in the whole list
 };
+
+// Quotient of two numbers that are not negative: a 64-bit division costs several times a 32-bit one.
+__device__ __forceinline__ int64_t divide(int64_t a, int64_t b) {
+    return ((a | b) >> 31) == 0 ? int64_t(uint32_t(a) / uint32_t(b)) : a / b;
+}
 
 // Walks the parts of a block's run [at, end) of the list.  Order of items: prefix by (key head, rows); then by (sequence, key head,
 // rows).  With chosen pages: by (token, key head, rows).
@@ -65,48 +72,54 @@ struct Walk {
     __device__ __forceinline__ int row_tiles(int count) const { return int((int64_t(count) * p.group + kKvRows - 1) / kKvRows); }
     __device__ __forceinline__ KvSpan span(int i) const { return kv_span(p.batch.offsets[i], p.batch.offsets[i + 1], p.tokens); }
     __device__ __forceinline__ int64_t cost(int i) const {
-        return int64_t(row_tiles(span(i).count)) * p.kv_heads * tiles_of(p.batch.lens[i]);
+        return int64_t(row_tiles(span(i).count)) * p.kv_heads * (p.item_cost + tiles_of(p.batch.lens[i]));
     }
     __device__ __forceinline__ int64_t items(int i) const { return int64_t(row_tiles(span(i).count)) * p.kv_heads; }
 
+    // the next part; false when the run is over
     __device__ __forceinline__ bool next(Part &out) {
-        if (at >= end) return false;
-        if constexpr (CHOSEN) {
-            const int per_item = (((p.budget << p.page_shift) + kKvTile - 1) / kKvTile), mt = row_tiles(1);
-            const int item = int(at / per_item), tile = int(at - int64_t(item) * per_item);
-            const int m = item % mt, th = item / mt;
-            out.item = item; out.b = 0;
-            out.h = th % p.kv_heads; out.first_token = live_first + th / p.kv_heads;
-            out.row0 = m * kKvRows; out.rows = min(kKvRows, p.group - out.row0);
-            out.tile0 = tile; out.item_tiles = per_item; out.item_start = at - tile;
-        } else if (at < prefix_total) {
-            const int item = int(at / prefix_tiles), tile = int(at - int64_t(item) * prefix_tiles);
-            const int m = item % prefix_mt;
-            out.item = item; out.b = -1; out.h = item / prefix_mt; out.first_token = live_first;
-            out.row0 = m * kKvRows; out.rows = min(int64_t(kKvRows), int64_t(live) * p.group - out.row0);
-            out.tile0 = tile; out.item_tiles = prefix_tiles; out.item_start = at - tile;
-        } else {
-            KvSpan sp = span(b);
-            int mt = row_tiles(sp.count), tiles = tiles_of(p.batch.lens[b]);
-            while (at - start_of_b >= int64_t(mt) * p.kv_heads * tiles) {
-                if (b + 1 >= p.batch.sequences) return false;
-                start_of_b += int64_t(mt) * p.kv_heads * tiles;
-                item_of_b += mt * p.kv_heads;
-                ++b;
-                sp = span(b); mt = row_tiles(sp.count); tiles = tiles_of(p.batch.lens[b]);
+        while (at < end) {
+            int64_t begin;                                  // the item's first place
+            if constexpr (CHOSEN) {
+                const int places = p.item_cost + chosen_tiles(), mt = row_tiles(1);
+                const int item = int(divide(at, places));
+                const int m = item % mt, th = item / mt;
+                begin = int64_t(item) * places;
+                out.item = item; out.b = 0; out.item_tiles = chosen_tiles();
+                out.h = th % p.kv_heads; out.first_token = live_first + th / p.kv_heads;
+                out.row0 = m * kKvRows; out.rows = min(kKvRows, p.group - out.row0);
+            } else if (at < prefix_total) {
+                const int places = p.item_cost + prefix_tiles, item = int(divide(at, places));
+                const int m = item % prefix_mt;
+                begin = int64_t(item) * places;
+                out.item = item; out.b = -1; out.h = item / prefix_mt; out.first_token = live_first; out.item_tiles = prefix_tiles;
+                out.row0 = m * kKvRows; out.rows = int(min(int64_t(kKvRows), int64_t(live) * p.group - out.row0));
+            } else {
+                KvSpan sp = span(b);
+                int mt = row_tiles(sp.count), places = p.item_cost + tiles_of(p.batch.lens[b]);
+                while (at - start_of_b >= int64_t(mt) * p.kv_heads * places) {
+                    if (b + 1 >= p.batch.sequences) return false;
+                    start_of_b += int64_t(mt) * p.kv_heads * places;
+                    item_of_b += mt * p.kv_heads;
+                    ++b;
+                    sp = span(b); mt = row_tiles(sp.count); places = p.item_cost + tiles_of(p.batch.lens[b]);
+                }
+                const int item = int(divide(at - start_of_b, places));
+                const int m = item % mt;
+                begin = start_of_b + int64_t(item) * places;
+                out.item = item_of_b + item; out.b = b; out.h = item / mt; out.first_token = sp.first; out.item_tiles = places - p.item_cost;
+                out.row0 = m * kKvRows; out.rows = int(min(int64_t(kKvRows), int64_t(sp.count) * p.group - out.row0));
             }
-            const int64_t place = at - start_of_b;
-            const int item = int(place / tiles), tile = int(place - int64_t(item) * tiles);
-            const int m = item % mt;
-            out.item = item_of_b + item; out.b = b; out.h = item / mt; out.first_token = sp.first;
-            out.row0 = m * kKvRows; out.rows = min(int64_t(kKvRows), int64_t(sp.count) * p.group - out.row0);
-            out.tile0 = tile; out.item_tiles = tiles; out.item_start = at - tile;
+            out.item_start = begin + p.item_cost;
+            const int64_t stop = min(end, out.item_start + out.item_tiles);
+            out.tile0 = int(max(at, out.item_start) - out.item_start);
+            out.tile1 = int(stop - out.item_start);
+            at = min(end, out.item_start + out.item_tiles);
+            if (out.tile1 > out.tile0) return true;         // else the run ended before the item's first tile
         }
-        const int64_t left = end - at;
-        out.tile1 = out.tile0 + int(left < out.item_tiles - out.tile0 ? left : out.item_tiles - out.tile0);
-        at += out.tile1 - out.tile0;
-        return true;
+        return false;
     }
+    __device__ __forceinline__ int chosen_tiles() const { return ((p.budget << p.page_shift) + kKvTile - 1) / kKvTile; }
     // keys that row `r` of the part sees: those before this position
     __device__ __forceinline__ int limit(const Part &w, int r) const {
         if constexpr (CHOSEN) return p.token_pos[w.first_token] + 1;
@@ -116,7 +129,10 @@ struct Walk {
     }
     // one past the last tile of the part that some row sees a key of
     __device__ __forceinline__ int last_tile(const Part &w) const {
-        if constexpr (CHOSEN) return w.tile1;
+        if constexpr (CHOSEN) {                              // the list is shorter where the sequence has fewer pages
+            const int64_t keys = (int64_t(p.token_pos[w.first_token]) >> p.page_shift) + 1 << p.page_shift;
+            return int(min(int64_t(w.tile1), (keys + kKvTile - 1) / kKvTile));
+        }
         return min(w.tile1, (limit(w, w.rows - 1) + kKvTile - 1) / kKvTile);
     }
 };
@@ -132,11 +148,11 @@ __device__ __forceinline__ void set_up(Walk<CHOSEN> &w, int64_t *scratch, int64_
     w.start_of_b = 0;
     if constexpr (CHOSEN) {
         w.prefix_total = 0; w.prefix_tiles = w.prefix_mt = 1;
-        total = int64_t(w.live) * p.kv_heads * w.row_tiles(1) * (((p.budget << p.page_shift) + kKvTile - 1) / kKvTile);
+        total = int64_t(w.live) * p.kv_heads * w.row_tiles(1) * (p.item_cost + w.chosen_tiles());
     } else {
         w.prefix_tiles = max(1, (p.prefix_len + kKvTile - 1) / kKvTile);
         w.prefix_mt = max(1, w.row_tiles(w.live));
-        w.prefix_total = p.prefix_len > 0 && !p.tensor_prefix && w.live > 0 ? int64_t(w.prefix_mt) * p.kv_heads * w.prefix_tiles : 0;
+        w.prefix_total = p.prefix_len > 0 && !p.tensor_prefix && w.live > 0 ? int64_t(w.prefix_mt) * p.kv_heads * (p.item_cost + w.prefix_tiles) : 0;
         // total cost of the sequences
         int64_t sum = 0;
         for (int i = threadIdx.x; i < p.batch.sequences; i += kAttendThreads) sum += w.cost(i);
@@ -150,7 +166,7 @@ __device__ __forceinline__ void set_up(Walk<CHOSEN> &w, int64_t *scratch, int64_
         w.item_of_b = w.prefix_total > 0 ? w.prefix_mt * p.kv_heads : 0;
         w.start_of_b = w.prefix_total;
     }
-    per = max(int64_t(1), (total + gridDim.x - 1) / gridDim.x);
+    per = max(int64_t(p.item_cost + kLeastTiles), divide(total + gridDim.x - 1, gridDim.x));
     w.at = min(total, int64_t(blockIdx.x) * per);
     w.end = min(total, w.at + per);
     if constexpr (!CHOSEN) {
@@ -212,6 +228,10 @@ __global__ void __launch_bounds__(kAttendThreads, 2) kv_attend_kernel(const KvAt
 
     asm volatile("griddepcontrol.launch_dependents;");
     if constexpr (CHOSEN) asm volatile("griddepcontrol.wait;" ::: "memory");
+    if (tid == kConsumers * 32) {
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&maps.k) : "memory");
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&maps.v) : "memory");
+    }
     if (tid == 0) {
         for (int s = 0; s < G::kStages; ++s) { mbar_init(&sh.full[s], 1); mbar_init(&sh.empty[s], kConsumers); }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -475,7 +495,7 @@ __global__ void __launch_bounds__(kAttendThreads, 2) kv_attend_kernel(const KvAt
                 if (c2 == 0) p.part_ml[slot * kKvRows + r] = make_float2(big, sum);
             }
             if (c2 == 0 && w.tile0 == 0) {                      // where the parts of the item lie, packed with the row within a slot
-                const int64_t begin = w.item_start / per, finish_at = (w.item_start + w.item_tiles - 1) / per;
+                const int64_t begin = divide(w.item_start, per), finish_at = divide(w.item_start + w.item_tiles - 1, per);
                 KvPieces pc{int(w.item + begin), whole ? 0 : int(finish_at - begin + 1)};
                 (w.b < 0 ? p.prefix_pieces : p.own_pieces)[token * p.heads + head] = pc;
             }
@@ -485,19 +505,27 @@ __global__ void __launch_bounds__(kAttendThreads, 2) kv_attend_kernel(const KvAt
     }
 }
 
-// Joins the parts of a row: one warp per (token, head).
-template <typename T, int D>
+// Joins the parts of a row (token, head): WARPS warps each take every WARPS-th part.
+template <typename T, int D, int WARPS>
 __global__ void __launch_bounds__(128) kv_join_kernel(const KvAttendParams p) {
     constexpr int kPer = D / 32;
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    const int lane = threadIdx.x & 31;
-    const int64_t row = int64_t(blockIdx.x) * 4 + (threadIdx.x >> 5);
+    __shared__ float4 others[WARPS > 1 ? WARPS - 1 : 1][32];
+    __shared__ float2 others_ml[WARPS > 1 ? WARPS - 1 : 1];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, turn = warp % WARPS;
+    const int64_t row = int64_t(blockIdx.x) * (4 / WARPS) + warp / WARPS;
     const int token = int(row / p.heads), head = int(row % p.heads);
     const KvSpan all = kv_span(p.batch.offsets[0], p.batch.offsets[p.batch.sequences], p.tokens);
     if (token < all.first || token >= all.first + all.count) return;       // behind the last sequence: as it was
     float big = -INFINITY, sum = 0.0f, acc[kPer] = {};
     // parts at o + i * step, (largest logit, sum) at ml + i * step / D
     auto add = [&](const float *o, const float2 *ml_at, int64_t step, int count) {
+        if (WARPS > 1) {                             // this warp's parts
+            o += turn * step;
+            ml_at += turn * (step / D);
+            step *= WARPS;
+            count = (count - turn + WARPS - 1) / WARPS;
+        }
         for (int i0 = 0; i0 < count; i0 += 32) {
             const int left = min(32, count - i0);
             const float2 ml = lane < left ? ml_at[(i0 + lane) * (step / D)] : make_float2(-INFINITY, 0.0f);
@@ -513,7 +541,7 @@ __global__ void __launch_bounds__(128) kv_join_kernel(const KvAttendParams p) {
             big = next;
 #pragma unroll
             for (int j = 0; j < kPer; ++j) acc[j] *= old;
-#pragma unroll 4
+#pragma unroll 8
             for (int i = 0; i < left; ++i) {
                 const float f = __shfl_sync(kFullMask, mine, i);
                 const float *src = o + (i0 + i) * step + lane * kPer;
@@ -563,6 +591,29 @@ __global__ void __launch_bounds__(128) kv_join_kernel(const KvAttendParams p) {
     } else {
         add_items(own, g % kKvRows);
     }
+    if constexpr (WARPS > 1) {
+        static_assert(WARPS == 4, "a block is one row");
+        if (turn > 0) {
+            float4 y = make_float4(acc[0], acc[1], 0.0f, 0.0f);
+            if constexpr (kPer == 4) { y.z = acc[2]; y.w = acc[3]; }
+            others[turn - 1][lane] = y;
+            if (lane == 0) others_ml[turn - 1] = make_float2(big, sum);
+        }
+        __syncthreads();
+        if (turn > 0) return;
+#pragma unroll
+        for (int i = 0; i < WARPS - 1; ++i) {
+            const float2 ml = others_ml[i];
+            const float4 y = others[i][lane];
+            const float next = fmaxf(big, ml.x), base = next == -INFINITY ? 0.0f : next;
+            const float old = kv_exp2(big - base), f = kv_exp2(ml.x - base);
+            const float x[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+            for (int j = 0; j < kPer; ++j) acc[j] = fmaf(f, x[j], acc[j] * old);
+            sum = fmaf(f, ml.y, sum * old);
+            big = next;
+        }
+    }
     const float inv = sum > 0.0f || sum != sum ? 1.0f / sum : 0.0f;
     uint32_t *dst = reinterpret_cast<uint32_t *>(static_cast<T *>(p.out.data) + token * p.out.token_stride + head * p.out.head_stride + lane * kPer);
 #pragma unroll
@@ -589,11 +640,14 @@ cudaError_t launch(const KvAttendParams &p, const KvMaps &maps, int sm_count, cu
     cfg.numAttrs = CHOSEN || p.tensor_prefix ? 1 : 0;
     e = cudaLaunchKernelEx(&cfg, kern, p, maps);
     if (e != cudaSuccess) return e;
-    cfg.gridDim = dim3(unsigned((int64_t(p.tokens) * p.heads + 3) / 4));
+    // few rows have many parts each
+    const int64_t rows = int64_t(p.tokens) * p.heads;
+    const bool few = rows <= 16 * sm_count;
+    cfg.gridDim = dim3(unsigned(few ? rows : (rows + 3) / 4));
     cfg.blockDim = dim3(128);
     cfg.dynamicSmemBytes = 0;
     cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, kv_join_kernel<T, D>, p);
+    return few ? cudaLaunchKernelEx(&cfg, kv_join_kernel<T, D, 4>, p) : cudaLaunchKernelEx(&cfg, kv_join_kernel<T, D, 1>, p);
 }
 
 }  // namespace
