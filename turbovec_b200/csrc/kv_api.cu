@@ -15,7 +15,6 @@ namespace {
 
 using namespace tv;
 
-constexpr int kMaxDevices = 64;
 constexpr int64_t kMaxCount = 1 << 30;                        // tokens, pages, places of a table: 32-bit indices with room
 
 // The caller's current device is put back when the call ends.
@@ -33,8 +32,8 @@ struct DeviceScope {
 };
 
 int sm_count_of(int device) {
-    static std::atomic<int> known[kMaxDevices];
-    if (device < 0 || device >= kMaxDevices) return 0;
+    static std::atomic<int> known[kKvMaxDevices];
+    if (device < 0 || device >= kKvMaxDevices) return 0;
     int n = known[device].load(std::memory_order_relaxed);
     if (n == 0) {
         if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, device) != cudaSuccess) { cudaGetLastError(); return 0; }
@@ -256,17 +255,17 @@ int tv_kv_attend(const tv_kv_cache *c, const tv_kv_batch *b, int64_t tokens, int
     p.prefix_pages = prefix_pages; p.prefix_len = int(prefix_len); p.prefix_width = int(prefix_width);
     DeviceScope scope(c->device);
     if (!scope.ok) return cuda_error("no such CUDA device", cudaGetLastError());
-    p.timeouts = kv_timeouts_symbol();
+    p.timeouts = kv_timeouts_symbol(c->device);
     KvMaps maps;
     if (!p.timeouts || !make_maps(&maps, c, c->page_size < kKvTile ? c->page_size : kKvTile)) return set_create_error(TV_ERR_CUDA, "the tensor maps of the cache cannot be made");
     cudaError_t e;
     if (p.tensor_prefix) {
         KvMaps wide;
         if (!make_maps(&wide, c, c->page_size)) return set_create_error(TV_ERR_CUDA, "the tensor maps of the cache cannot be made");
-        e = launch_kv_prefix(p, wide, c->dtype, c->head_dim, static_cast<cudaStream_t>(stream));
+        e = launch_kv_prefix(p, wide, c->dtype, c->head_dim, c->device, static_cast<cudaStream_t>(stream));
         if (e != cudaSuccess) return cuda_error("prefix kernel", e);
     }
-    e = launch_kv_attend(p, maps, c->dtype, c->head_dim, false, sms, static_cast<cudaStream_t>(stream));
+    e = launch_kv_attend(p, maps, c->dtype, c->head_dim, false, c->device, sms, static_cast<cudaStream_t>(stream));
     return e == cudaSuccess ? int(TV_OK) : cuda_error("attention kernel", e);
 }
 
@@ -305,19 +304,20 @@ int tv_kv_attend_selected(const tv_kv_cache *c, const tv_kv_batch *b, int64_t to
     p.chosen = pages_out; p.chosen_pool = s.chosen_pool; p.token_pos = s.token_pos; p.budget = int(budget);
     DeviceScope scope(c->device);
     if (!scope.ok) return cuda_error("no such CUDA device", cudaGetLastError());
-    p.timeouts = kv_timeouts_symbol();
+    p.timeouts = kv_timeouts_symbol(c->device);
     KvMaps maps;
     if (!p.timeouts || !make_maps(&maps, c, c->page_size < kKvTile ? c->page_size : kKvTile)) return set_create_error(TV_ERR_CUDA, "the tensor maps of the cache cannot be made");
-    cudaError_t e = launch_kv_select(s, c->dtype, c->head_dim, sms, static_cast<cudaStream_t>(stream));
+    cudaError_t e = launch_kv_select(s, c->dtype, c->head_dim, c->device, sms, static_cast<cudaStream_t>(stream));
     if (e != cudaSuccess) return cuda_error("selection kernel", e);
-    e = launch_kv_attend(p, maps, c->dtype, c->head_dim, true, sms, static_cast<cudaStream_t>(stream));
+    e = launch_kv_attend(p, maps, c->dtype, c->head_dim, true, c->device, sms, static_cast<cudaStream_t>(stream));
     return e == cudaSuccess ? int(TV_OK) : cuda_error("attention kernel", e);
 }
 
 int tv_kv_status(int device) {
+    if (device < 0 || device >= kKvMaxDevices) return set_create_error(TV_ERR_CUDA, "no such CUDA device");
     DeviceScope scope(device);
     if (!scope.ok) return cuda_error("no such CUDA device", cudaGetLastError());
-    uint32_t *flag = kv_timeouts_symbol(), value = 0;
+    uint32_t *flag = kv_timeouts_symbol(device), value = 0;
     cudaError_t e = flag ? cudaDeviceSynchronize() : cudaGetLastError();
     if (flag && e == cudaSuccess) e = cudaMemcpy(&value, flag, 4, cudaMemcpyDeviceToHost);
     if (flag && e == cudaSuccess && value) e = cudaMemset(flag, 0, 4);

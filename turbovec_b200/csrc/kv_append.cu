@@ -89,6 +89,8 @@ __global__ void __launch_bounds__(kAppendThreads, 3) kv_append_kernel(const KvAp
     __shared__ int64_t scratch[kWarps + 2];
     __shared__ uint32_t lows[kWarps][D / 2], highs[kWarps][D / 2];   // pairs of channels
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, page_size = 1 << p.page_shift;
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;");
 
     int b;
     int64_t place;
@@ -227,11 +229,10 @@ cudaError_t launch(const KvAppendParams &p, cudaStream_t s) {
     const int64_t tokens_of_page = p.tokens / blocks;
     const int heads = tokens_of_page >= 16 || p.kv_heads == 1 ? 1 : tokens_of_page >= 8 || p.kv_heads == 2 ? 2 : tokens_of_page >= 4 || p.kv_heads <= 4 ? 4 : 8;
     const dim3 grid(blocks, unsigned((p.kv_heads + heads - 1) / heads));
-    if (heads == 1) kv_append_kernel<T, D, 1><<<grid, kAppendThreads, 0, s>>>(p);
-    else if (heads == 2) kv_append_kernel<T, D, 2><<<grid, kAppendThreads, 0, s>>>(p);
-    else if (heads == 4) kv_append_kernel<T, D, 4><<<grid, kAppendThreads, 0, s>>>(p);
-    else kv_append_kernel<T, D, 8><<<grid, kAppendThreads, 0, s>>>(p);
-    return cudaGetLastError();
+    if (heads == 1) return kv_launch(kv_append_kernel<T, D, 1>, grid, kAppendThreads, 0, s, p);
+    if (heads == 2) return kv_launch(kv_append_kernel<T, D, 2>, grid, kAppendThreads, 0, s, p);
+    if (heads == 4) return kv_launch(kv_append_kernel<T, D, 4>, grid, kAppendThreads, 0, s, p);
+    return kv_launch(kv_append_kernel<T, D, 8>, grid, kAppendThreads, 0, s, p);
 }
 
 }  // namespace

@@ -35,7 +35,7 @@ struct AttendShared {
     float o[kKvRows][D];
     float2 ml[kConsumers][kKvRows];
     int first_key[Geometry<D>::kStages][kConsumers];
-    int64_t scratch[kAttendThreads / 32 + 2];
+    int64_t scratch[2 * (kAttendThreads / 32) + 3];
     uint64_t full[Geometry<D>::kStages], empty[Geometry<D>::kStages];
 };
 
@@ -153,39 +153,58 @@ __device__ __forceinline__ void set_up(Walk<CHOSEN> &w, int64_t *scratch, int64_
         w.prefix_tiles = max(1, (p.prefix_len + kKvTile - 1) / kKvTile);
         w.prefix_mt = max(1, w.row_tiles(w.live));
         w.prefix_total = p.prefix_len > 0 && !p.tensor_prefix && w.live > 0 ? int64_t(w.prefix_mt) * p.kv_heads * (p.item_cost + w.prefix_tiles) : 0;
-        // total cost of the sequences
-        int64_t sum = 0;
-        for (int i = threadIdx.x; i < p.batch.sequences; i += kAttendThreads) sum += w.cost(i);
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(kFullMask, sum, o);
-        if ((threadIdx.x & 31) == 0) scratch[threadIdx.x >> 5] = sum;
-        __syncthreads();
-        total = w.prefix_total;
-#pragma unroll
-        for (int i = 0; i < kAttendThreads / 32; ++i) total += scratch[i];
         w.item_of_b = w.prefix_total > 0 ? w.prefix_mt * p.kv_heads : 0;
         w.start_of_b = w.prefix_total;
+    }
+    // (cost, items) before this thread's sequence of the run of sequences that begins at b0, and of the whole run
+    struct Sums { int64_t cost, items, before_cost, before_items, all_cost, all_items; };
+    auto sums = [&](int b0) {
+        const int i = b0 + int(threadIdx.x), lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+        Sums x{};
+        if (i < p.batch.sequences) { x.items = w.items(i); x.cost = x.items * (p.item_cost + w.tiles_of(p.batch.lens[i])); }
+        int64_t c = x.cost, n = x.items;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int64_t uc = __shfl_up_sync(kFullMask, c, o), un = __shfl_up_sync(kFullMask, n, o);
+            if (lane >= o) { c += uc; n += un; }
+        }
+        __syncthreads();
+        if (lane == 31) { scratch[2 * warp] = c; scratch[2 * warp + 1] = n; }
+        __syncthreads();
+        x.before_cost = c - x.cost; x.before_items = n - x.items;
+#pragma unroll
+        for (int v = 0; v < kAttendThreads / 32; ++v) {
+            if (v < warp) { x.before_cost += scratch[2 * v]; x.before_items += scratch[2 * v + 1]; }
+            x.all_cost += scratch[2 * v]; x.all_items += scratch[2 * v + 1];
+        }
+        return x;
+    };
+    Sums mine{};
+    if constexpr (!CHOSEN) {
+        total = w.prefix_total;
+        for (int b0 = 0; b0 < p.batch.sequences; b0 += kAttendThreads) {
+            mine = sums(b0);
+            total += mine.all_cost;
+        }
     }
     per = max(int64_t(p.item_cost + kLeastTiles), divide(total + gridDim.x - 1, gridDim.x));
     w.at = min(total, int64_t(blockIdx.x) * per);
     w.end = min(total, w.at + per);
     if constexpr (!CHOSEN) {
-        if (w.at < w.end && w.at > w.prefix_total) {
-            int b;
-            int64_t place;
-            kv_locate<kAttendThreads>(w.at - w.prefix_total, p.batch.sequences, [&](int i) { return w.cost(i); }, scratch, b, place);
-            w.b = b < p.batch.sequences ? b : p.batch.sequences - 1;
-            // items before sequence b
-            int64_t before = 0;
-            for (int i = threadIdx.x; i < w.b; i += kAttendThreads) before += w.items(i);
-#pragma unroll
-            for (int o = 16; o > 0; o >>= 1) before += __shfl_xor_sync(kFullMask, before, o);
+        if (w.at < w.end && w.at > w.prefix_total) {             // the sequence that the run begins in
+            int64_t *found = scratch + 2 * (kAttendThreads / 32);
+            int64_t base_cost = w.prefix_total, base_items = w.item_of_b;
+            for (int b0 = 0; b0 < p.batch.sequences; b0 += kAttendThreads) {
+                if (p.batch.sequences > kAttendThreads) mine = sums(b0);
+                if (w.at < base_cost + mine.all_cost) {
+                    const int64_t start = base_cost + mine.before_cost;
+                    if (w.at >= start && w.at < start + mine.cost) { found[0] = b0 + int(threadIdx.x); found[1] = start; found[2] = base_items + mine.before_items; }
+                    break;
+                }
+                base_cost += mine.all_cost; base_items += mine.all_items;
+            }
             __syncthreads();
-            if ((threadIdx.x & 31) == 0) scratch[threadIdx.x >> 5] = before;
-            __syncthreads();
-#pragma unroll
-            for (int i = 0; i < kAttendThreads / 32; ++i) w.item_of_b += int(scratch[i]);
-            w.start_of_b = w.at - place;
+            w.b = int(found[0]); w.start_of_b = found[1]; w.item_of_b = int(found[2]);
         }
     }
 }
@@ -226,8 +245,6 @@ __global__ void __launch_bounds__(kAttendThreads, 2) kv_attend_kernel(const KvAt
     AttendShared<D> &sh = *reinterpret_cast<AttendShared<D> *>(ring + G::kStages * G::kStageBytes);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
-    asm volatile("griddepcontrol.launch_dependents;");
-    if constexpr (CHOSEN) asm volatile("griddepcontrol.wait;" ::: "memory");
     if (tid == kConsumers * 32) {
         asm volatile("prefetch.tensormap [%0];" ::"l"(&maps.k) : "memory");
         asm volatile("prefetch.tensormap [%0];" ::"l"(&maps.v) : "memory");
@@ -236,6 +253,10 @@ __global__ void __launch_bounds__(kAttendThreads, 2) kv_attend_kernel(const KvAt
         for (int s = 0; s < G::kStages; ++s) { mbar_init(&sh.full[s], 1); mbar_init(&sh.empty[s], kConsumers); }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
+    // after a prefix kernel nothing that it writes is read here: this one may run beside it, and what was before it had ended
+    // when it let this one begin
+    if (CHOSEN || !p.tensor_prefix) asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;");
     __syncthreads();
     Walk<CHOSEN> walk{p};
     int64_t per;
@@ -496,7 +517,7 @@ __global__ void __launch_bounds__(kAttendThreads, 2) kv_attend_kernel(const KvAt
             }
             if (c2 == 0 && w.tile0 == 0) {                      // where the parts of the item lie, packed with the row within a slot
                 const int64_t begin = divide(w.item_start, per), finish_at = divide(w.item_start + w.item_tiles - 1, per);
-                KvPieces pc{int(w.item + begin), whole ? 0 : int(finish_at - begin + 1)};
+                const KvPieces pc{(w.item + begin) * kKvRows + r, whole ? 0 : int(finish_at - begin + 1), 0};
                 (w.b < 0 ? p.prefix_pieces : p.own_pieces)[token * p.heads + head] = pc;
             }
         };
@@ -510,6 +531,7 @@ template <typename T, int D, int WARPS>
 __global__ void __launch_bounds__(128) kv_join_kernel(const KvAttendParams p) {
     constexpr int kPer = D / 32;
     asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;");
     __shared__ float4 others[WARPS > 1 ? WARPS - 1 : 1][32];
     __shared__ float2 others_ml[WARPS > 1 ? WARPS - 1 : 1];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, turn = warp % WARPS;
@@ -555,17 +577,15 @@ __global__ void __launch_bounds__(128) kv_join_kernel(const KvAttendParams p) {
             }
         }
     };
-    auto add_items = [&](const KvPieces &pc, int in_item) {
-        if (pc.first_slot < 0 || pc.count < 0 || int64_t(pc.first_slot) + pc.count > p.slots) return;
-        const int64_t at = int64_t(pc.first_slot) * kKvRows + in_item;
-        add(p.part_o + at * D, p.part_ml + at, int64_t(kKvRows) * D, pc.count);
+    auto add_items = [&](const KvPieces &pc) {
+        if (pc.first_row < 0 || pc.count < 0 || pc.first_row / kKvRows + pc.count > p.slots) return;
+        add(p.part_o + pc.first_row * D, p.part_ml + pc.first_row, int64_t(kKvRows) * D, pc.count);
     };
     const KvPieces own = p.own_pieces[row];
     if (own.count == 0 && p.prefix_len == 0) return;
-    // the row's place within its items: rows of a group lie together, token after token
-    const int h = head / p.group, g = head - h * p.group;
-    const int64_t r = int64_t(token - all.first) * p.group + g;
     if (p.tensor_prefix) {
+        const int h = head / p.group;                // rows of a key head lie together, token after token
+        const int64_t r = int64_t(token - all.first) * p.group + head - h * p.group;
         const KvPrefixPlan &w = p.plan;
         const int first = int(int64_t(h) * w.tiles / w.per), count = int((int64_t(h + 1) * w.tiles - 1) / w.per) - first + 1;
         const int64_t block = int64_t(kKvPrefixRows) * D;
@@ -577,20 +597,9 @@ __global__ void __launch_bounds__(128) kv_join_kernel(const KvAttendParams p) {
             add(p.pre_o + at * D, p.pre_ml + at, block, 2 * count);
         }
     } else if (p.prefix_len > 0) {
-        add_items(p.prefix_pieces[row], int(r % kKvRows));
+        add_items(p.prefix_pieces[row]);
     }
-    int from = 0;
-    if (p.chosen == nullptr) {                       // first token of the row's sequence
-        int lo = 0, hi = p.batch.sequences;
-        while (hi - lo > 1) {
-            const int mid = (lo + hi) >> 1;
-            if (p.batch.offsets[mid] <= token) lo = mid; else hi = mid;
-        }
-        from = kv_span(p.batch.offsets[lo], p.batch.offsets[lo + 1], p.tokens).first;
-        add_items(own, int((int64_t(token - from) * p.group + g) % kKvRows));
-    } else {
-        add_items(own, g % kKvRows);
-    }
+    add_items(own);
     if constexpr (WARPS > 1) {
         static_assert(WARPS == 4, "a block is one row");
         if (turn > 0) {
@@ -622,49 +631,38 @@ __global__ void __launch_bounds__(128) kv_join_kernel(const KvAttendParams p) {
 }
 
 template <typename T, int D, bool CHOSEN>
-cudaError_t launch(const KvAttendParams &p, const KvMaps &maps, int sm_count, cudaStream_t s) {
+cudaError_t launch(const KvAttendParams &p, const KvMaps &maps, int device, int sm_count, cudaStream_t s) {
     using G = Geometry<D>;
     const size_t smem = size_t(G::kStages) * G::kStageBytes + sizeof(AttendShared<D>) + 1024;
     auto *kern = kv_attend_kernel<T, D, CHOSEN>;
-    cudaError_t e = allow_dynamic_shared(kern);
+    static std::atomic<uint64_t> allowed{0};
+    cudaError_t e = kv_allow_shared(kern, allowed, device);
     if (e != cudaSuccess) return e;
-    cudaLaunchAttribute after;
-    after.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    after.val.programmaticStreamSerializationAllowed = 1;
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(unsigned(kv_attend_grid(sm_count)));
-    cfg.blockDim = dim3(kAttendThreads);
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = s;
-    cfg.attrs = &after;
-    cfg.numAttrs = CHOSEN || p.tensor_prefix ? 1 : 0;
-    e = cudaLaunchKernelEx(&cfg, kern, p, maps);
+    e = kv_launch(kern, dim3(unsigned(kv_attend_grid(sm_count))), kAttendThreads, smem, s, p, maps);
     if (e != cudaSuccess) return e;
     // few rows have many parts each
     const int64_t rows = int64_t(p.tokens) * p.heads;
-    const bool few = rows <= 16 * sm_count;
-    cfg.gridDim = dim3(unsigned(few ? rows : (rows + 3) / 4));
-    cfg.blockDim = dim3(128);
-    cfg.dynamicSmemBytes = 0;
-    cfg.numAttrs = 1;
-    return few ? cudaLaunchKernelEx(&cfg, kv_join_kernel<T, D, 4>, p) : cudaLaunchKernelEx(&cfg, kv_join_kernel<T, D, 1>, p);
+    if (rows <= 16 * sm_count) return kv_launch(kv_join_kernel<T, D, 4>, dim3(unsigned(rows)), 128, 0, s, p);
+    return kv_launch(kv_join_kernel<T, D, 1>, dim3(unsigned((rows + 3) / 4)), 128, 0, s, p);
 }
 
 }  // namespace
 
 int kv_attend_grid(int sm_count) { return 2 * sm_count; }
 
-uint32_t *kv_timeouts_symbol() {
-    void *ptr = nullptr;
-    return cudaGetSymbolAddress(&ptr, g_kv_timeouts) == cudaSuccess ? static_cast<uint32_t *>(ptr) : nullptr;
+uint32_t *kv_timeouts_symbol(int device) {
+    static std::atomic<void *> known[kKvMaxDevices];
+    void *ptr = known[device].load(std::memory_order_relaxed);
+    if (ptr == nullptr && cudaGetSymbolAddress(&ptr, g_kv_timeouts) == cudaSuccess) known[device].store(ptr, std::memory_order_relaxed);
+    return static_cast<uint32_t *>(ptr);
 }
 
-cudaError_t launch_kv_attend(const KvAttendParams &p, const KvMaps &maps, int dtype, int head_dim, bool chosen, int sm_count, cudaStream_t s) {
+cudaError_t launch_kv_attend(const KvAttendParams &p, const KvMaps &maps, int dtype, int head_dim, bool chosen, int device, int sm_count, cudaStream_t s) {
     if (p.tokens == 0 || p.batch.sequences == 0) return cudaSuccess;
     auto go = [&](auto t, auto d) {
         using T = decltype(t);
         constexpr int D = decltype(d)::value;
-        return chosen ? launch<T, D, true>(p, maps, sm_count, s) : launch<T, D, false>(p, maps, sm_count, s);
+        return chosen ? launch<T, D, true>(p, maps, device, sm_count, s) : launch<T, D, false>(p, maps, device, sm_count, s);
     };
     using D64 = std::integral_constant<int, 64>;
     using D128 = std::integral_constant<int, 128>;

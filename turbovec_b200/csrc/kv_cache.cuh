@@ -11,6 +11,7 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <atomic>
 #include <climits>
 #include <cstdint>
 #include <type_traits>
@@ -91,6 +92,34 @@ __device__ __forceinline__ float kv_exp2(float x) {
     return y;
 }
 
+// Lets a kernel have all of a block's shared memory, once per device: the call costs as much as a launch's arguments.
+constexpr int kKvMaxDevices = 64;
+template <typename Kernel>
+inline cudaError_t kv_allow_shared(Kernel *kern, std::atomic<uint64_t> &done, int device, int static_bytes = 0) {
+    const uint64_t bit = uint64_t(1) << device;
+    if (done.load(std::memory_order_relaxed) & bit) return cudaSuccess;
+    const cudaError_t e = allow_dynamic_shared(kern, static_bytes);
+    if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_relaxed);
+    return e;
+}
+
+// Launches a kernel that may begin before the one in front of it in the stream has ended: each of them waits (griddepcontrol.wait)
+// before it touches memory.
+template <typename... Params, typename... Args>
+inline cudaError_t kv_launch(void (*kern)(Params...), dim3 grid, int threads, size_t smem, cudaStream_t s, const Args &...args) {
+    cudaLaunchAttribute early;
+    early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    early.val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(unsigned(threads));
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    cfg.attrs = &early;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kern, args...);
+}
+
 // Index of the work unit `at` (block-uniform) of a list in which sequence b has cost(b) units, b ascending: gives b and the
 // unit's place within it; b = sequences when the list is shorter.  All threads of the block call this; `scratch` holds one
 // int64 per warp and two more.
@@ -146,7 +175,8 @@ cudaError_t launch_kv_append(const KvAppendParams &p, int dtype, int head_dim, c
 // Keys that an item of the attention reads, as tiles of kKvTile keys; a row of partial results for every part of it that a block
 // computes.  The parts of an item lie in consecutive slots (kv_attend.cu).
 struct KvPieces {
-    int first_slot, count;                   // count 0: the row was written where it belongs
+    int64_t first_row;                       // first slot * kKvRows + the row within the item
+    int count, unused;                       // count 0: the row was written where it belongs
 };
 // Partial results of the tensor-memory form for a prefix (kv_prefix.cu): blocks of 128 rows.
 constexpr int kKvPrefixRows = 128;           // M of tcgen05.mma
@@ -207,10 +237,10 @@ inline int64_t kv_attend_slots(int64_t tokens, int64_t sequences, int group, int
 }
 inline int64_t kv_chosen_slots(int64_t tokens, int group, int kv_heads, int grid) { return tokens * ((group + kKvRows - 1) / kKvRows) * kv_heads + grid; }
 int kv_attend_grid(int sm_count);
-cudaError_t launch_kv_attend(const KvAttendParams &p, const KvMaps &maps, int dtype, int head_dim, bool chosen, int sm_count, cudaStream_t s);
+cudaError_t launch_kv_attend(const KvAttendParams &p, const KvMaps &maps, int dtype, int head_dim, bool chosen, int device, int sm_count, cudaStream_t s);
 // The prefix by tcgen05 (kv_prefix.cu); launched before launch_kv_attend with the same parameters.
-cudaError_t launch_kv_prefix(const KvAttendParams &p, const KvMaps &maps, int dtype, int head_dim, cudaStream_t s);
-uint32_t *kv_timeouts_symbol();              // address on the current device, null if it cannot be had
+cudaError_t launch_kv_prefix(const KvAttendParams &p, const KvMaps &maps, int dtype, int head_dim, int device, cudaStream_t s);
+uint32_t *kv_timeouts_symbol(int device);    // address on `device`, which is the current one; null if it cannot be had
 
 constexpr int kKvMaxScored = 49152;          // pages of a sequence whose scores fit a block's shared memory
 struct KvSelectParams {
@@ -221,6 +251,6 @@ struct KvSelectParams {
     int32_t *chosen, *chosen_pool, *token_pos;
     int tokens, group, kv_heads, page_shift, pages, budget, first, recent;
 };
-cudaError_t launch_kv_select(const KvSelectParams &p, int dtype, int head_dim, int sm_count, cudaStream_t s);
+cudaError_t launch_kv_select(const KvSelectParams &p, int dtype, int head_dim, int device, int sm_count, cudaStream_t s);
 
 }  // namespace tv

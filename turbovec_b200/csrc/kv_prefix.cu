@@ -105,8 +105,6 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) kv_prefix_kernel(const KvAt
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const KvPrefixPlan plan = p.plan;
     const int unit = blockIdx.x % plan.units, group = blockIdx.x / plan.units;
-    asm volatile("griddepcontrol.launch_dependents;");
-
     if (tid == 0) {
         for (int s = 0; s < G::kSlots; ++s) { mbar_init(&sh.full[s], 1); mbar_init(&sh.empty[s], 1); }
         for (int s = 0; s < 2; ++s) { mbar_init(&sh.s_full[s], 1); mbar_init(&sh.p_ready[s], 4); mbar_init(&sh.o_done[s], 1); }
@@ -121,6 +119,9 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) kv_prefix_kernel(const KvAt
     __syncthreads();
     fence_after();
     const uint32_t tmem = sh.tmem_base;
+    // the attention kernel that follows does not wait for this one before it reads: what both read must be there by now
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;");
     const int64_t steps = int64_t(p.kv_heads) * plan.tiles;
     int64_t at = min(steps, group * plan.per);
     const int64_t end = min(steps, at + plan.per);
@@ -372,21 +373,22 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) kv_prefix_kernel(const KvAt
 }
 
 template <typename T, int D>
-cudaError_t launch(const KvAttendParams &p, const KvMaps &maps, cudaStream_t s) {
+cudaError_t launch(const KvAttendParams &p, const KvMaps &maps, int device, cudaStream_t s) {
     using G = PrefixGeometry<D>;
     const size_t smem = G::kQBytes + size_t(G::kSlots) * G::kTileBytes + sizeof(PrefixShared<D>) + 1024;
     static_assert(G::kQBytes + G::kSlots * G::kTileBytes + sizeof(PrefixShared<D>) + 1024 <= kBlockSharedBytes, "more shared memory than a block can have");
-    cudaError_t e = allow_dynamic_shared(kv_prefix_kernel<T, D>);
+    auto *kern = kv_prefix_kernel<T, D>;
+    static std::atomic<uint64_t> allowed{0};
+    const cudaError_t e = kv_allow_shared(kern, allowed, device);
     if (e != cudaSuccess) return e;
-    kv_prefix_kernel<T, D><<<unsigned(p.plan.units * p.plan.groups), kPrefixThreads, smem, s>>>(p, maps);
-    return cudaGetLastError();
+    return kv_launch(kern, dim3(unsigned(p.plan.units * p.plan.groups)), kPrefixThreads, smem, s, p, maps);
 }
 
 }  // namespace
 
-cudaError_t launch_kv_prefix(const KvAttendParams &p, const KvMaps &maps, int dtype, int head_dim, cudaStream_t s) {
-    if (dtype == TV_KV_BF16) return head_dim == 128 ? launch<__nv_bfloat16, 128>(p, maps, s) : launch<__nv_bfloat16, 64>(p, maps, s);
-    return head_dim == 128 ? launch<__half, 128>(p, maps, s) : launch<__half, 64>(p, maps, s);
+cudaError_t launch_kv_prefix(const KvAttendParams &p, const KvMaps &maps, int dtype, int head_dim, int device, cudaStream_t s) {
+    if (dtype == TV_KV_BF16) return head_dim == 128 ? launch<__nv_bfloat16, 128>(p, maps, device, s) : launch<__nv_bfloat16, 64>(p, maps, device, s);
+    return head_dim == 128 ? launch<__half, 128>(p, maps, device, s) : launch<__half, 64>(p, maps, device, s);
 }
 
 }  // namespace tv

@@ -48,6 +48,7 @@ __global__ void __launch_bounds__(kSelectThreads, 2) kv_select_kernel(const KvSe
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, token = blockIdx.x / blocks, h = blockIdx.y;
     const int rank = blocks > 1 ? int(cluster_ctarank()) : 0;              // clusters lie along x
 
+    asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;");
     if (blocks > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");   // this block has begun: others may write into it
     auto others_begun = [&] { if (blocks > 1) asm volatile("barrier.cluster.wait.aligned;" ::: "memory"); };
@@ -249,34 +250,37 @@ __global__ void __launch_bounds__(kSelectThreads, 2) kv_select_kernel(const KvSe
 }
 
 template <typename T, int D>
-cudaError_t launch(const KvSelectParams &p, int sm_count, cudaStream_t s) {
+cudaError_t launch(const KvSelectParams &p, int device, int sm_count, cudaStream_t s) {
     constexpr int kStatic = 8 * 1024;
     auto *kern = kv_select_kernel<T, D>;
-    cudaError_t e = allow_dynamic_shared(kern, kStatic);
+    static std::atomic<uint64_t> allowed{0};
+    const cudaError_t e = kv_allow_shared(kern, allowed, device, kStatic);
     if (e != cudaSuccess) return e;
     // as many blocks to a token and key head as the device holds at once (two to a multiprocessor), none with less than a round of pages
     const int64_t items = int64_t(p.tokens) * p.kv_heads;
     int blocks = 1;
     while (blocks < 8 && items * blocks * 2 <= 2 * sm_count && blocks * kSelectWarps * 8 < p.batch.table_width) blocks *= 2;
-    cudaLaunchAttribute cluster;
-    cluster.id = cudaLaunchAttributeClusterDimension;
-    cluster.val.clusterDim.x = unsigned(blocks); cluster.val.clusterDim.y = 1; cluster.val.clusterDim.z = 1;
+    cudaLaunchAttribute attrs[2];
+    attrs[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attrs[0].val.programmaticStreamSerializationAllowed = 1;
+    attrs[1].id = cudaLaunchAttributeClusterDimension;
+    attrs[1].val.clusterDim.x = unsigned(blocks); attrs[1].val.clusterDim.y = 1; attrs[1].val.clusterDim.z = 1;
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(unsigned(p.tokens) * unsigned(blocks), unsigned(p.kv_heads));
     cfg.blockDim = dim3(kSelectThreads);
     cfg.dynamicSmemBytes = size_t(p.batch.table_width) * 4;
     cfg.stream = s;
-    cfg.attrs = &cluster;
-    cfg.numAttrs = blocks > 1 ? 1 : 0;
+    cfg.attrs = attrs;
+    cfg.numAttrs = blocks > 1 ? 2 : 1;
     return cudaLaunchKernelEx(&cfg, kern, p, blocks);
 }
 
 }  // namespace
 
-cudaError_t launch_kv_select(const KvSelectParams &p, int dtype, int head_dim, int sm_count, cudaStream_t s) {
+cudaError_t launch_kv_select(const KvSelectParams &p, int dtype, int head_dim, int device, int sm_count, cudaStream_t s) {
     if (p.tokens == 0 || p.batch.sequences == 0) return cudaSuccess;
-    if (dtype == TV_KV_BF16) return head_dim == 128 ? launch<__nv_bfloat16, 128>(p, sm_count, s) : launch<__nv_bfloat16, 64>(p, sm_count, s);
-    return head_dim == 128 ? launch<__half, 128>(p, sm_count, s) : launch<__half, 64>(p, sm_count, s);
+    if (dtype == TV_KV_BF16) return head_dim == 128 ? launch<__nv_bfloat16, 128>(p, device, sm_count, s) : launch<__nv_bfloat16, 64>(p, device, sm_count, s);
+    return head_dim == 128 ? launch<__half, 128>(p, device, sm_count, s) : launch<__half, 64>(p, device, sm_count, s);
 }
 
 }  // namespace tv

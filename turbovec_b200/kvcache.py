@@ -16,8 +16,6 @@ in place between calls, and a captured graph sees the new values.  There is no C
 """
 from __future__ import annotations
 
-import ctypes as C
-
 import torch
 
 from . import _native
@@ -25,7 +23,15 @@ from . import _native
 __all__ = ["PagedKVCache", "KVBatch"]
 
 _DTYPES = {torch.bfloat16: 0, torch.float16: 1}
-_ref = C.byref
+
+
+def _stream(index: int) -> int:
+    """torch's current stream of a device, as a number."""
+    return torch.cuda.current_stream(index).cuda_stream
+
+
+# the same without a Stream object around it: 0.2 us instead of 2.4
+_stream = getattr(torch._C, "_cuda_getCurrentRawStream", _stream)
 
 
 def _fail(lib, rc: int):
@@ -120,6 +126,7 @@ class PagedKVCache:
         self.k, self.v, self.bounds, self.scales = k, v, bounds, scales
         self.device, self.dtype = k.device, k.dtype
         self.pages, self.kv_heads, self.page_size, self.head_dim = pages, heads, page_size, dim
+        self._index, self._scale, self._sizes = k.device.index, dim ** -0.5, {}
 
         def stride(t, i, natural):                      # of a dimension of one, whatever it says
             return t.stride(i) if t.shape[i] > 1 else natural
@@ -141,18 +148,33 @@ class PagedKVCache:
         s = torch.full((pages, kv_heads), 2.0 ** -24, dtype=torch.float32, device=device) if bounds else None
         return cls(k, v, b, s)
 
-    # ---- helpers ----
-    def _rows(self, name: str, t, tokens: int | None, heads: int | None) -> _native.KvRowsView:
-        _tensor(name, t, self.dtype, 3, self.device)
-        n, h, d = t.shape
+    # ---- helpers (on the path of every call: a tensor's attributes cost 0.2 us each, a check by a function of its own 0.3) ----
+    def _rows(self, name: str, t, tokens: int | None, heads: int | None):
+        """(rows, heads, view) of a [rows, heads, head_dim] tensor, of `tokens` and `heads` where given."""
+        if not isinstance(t, torch.Tensor):
+            raise TypeError(f"{name} must be a torch tensor, got {type(t).__name__}")
+        if t.dtype != self.dtype:
+            raise TypeError(f"{name} must be of {self.dtype}, got {t.dtype}")
+        shape = t.shape
+        if len(shape) != 3:
+            raise ValueError(f"{name} must have 3 dimensions, got {len(shape)}")
+        if t.get_device() != self._index:
+            raise ValueError(f"{name} must be on {self.device}, got {t.device}")
+        n, h, d = shape
         if d != self.head_dim:
             raise ValueError(f"{name} must have {self.head_dim} channels, got {d}")
         if (tokens is not None and n != tokens) or (heads is not None and h != heads):
-            raise ValueError(f"{name} must have {tokens if tokens is not None else n} rows of {heads if heads is not None else h} heads, got {n} of {h}")
+            raise ValueError(f"{name} must have {n if tokens is None else tokens} rows of {h if heads is None else heads} heads, got {n} of {h}")
         st = t.stride()
         if st[2] != 1:
             raise ValueError(f"{name}: the elements of the last dimension must be adjacent")
-        return _native.KvRowsView(t.data_ptr(), st[0] if n > 1 else h * d, st[1] if h > 1 else d)
+        return n, h, _native.KvRowsView(t.data_ptr(), st[0] if n > 1 else h * d, st[1] if h > 1 else d)
+
+    def _query(self, q, tokens: int | None = None):
+        n, heads, view = self._rows("q", q, tokens, None)
+        if heads < 1 or heads % self.kv_heads:
+            raise ValueError(f"the number of query heads must be a positive multiple of {self.kv_heads}, got {heads}")
+        return n, heads, view
 
     def _batch(self, batch) -> _native.KvBatchView:
         if not isinstance(batch, KVBatch):
@@ -161,27 +183,29 @@ class PagedKVCache:
             raise ValueError(f"batch must be on {self.device}, got {batch.device}")
         return batch._view
 
-    def _query(self, q):
-        _tensor("q", q, self.dtype, 3, self.device)
-        heads = q.shape[1]
-        if heads < 1 or heads % self.kv_heads:
-            raise ValueError(f"the number of query heads must be a positive multiple of {self.kv_heads}, got {heads}")
-        return q.shape[0], heads
+    def _array(self, name: str, t, dtype, shape) -> int:
+        """Address of a contiguous tensor of that type and shape (None: any length of one dimension)."""
+        if not isinstance(t, torch.Tensor):
+            raise TypeError(f"{name} must be a torch tensor, got {type(t).__name__}")
+        if t.dtype != dtype:
+            raise TypeError(f"{name} must be of {dtype}, got {t.dtype}")
+        if (len(t.shape) != 1 if shape is None else t.shape != shape) or not t.is_contiguous():
+            raise ValueError(f"{name} must be contiguous with {'one dimension' if shape is None else f'shape {tuple(shape)}'}, got {tuple(t.shape)}")
+        if t.get_device() != self._index:
+            raise ValueError(f"{name} must be on {self.device}, got {t.device}")
+        return t.data_ptr()
 
-    def _stream(self) -> int:
-        return torch.cuda.current_stream(self.device).cuda_stream
-
-    def _lse(self, lse, tokens: int, heads: int):
-        if lse is None:
-            return None
-        _tensor("lse", lse, torch.float32, 2, self.device)
-        if tuple(lse.shape) != (tokens, heads) or not lse.is_contiguous():
-            raise ValueError(f"lse must be contiguous with shape {(tokens, heads)}, got {tuple(lse.shape)}")
-        return lse.data_ptr()
-
-    def _workspace(self, n: int) -> torch.Tensor:
-        if n == 0:
-            _fail(self._lib, 90)
+    def _workspace(self, op: str, batch, *sizes) -> torch.Tensor:
+        """A workspace for an operator; its size for these sizes is asked for once."""
+        key = (op, batch._view.sequences, *sizes)
+        n = self._sizes.get(key)
+        if n is None:
+            n = getattr(self._lib, f"tv_kv_{op}_workspace")(self._view, batch._view, *sizes)
+            if n == 0:
+                _fail(self._lib, 90)
+            if len(self._sizes) >= 256:
+                self._sizes.clear()
+            self._sizes[key] = n
         return torch.empty(n, dtype=torch.uint8, device=self.device)
 
     # ---- operators ----
@@ -192,30 +216,27 @@ class PagedKVCache:
         returns it.  cos and sin: float32 [positions, rotary / 2], rotary a multiple of 16 up to head_dim; None: no rotation.  Pairs are
         channels i and i + rotary / 2, or 2i and 2i + 1 where `interleaved`.  Tokens at positions below 0 or without an angle are left out."""
         b = self._batch(batch)
-        kr = self._rows("k", k, None, self.kv_heads)
-        tokens = k.shape[0]
-        vr = self._rows("v", v, tokens, self.kv_heads)
-        heads, qr, qo = self.kv_heads, None, None
+        tokens, heads, kr = self._rows("k", k, None, self.kv_heads)
+        vr = self._rows("v", v, tokens, heads)[2]
+        qr = qo = None
         if q is not None:
-            n, heads = self._query(q)
-            qr = self._rows("q", q, tokens, heads)
+            _, heads, qr = self._query(q, tokens)
             if q_out is None:
                 q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
-            qo = self._rows("q_out", q_out, tokens, heads)
+            qo = self._rows("q_out", q_out, tokens, heads)[2]
         elif q_out is not None:
             raise ValueError("q_out must not be given without q")
         positions = rotary = 0
+        cos_at = sin_at = None
         if (cos is None) != (sin is None):
             raise ValueError("cos and sin must be given together")
         if cos is not None:
-            _tensor("cos", cos, torch.float32, 2, self.device)
-            _tensor("sin", sin, torch.float32, 2, self.device)
-            if cos.shape != sin.shape or not cos.is_contiguous() or not sin.is_contiguous():
-                raise ValueError("cos and sin must be contiguous and have the same shape")
+            if not isinstance(cos, torch.Tensor) or len(cos.shape) != 2:
+                raise ValueError("cos must be a tensor of two dimensions")
+            cos_at, sin_at = self._array("cos", cos, torch.float32, cos.shape), self._array("sin", sin, torch.float32, cos.shape)
             positions, rotary = cos.shape[0], 2 * cos.shape[1]
-        rc = self._lib.tv_kv_append(self._view, b, tokens, heads, kr, vr, qr, qo, cos.data_ptr() if positions else None,
-                                    sin.data_ptr() if positions else None, positions, rotary if positions else 0, int(bool(interleaved)),
-                                    int(position_offset), self._stream())
+        rc = self._lib.tv_kv_append(self._view, b, tokens, heads, kr, vr, qr, qo, cos_at, sin_at, positions, rotary,
+                                    1 if interleaved else 0, position_offset, _stream(self._index))
         if rc:
             _fail(self._lib, rc)
         return q_out
@@ -227,24 +248,23 @@ class PagedKVCache:
         receives the logarithm of each row's sum of exponentials.  scale: head_dim ** -0.5 by default.  Rows that see no key: zeros
         and -inf."""
         b = self._batch(batch)
-        tokens, heads = self._query(q)
-        qr = self._rows("q", q, tokens, heads)
+        tokens, heads, qr = self._query(q)
         if out is None:
             out = torch.empty_like(q, memory_format=torch.contiguous_format)
-        orow = self._rows("out", out, tokens, heads)
-        width = 0
+        orow = self._rows("out", out, tokens, heads)[2]
+        width, pages_at = 0, None
         if prefix_pages is not None:
-            _tensor("prefix_pages", prefix_pages, torch.int32, 1, self.device)
-            if not prefix_pages.is_contiguous():
-                raise ValueError("prefix_pages must be contiguous")
-            width = prefix_pages.numel()
-        prefix_len = int(prefix_len)
+            pages_at = self._array("prefix_pages", prefix_pages, torch.int32, None)
+            width = prefix_pages.shape[0]
         if not 0 <= prefix_len <= width * self.page_size:
             raise ValueError(f"prefix_len must be between 0 and the {width * self.page_size} tokens of prefix_pages, got {prefix_len}")
-        ws = self._workspace(self._lib.tv_kv_attend_workspace(self._view, b, tokens, heads, prefix_len)) if tokens and len(batch) else None
-        rc = self._lib.tv_kv_attend(self._view, b, tokens, heads, qr, prefix_pages.data_ptr() if prefix_len else None, width, prefix_len,
-                                    self.head_dim ** -0.5 if scale is None else float(scale), orow, self._lse(lse, tokens, heads),
-                                    ws.data_ptr() if ws is not None else None, ws.numel() if ws is not None else 0, self._stream())
+        lse_at = None if lse is None else self._array("lse", lse, torch.float32, (tokens, heads))
+        ws_at, ws_n = None, 0
+        if tokens and len(batch):
+            ws = self._workspace("attend", batch, tokens, heads, prefix_len)
+            ws_at, ws_n = ws.data_ptr(), ws.shape[0]
+        rc = self._lib.tv_kv_attend(self._view, b, tokens, heads, qr, pages_at, width, prefix_len, self._scale if scale is None else scale,
+                                    orow, lse_at, ws_at, ws_n, _stream(self._index))
         if rc:
             _fail(self._lib, rc)
         return out
@@ -257,30 +277,28 @@ class PagedKVCache:
         if self.bounds is None:
             raise ValueError("the cache has no bounds to choose pages by")
         b = self._batch(batch)
-        tokens, heads = self._query(q)
-        qr = self._rows("q", q, tokens, heads)
-        budget, first, recent = int(budget), int(first), int(recent)
+        tokens, heads, qr = self._query(q)
         if budget < 1 or first < 0 or recent < 0 or first + recent > budget:
             raise ValueError(f"budget must be positive and first + recent at most budget, got {budget}, {first} and {recent}")
         if out is None:
             out = torch.empty_like(q, memory_format=torch.contiguous_format)
-        orow = self._rows("out", out, tokens, heads)
+        orow = self._rows("out", out, tokens, heads)[2]
         if pages is None:
             pages = torch.empty(tokens, self.kv_heads, budget, dtype=torch.int32, device=self.device)
-        _tensor("pages", pages, torch.int32, 3, self.device)
-        if tuple(pages.shape) != (tokens, self.kv_heads, budget) or not pages.is_contiguous():
-            raise ValueError(f"pages must be contiguous with shape {(tokens, self.kv_heads, budget)}, got {tuple(pages.shape)}")
-        ws = self._workspace(self._lib.tv_kv_attend_selected_workspace(self._view, b, tokens, heads, budget)) if tokens and len(batch) else None
-        rc = self._lib.tv_kv_attend_selected(self._view, b, tokens, heads, qr, budget, first, recent,
-                                             self.head_dim ** -0.5 if scale is None else float(scale), orow, self._lse(lse, tokens, heads),
-                                             pages.data_ptr(), ws.data_ptr() if ws is not None else None, ws.numel() if ws is not None else 0,
-                                             self._stream())
+        pages_at = self._array("pages", pages, torch.int32, (tokens, self.kv_heads, budget))
+        lse_at = None if lse is None else self._array("lse", lse, torch.float32, (tokens, heads))
+        ws_at, ws_n = None, 0
+        if tokens and len(batch):
+            ws = self._workspace("attend_selected", batch, tokens, heads, budget)
+            ws_at, ws_n = ws.data_ptr(), ws.shape[0]
+        rc = self._lib.tv_kv_attend_selected(self._view, b, tokens, heads, qr, budget, first, recent, self._scale if scale is None else scale,
+                                             orow, lse_at, pages_at, ws_at, ws_n, _stream(self._index))
         if rc:
             _fail(self._lib, rc)
         return out, pages
 
     def check(self) -> None:
         """Waits for the device and raises RuntimeError if a kernel of the cache gave up a wait since the last check."""
-        rc = self._lib.tv_kv_status(self.device.index)
+        rc = self._lib.tv_kv_status(self._index)
         if rc:
             _fail(self._lib, rc)
