@@ -19,7 +19,9 @@
 namespace tv {
 namespace {
 
-constexpr int kPrefixThreads = 10 * 32;          // 2 x 4 warps of weights, one of MMAs, one of copies
+constexpr int kPrefixThreads = 12 * 32;          // 2 x 4 warps of weights, one of MMAs, one of copies, two that complete the group
+constexpr int kWeightRegs = 208, kOtherRegs = 88;   // registers a thread: 256 * 208 + 128 * 88 = 384 * 168, what the block starts with
+static_assert(256 * kWeightRegs + 128 * kOtherRegs <= kPrefixThreads * 168, "more registers than the block has");
 constexpr int kMmaWarp = 8, kCopyWarp = 9;
 constexpr float kRescaleAt = 8.0f;
 
@@ -52,19 +54,36 @@ template <typename T>
 constexpr uint32_t idesc(int n, bool b_adjacent) {
     return (1u << 4) | (std::is_same<T, __nv_bfloat16>::value ? (1u << 7) | (1u << 10) : 0u) | (b_adjacent ? 1u << 16 : 0u) | (uint32_t(n >> 3) << 17) | (128u >> 4 << 24);
 }
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t id, uint32_t accumulate) {
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
-        ::"r"(d), "l"(a), "l"(b), "r"(id), "r"(accumulate) : "memory");
+// MMAs and commits are executed by the whole warp and issued by its elected lane: no branch, so that descriptors and addresses, which are
+// the same in all lanes, stay in uniform registers.  (With a branch around them an MMA took 100 cycles to issue, 64 to execute.)
+__device__ __forceinline__ uint32_t elected() {
+    uint32_t x;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(x));
+    return x;
 }
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t id, uint32_t accumulate) {
+template <bool ACCUMULATE>
+__device__ __forceinline__ void mma_ss(uint32_t leader, uint32_t d, uint64_t a, uint64_t b, uint32_t id) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
-        ::"r"(d), "r"(a), "l"(b), "r"(id), "r"(accumulate) : "memory");
+        "{\n\t.reg .pred p, q;\n\t"
+        "setp.ne.b32 q, %4, 0;\n\t"
+        "setp.ne.b32 p, %5, 0;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+        ::"r"(d), "l"(a), "l"(b), "r"(id), "r"(leader), "n"(ACCUMULATE ? 1 : 0) : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t leader, uint32_t d, uint32_t a, uint64_t b, uint32_t id, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\t"
+        "setp.ne.b32 q, %4, 0;\n\t"
+        "setp.ne.b32 p, %5, 0;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+        ::"r"(d), "r"(a), "l"(b), "r"(id), "r"(leader), "r"(accumulate) : "memory");
+}
+__device__ __forceinline__ void commit(uint32_t leader, uint64_t *bar) {
+    asm volatile(
+        "{\n\t.reg .pred q;\n\t"
+        "setp.ne.b32 q, %1, 0;\n\t"
+        "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}"
+        ::"r"(smem_u32(bar)), "r"(leader) : "memory");
 }
 __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t *r) {
     asm volatile(
@@ -75,6 +94,27 @@ __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t *r) {
           "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]),
           "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]),
           "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31]), "r"(taddr) : "memory");
+}
+// two at a time: twice the rate of the single form
+__device__ __forceinline__ uint64_t pair(float a, float b) {
+    uint64_t d;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(a), "f"(b));
+    return d;
+}
+__device__ __forceinline__ float2 unpair(uint64_t x) {
+    float2 y;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(y.x), "=f"(y.y) : "l"(x));
+    return y;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+    return d;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
 }
 __device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
@@ -129,6 +169,8 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) kv_prefix_kernel(const KvAt
     PrefixPart w;
     bool ok = true;
 
+    if (warp >= 8) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
     if (warp == kCopyWarp) {
         // ---- tiles in the order of their use: the keys `lookahead` tiles ahead of the values
         const int box = min(kKvPrefixTile, 1 << p.page_shift), boxes = kKvPrefixTile / box;
@@ -163,59 +205,54 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) kv_prefix_kernel(const KvAt
         if (!ok)                                                 // the copies in flight land before the block ends
             for (uint32_t i = n > G::kSlots ? n - G::kSlots : 0; i < n; ++i) mbar_wait(&sh.full[i % G::kSlots], (i / G::kSlots) & 1, p.timeouts);
     } else if (warp == kMmaWarp) {
-        uint32_t n = 0, parts = 0, p_count[2] = {0, 0};
+        uint32_t parts = 0, p_count[2] = {0, 0};
         constexpr uint32_t kIdS = idesc<T>(128, false), kIdO = idesc<T>(D, true);
         const uint32_t ring_addr = smem_u32(ring), q_addr = smem_u32(q_smem);
         auto wait = [&](uint64_t *bar, uint32_t parity) {
             if (ok) ok = mbar_wait(bar, parity, p.timeouts);
         };
-        auto logits = [&](int s, uint32_t k_addr) {              // S_s = Q_s K^T
-            if (lane == 0) {
-                const uint32_t a = q_addr + (plan.paired ? s * G::kTileBytes : 0);
+        const uint32_t leader = elected();
+        const uint64_t q_desc = umma_desc(q_addr), ring_k = umma_desc(ring_addr), ring_v = desc_mn(ring_addr, G::kHalfBytes);
+        // descriptors of other addresses: 16-byte units added to the address field, which has room for all of shared memory
+        auto logits = [&](int s, uint32_t slot) {                // S_s = Q_s K^T
+            const uint64_t a = q_desc + (plan.paired ? uint32_t(s * (G::kTileBytes >> 4)) : 0u), b = ring_k + slot * uint32_t(G::kTileBytes >> 4);
+            mma_ss<false>(leader, tmem + 128 * s, a, b, kIdS);
 #pragma unroll
-                for (int i = 0; i < D / 16; ++i) {
-                    const uint32_t off = (i >> 2) * G::kHalfBytes + (i & 3) * 32;
-                    mma_ss(tmem + 128 * s, umma_desc(a + off), umma_desc(k_addr + off), kIdS, i > 0);
-                }
-                umma_commit(&sh.s_full[s]);
+            for (int i = 1; i < D / 16; ++i) {
+                const uint32_t off = ((i >> 2) * G::kHalfBytes + (i & 3) * 32) >> 4;
+                mma_ss<true>(leader, tmem + 128 * s, a + off, b + off, kIdS);
             }
-            __syncwarp();
+            commit(leader, &sh.s_full[s]);
         };
-        auto sums = [&](int s, uint32_t v_addr, bool first) {    // O_s += P_s V
-            if (lane == 0) {
+        auto sums = [&](int s, uint32_t slot, bool first) {      // O_s += P_s V
+            const uint64_t b = ring_v + slot * uint32_t(G::kTileBytes >> 4);
 #pragma unroll
-                for (int i = 0; i < kKvPrefixTile / 16; ++i)
-                    mma_ts(tmem + 256 + G::kOColumns * s, tmem + 128 * s + 8 * i, desc_mn(v_addr + i * 2048, G::kHalfBytes), kIdO, !first || i > 0);
-                umma_commit(&sh.o_done[s]);
-            }
-            __syncwarp();
+            for (int i = 0; i < kKvPrefixTile / 16; ++i)
+                mma_ts(leader, tmem + 256 + G::kOColumns * s, tmem + 128 * s + 8 * i, b + i * (2048 >> 4), kIdO, !first || i > 0);
+            commit(leader, &sh.o_done[s]);
         };
-        auto release = [&](uint32_t slot) {
-            if (lane == 0) umma_commit(&sh.empty[slot]);
-            __syncwarp();
-        };
-        auto next_tile = [&](uint32_t &slot) {                   // waits for the next tile of the ring
-            slot = n % G::kSlots;
-            wait(&sh.full[slot], (n / G::kSlots) & 1);
+        auto release = [&](uint32_t slot) { commit(leader, &sh.empty[slot]); };
+        uint32_t ring_slot = 0, ring_round = 0;
+        auto next_tile = [&] {                                   // waits for the next tile of the ring
+            const uint32_t slot = ring_slot;
+            wait(&sh.full[slot], ring_round & 1);
             fence_after();
-            ++n;
-            return ring_addr + slot * G::kTileBytes;
+            if (++ring_slot == G::kSlots) { ring_slot = 0; ++ring_round; }
+            return slot;
         };
         while (next_part(plan, at, end, w)) {
             wait(&sh.q_ready, parts & 1);
             fence_after();
             ++parts;
-            uint32_t slot;
             auto begin = [&](int i) {                            // logits of tile i
-                const uint32_t k_addr = next_tile(slot);
-                if (plan.paired) { logits(0, k_addr); logits(1, k_addr); }
-                else logits(i & 1, k_addr);
+                const uint32_t slot = next_tile();
+                if (plan.paired) { logits(0, slot); logits(1, slot); }
+                else logits(i & 1, slot);
                 release(slot);
             };
             for (int i = 0; i < min(lookahead, w.count); ++i) begin(i);
             for (int i = 0; i < w.count; ++i) {
-                uint32_t v_slot;
-                const uint32_t v_addr = next_tile(v_slot);
+                const uint32_t v_slot = next_tile();
                 const int64_t left = int64_t(p.prefix_len) - int64_t(w.tile0 + i) * kKvPrefixTile;
                 if (left < kKvPrefixTile) {                      // places behind the prefix may hold anything, and 0 * NaN is not 0
                     uint8_t *v = ring + v_slot * G::kTileBytes;
@@ -225,17 +262,17 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) kv_prefix_kernel(const KvAt
                     __syncwarp();
                 }
                 if (plan.paired) {
-                    uint32_t k_slot = 0, k_addr = 0;
+                    uint32_t k_slot = 0;
                     const bool more = i + 1 < w.count;
 #pragma unroll
                     for (int s = 0; s < 2; ++s) {
                         wait(&sh.p_ready[s], p_count[s]++ & 1);
                         fence_after();
-                        sums(s, v_addr, i == 0);
+                        sums(s, v_slot, i == 0);
                         if (s == 1) release(v_slot);
                         if (more) {
-                            if (s == 0) k_addr = next_tile(k_slot);
-                            logits(s, k_addr);
+                            if (s == 0) k_slot = next_tile();
+                            logits(s, k_slot);
                             if (s == 1) release(k_slot);
                         }
                     }
@@ -243,13 +280,15 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) kv_prefix_kernel(const KvAt
                     const int s = i & 1;
                     wait(&sh.p_ready[s], p_count[s]++ & 1);
                     fence_after();
-                    sums(s, v_addr, i < 2);
+                    sums(s, v_slot, i < 2);
                     release(v_slot);
                     if (i + 2 < w.count) begin(i + 2);
                 }
             }
         }
+    }
     } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kWeightRegs));
         // ---- weights: stream `s`, a row to a thread
         const int s = warp >> 2, r = (warp & 3) * 32 + lane;
         const uint32_t quarter = uint32_t((warp & 3) * 32) << 16, s_addr = tmem + 128 * s + quarter, o_addr = tmem + 256 + G::kOColumns * s + quarter;
@@ -279,13 +318,17 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) kv_prefix_kernel(const KvAt
             if (lane == 0) mbar_arrive(&sh.q_ready);
             float m = -INFINITY, l = 0.0f;
             int done = 0;                                        // tiles of this stream so far
-            for (int i = plan.paired ? 0 : s; i < w.count; i += plan.paired ? 1 : 2, ++done) {
-                // pages outside the pool hold no keys
-                const int64_t tile_key = int64_t(w.tile0 + i) * kKvPrefixTile, left = int64_t(p.prefix_len) - tile_key;
-                const int64_t first = tile_key + 16 * (lane & 7), entry = first >> p.page_shift;
-                int page = -1;
-                if (first < p.prefix_len && entry < p.prefix_width) page = __ldg(p.prefix_pages + entry);
+            // pages outside the pool hold no keys: lane l < 8 looks after keys 16 l .. 16 l + 15 of a tile, one tile ahead
+            auto page_of = [&](int i) {
+                const int64_t first = int64_t(w.tile0 + i) * kKvPrefixTile + 16 * (lane & 7), entry = first >> p.page_shift;
+                return i < w.count && first < p.prefix_len && entry < p.prefix_width ? __ldg(p.prefix_pages + entry) : -1;
+            };
+            const int stride = plan.paired ? 1 : 2;
+            int page = page_of(plan.paired ? 0 : s);
+            for (int i = plan.paired ? 0 : s; i < w.count; i += stride, ++done) {
+                const int64_t left = int64_t(p.prefix_len) - int64_t(w.tile0 + i) * kKvPrefixTile;
                 const uint32_t good = __ballot_sync(kFullMask, page >= 0 && page < p.pages) & 0xffu;
+                page = page_of(i + stride);
                 wait(&sh.s_full[s], s_count++ & 1);
                 fence_after();
                 uint32_t x[128];
@@ -299,10 +342,16 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) kv_prefix_kernel(const KvAt
                 }
                 float top = -INFINITY;
                 {
-                    float t4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+                    float t8[8];
 #pragma unroll
-                    for (int c = 0; c < 128; ++c) t4[c & 3] = fmaxf(t4[c & 3], __uint_as_float(x[c]));
-                    top = fmaxf(fmaxf(t4[0], t4[1]), fmaxf(t4[2], t4[3])) * p.scale_log2;
+                    for (int c = 0; c < 8; ++c) t8[c] = __uint_as_float(x[c]);
+#pragma unroll
+                    for (int c = 8; c < 120; c += 16)
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) t8[j] = fmaxf(fmaxf(t8[j], __uint_as_float(x[c + j])), __uint_as_float(x[c + 8 + j]));
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) t8[j] = fmaxf(t8[j], __uint_as_float(x[120 + j]));
+                    top = fmaxf(fmaxf(fmaxf(t8[0], t8[1]), fmaxf(t8[2], t8[3])), fmaxf(fmaxf(t8[4], t8[5]), fmaxf(t8[6], t8[7]))) * p.scale_log2;
                 }
                 if (done == 0) {
                     m = top;
@@ -323,19 +372,24 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) kv_prefix_kernel(const KvAt
                     }
                     tmem_wait_st();
                 }
-                const float base = m == -INFINITY ? 0.0f : m;
-                float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-                uint32_t pk[64];
+                const float base = m == -INFINITY ? 0.0f : -m;
+                const uint64_t scale2 = pair(p.scale_log2, p.scale_log2), base2 = pair(base, base);
+                uint64_t part[2] = {0, 0};
 #pragma unroll
-                for (int c = 0; c < 64; ++c) {
-                    const float a = kv_exp2(fmaf(__uint_as_float(x[2 * c]), p.scale_log2, -base)), b = kv_exp2(fmaf(__uint_as_float(x[2 * c + 1]), p.scale_log2, -base));
-                    part[(2 * c) & 3] += a;
-                    part[(2 * c + 1) & 3] += b;
-                    pk[c] = KvType<T>::pack(a, b);
+                for (int half = 0; half < 2; ++half) {
+                    uint32_t pk[32];
+#pragma unroll
+                    for (int c = 0; c < 32; ++c) {
+                        const int at = 64 * half + 2 * c;
+                        const float2 y = unpair(fma2(pair(__uint_as_float(x[at]), __uint_as_float(x[at + 1])), scale2, base2));
+                        const float a = kv_exp2(y.x), b = kv_exp2(y.y);
+                        part[c & 1] = add2(part[c & 1], pair(a, b));
+                        pk[c] = KvType<T>::pack(a, b);
+                    }
+                    tmem_st32(s_addr + 32 * half, pk);
                 }
-                l += (part[0] + part[1]) + (part[2] + part[3]);
-                tmem_st32(s_addr, pk);
-                tmem_st32(s_addr + 32, pk + 32);
+                const float2 sums = unpair(add2(part[0], part[1]));
+                l += sums.x + sums.y;
                 tmem_wait_st();
                 fence_before();
                 __syncwarp();
