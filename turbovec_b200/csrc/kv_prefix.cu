@@ -24,6 +24,7 @@ constexpr int kWeightRegs = 208, kOtherRegs = 88;   // registers a thread: 256 *
 static_assert(256 * kWeightRegs + 128 * kOtherRegs <= kPrefixThreads * 168, "more registers than the block has");
 constexpr int kMmaWarp = 8, kCopyWarp = 9;
 constexpr float kRescaleAt = 8.0f;
+constexpr int kByPolynomial = 2;                 // pairs of weights of every eight
 
 template <int D>
 struct PrefixGeometry {
@@ -85,6 +86,12 @@ __device__ __forceinline__ void commit(uint32_t leader, uint64_t *bar) {
         "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}"
         ::"r"(smem_u32(bar)), "r"(leader) : "memory");
 }
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15};"
+        ::"r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
+          "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(taddr) : "memory");
+}
 __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t *r) {
     asm volatile(
         "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], "
@@ -115,6 +122,27 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
     uint64_t d;
     asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
     return d;
+}
+// Largest of three, NaN if one is.
+__device__ __forceinline__ float max3_nan(float a, float b, float c) {
+    float d;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+// 2^y for a pair, -126 <= y < 127, on the multiply-add pipe: y = n + f with n whole and |f| <= 1/2 (adding 1.5 * 2^23 leaves n in the low
+// bits), 2^f by a polynomial of degree 4 (fitted to the smallest largest relative error: 2.7e-6, a hundredth of what rounding
+// the weight to 11 bits leaves), n added to the exponent.
+__device__ __forceinline__ float2 exp2_pair(float2 y) {
+    constexpr float kShift = 12582912.0f;
+    const uint64_t v = pair(fmaxf(y.x, -126.0f), fmaxf(y.y, -126.0f));
+    const uint64_t t = add2(v, pair(kShift, kShift)), n = add2(t, pair(-kShift, -kShift)), f = fma2(n, pair(-1.0f, -1.0f), v);
+    uint64_t r = pair(0x1.3997d4p-7f, 0x1.3997d4p-7f);
+    r = fma2(r, f, pair(0x1.ca1440p-5f, 0x1.ca1440p-5f));
+    r = fma2(r, f, pair(0x1.ec06dap-3f, 0x1.ec06dap-3f));
+    r = fma2(r, f, pair(0x1.62e0dcp-1f, 0x1.62e0dcp-1f));
+    r = fma2(r, f, pair(0x1.ffffe8p-1f, 0x1.ffffe8p-1f));
+    const float2 a = unpair(r), k = unpair(t);
+    return make_float2(__uint_as_float(__float_as_uint(a.x) + (__float_as_uint(k.x) << 23)), __uint_as_float(__float_as_uint(a.y) + (__float_as_uint(k.y) << 23)));
 }
 __device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
@@ -318,24 +346,30 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) kv_prefix_kernel(const KvAt
             if (lane == 0) mbar_arrive(&sh.q_ready);
             float m = -INFINITY, l = 0.0f;
             int done = 0;                                        // tiles of this stream so far
-            // pages outside the pool hold no keys: lane l < 8 looks after keys 16 l .. 16 l + 15 of a tile, one tile ahead
-            auto page_of = [&](int i) {
-                const int64_t first = int64_t(w.tile0 + i) * kKvPrefixTile + 16 * (lane & 7), entry = first >> p.page_shift;
-                return i < w.count && first < p.prefix_len && entry < p.prefix_width ? __ldg(p.prefix_pages + entry) : -1;
+            // pages outside the pool hold no keys: lane l < 8 looks after keys 16 l .. 16 l + 15 of a tile, if the part has any such page
+            auto page_is_good = [&](int64_t key) {
+                const int64_t entry = key >> p.page_shift;
+                const int page = key < p.prefix_len && entry < p.prefix_width ? __ldg(p.prefix_pages + entry) : -1;
+                return page >= 0 && page < p.pages;
             };
+            bool all_good = true;
+            {
+                const int64_t from = int64_t(w.tile0) * kKvPrefixTile, to = min(from + int64_t(w.count) * kKvPrefixTile, int64_t(p.prefix_len));
+                for (int64_t entry = (from >> p.page_shift) + lane; entry << p.page_shift < to; entry += 32) all_good = all_good && page_is_good(entry << p.page_shift);
+                all_good = __all_sync(kFullMask, all_good);
+            }
             const int stride = plan.paired ? 1 : 2;
-            int page = page_of(plan.paired ? 0 : s);
             for (int i = plan.paired ? 0 : s; i < w.count; i += stride, ++done) {
-                const int64_t left = int64_t(p.prefix_len) - int64_t(w.tile0 + i) * kKvPrefixTile;
-                const uint32_t good = __ballot_sync(kFullMask, page >= 0 && page < p.pages) & 0xffu;
-                page = page_of(i + stride);
                 wait(&sh.s_full[s], s_count++ & 1);
                 fence_after();
                 uint32_t x[128];
 #pragma unroll
                 for (int c = 0; c < 4; ++c) tmem_ld32(s_addr + 32 * c, reinterpret_cast<uint32_t (&)[32]>(x[32 * c]));
                 tmem_wait_ld();
-                if (good != 0xffu || left < kKvPrefixTile) {
+                const int64_t left = int64_t(p.prefix_len) - int64_t(w.tile0 + i) * kKvPrefixTile;
+                const bool border = !all_good || left < kKvPrefixTile;
+                if (border) {
+                    const uint32_t good = __ballot_sync(kFullMask, page_is_good(int64_t(w.tile0 + i) * kKvPrefixTile + 16 * (lane & 7)));
 #pragma unroll
                     for (int c = 0; c < 128; ++c)
                         if (c >= left || !((good >> (c >> 4)) & 1u)) x[c] = 0xff800000u;
@@ -344,19 +378,21 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) kv_prefix_kernel(const KvAt
                 {
                     float t8[8];
 #pragma unroll
-                    for (int c = 0; c < 8; ++c) t8[c] = __uint_as_float(x[c]);
+                    for (int j = 0; j < 8; ++j) t8[j] = __uint_as_float(x[j]);
 #pragma unroll
                     for (int c = 8; c < 120; c += 16)
 #pragma unroll
-                        for (int j = 0; j < 8; ++j) t8[j] = fmaxf(fmaxf(t8[j], __uint_as_float(x[c + j])), __uint_as_float(x[c + 8 + j]));
+                        for (int j = 0; j < 8; ++j) t8[j] = max3_nan(t8[j], __uint_as_float(x[c + j]), __uint_as_float(x[c + 8 + j]));
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) t8[j] = fmaxf(t8[j], __uint_as_float(x[120 + j]));
-                    top = fmaxf(fmaxf(fmaxf(t8[0], t8[1]), fmaxf(t8[2], t8[3])), fmaxf(fmaxf(t8[4], t8[5]), fmaxf(t8[6], t8[7]))) * p.scale_log2;
+                    for (int j = 0; j < 8; j += 2) t8[j] = max3_nan(max3_nan(t8[j], t8[j + 1], __uint_as_float(x[120 + j])), __uint_as_float(x[121 + j]), t8[j]);
+                    top = max3_nan(max3_nan(t8[0], t8[2], t8[4]), t8[6], t8[6]) * p.scale_log2;
                 }
+                top = top < INFINITY ? top : NAN;                // an infinite logit makes the row NaN, as inf - inf does
                 if (done == 0) {
                     m = top;
-                } else if (__any_sync(kFullMask, top > m + kRescaleAt)) {
-                    const float next = fmaxf(m, top), f = next == -INFINITY ? 1.0f : kv_exp2(m - next);
+                } else if (__any_sync(kFullMask, !(top <= m + kRescaleAt))) {
+                    // (a NaN becomes the maximum: the polynomial below would lose it)
+                    const float next = max3_nan(m, top, top), f = next == -INFINITY ? 1.0f : kv_exp2(m - next);
                     m = next;
                     l *= f;
                     wait(&sh.o_done[s], (o_count + done - 1) & 1);
@@ -376,17 +412,21 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) kv_prefix_kernel(const KvAt
                 const uint64_t scale2 = pair(p.scale_log2, p.scale_log2), base2 = pair(base, base);
                 uint64_t part[2] = {0, 0};
 #pragma unroll
-                for (int half = 0; half < 2; ++half) {
-                    uint32_t pk[32];
+                for (int c = 0; c < 4; ++c) {
+                    uint32_t pk[16];
 #pragma unroll
-                    for (int c = 0; c < 32; ++c) {
-                        const int at = 64 * half + 2 * c;
-                        const float2 y = unpair(fma2(pair(__uint_as_float(x[at]), __uint_as_float(x[at + 1])), scale2, base2));
-                        const float a = kv_exp2(y.x), b = kv_exp2(y.y);
-                        part[c & 1] = add2(part[c & 1], pair(a, b));
-                        pk[c] = KvType<T>::pack(a, b);
+                    for (int j = 0; j < 16; ++j) {
+                        const int at = 32 * c + 2 * j;
+                        const float2 z = unpair(fma2(pair(__uint_as_float(x[at]), __uint_as_float(x[at + 1])), scale2, base2));
+                        // some of the weights by the multiply-add pipe: the exponential unit gives 4 a cycle to each scheduler and
+                        // would take 2,048 cycles a step
+                        float2 e;
+                        if ((j & 7) < kByPolynomial) e = exp2_pair(z);
+                        else e = make_float2(kv_exp2(z.x), kv_exp2(z.y));
+                        part[j & 1] = add2(part[j & 1], pair(e.x, e.y));
+                        pk[j] = KvType<T>::pack(e.x, e.y);
                     }
-                    tmem_st32(s_addr + 32 * half, pk);
+                    tmem_st16(s_addr + 16 * c, pk);
                 }
                 const float2 sums = unpair(add2(part[0], part[1]));
                 l += sums.x + sums.y;
