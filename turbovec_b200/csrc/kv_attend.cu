@@ -25,15 +25,15 @@ __device__ uint32_t g_kv_timeouts;
 
 template <int D>
 struct Geometry {
-    static constexpr int kStages = D == 128 ? 3 : 6;
+    static constexpr int kStages = D == 128 ? 2 : 4;      // 64 KB in flight a block, two blocks to a multiprocessor
     static constexpr int kHalfBytes = kKvTile * 128;      // 64 channels of a tile
     static constexpr int kOperandBytes = kHalfBytes * (D / 64);
     static constexpr int kStageBytes = 2 * kOperandBytes;
 };
 template <int D>
 struct AttendShared {
-    float o[kKvRows][D];
-    float2 ml[kConsumers][kKvRows];
+    float o[kConsumers][kKvRows][D + 4];
+    float2 ml[kConsumers][kKvRows], total[kKvRows];
     int first_key[Geometry<D>::kStages][kConsumers];
     int64_t scratch[2 * (kAttendThreads / 32) + 3];
     uint64_t full[Geometry<D>::kStages], empty[Geometry<D>::kStages];
@@ -45,6 +45,7 @@ struct Part {
     int item, row0, rows;          // rows of the call's q: (token, head of the group) pairs row0 .. row0 + rows of `first_token` on
     int first_token, h, b;         // b = -1: prefix
     int tile0, tile1, item_tiles;  // tiles of this part, and of the item
+    int64_t pos;                   // position of first_token in its sequence
     int64_t item_start;            // place of the item's first tile in the whole list
 };
 
@@ -86,28 +87,28 @@ struct Walk {
                 const int m = item % mt, th = item / mt;
                 begin = int64_t(item) * places;
                 out.item = item; out.b = 0; out.item_tiles = chosen_tiles();
-                out.h = th % p.kv_heads; out.first_token = live_first + th / p.kv_heads;
+                out.h = th % p.kv_heads; out.first_token = live_first + th / p.kv_heads; out.pos = p.token_pos[out.first_token];
                 out.row0 = m * kKvRows; out.rows = min(kKvRows, p.group - out.row0);
             } else if (at < prefix_total) {
                 const int places = p.item_cost + prefix_tiles, item = int(divide(at, places));
                 const int m = item % prefix_mt;
                 begin = int64_t(item) * places;
-                out.item = item; out.b = -1; out.h = item / prefix_mt; out.first_token = live_first; out.item_tiles = prefix_tiles;
+                out.item = item; out.b = -1; out.h = item / prefix_mt; out.first_token = live_first; out.item_tiles = prefix_tiles; out.pos = 0;
                 out.row0 = m * kKvRows; out.rows = int(min(int64_t(kKvRows), int64_t(live) * p.group - out.row0));
             } else {
                 KvSpan sp = span(b);
-                int mt = row_tiles(sp.count), places = p.item_cost + tiles_of(p.batch.lens[b]);
+                int len = p.batch.lens[b], mt = row_tiles(sp.count), places = p.item_cost + tiles_of(len);
                 while (at - start_of_b >= int64_t(mt) * p.kv_heads * places) {
                     if (b + 1 >= p.batch.sequences) return false;
                     start_of_b += int64_t(mt) * p.kv_heads * places;
                     item_of_b += mt * p.kv_heads;
                     ++b;
-                    sp = span(b); mt = row_tiles(sp.count); places = p.item_cost + tiles_of(p.batch.lens[b]);
+                    sp = span(b); len = p.batch.lens[b]; mt = row_tiles(sp.count); places = p.item_cost + tiles_of(len);
                 }
                 const int item = int(divide(at - start_of_b, places));
                 const int m = item % mt;
                 begin = start_of_b + int64_t(item) * places;
-                out.item = item_of_b + item; out.b = b; out.h = item / mt; out.first_token = sp.first; out.item_tiles = places - p.item_cost;
+                out.item = item_of_b + item; out.b = b; out.h = item / mt; out.first_token = sp.first; out.item_tiles = places - p.item_cost; out.pos = int64_t(len) - sp.count;
                 out.row0 = m * kKvRows; out.rows = int(min(int64_t(kKvRows), int64_t(sp.count) * p.group - out.row0));
             }
             out.item_start = begin + p.item_cost;
@@ -120,20 +121,19 @@ struct Walk {
         return false;
     }
     __device__ __forceinline__ int chosen_tiles() const { return ((p.budget << p.page_shift) + kKvTile - 1) / kKvTile; }
-    // keys that row `r` of the part sees: those before this position
-    __device__ __forceinline__ int limit(const Part &w, int r) const {
-        if constexpr (CHOSEN) return p.token_pos[w.first_token] + 1;
+    // keys that token `j` (of first_token on) of the part sees: those before this position
+    __device__ __forceinline__ int limit(const Part &w, int j) const {
+        if constexpr (CHOSEN) return int(w.pos) + 1;
         if (w.b < 0) return p.prefix_len;
-        const KvSpan sp = span(w.b);
-        return kv_visible(int64_t(p.batch.lens[w.b]) - sp.count + (w.row0 + r) / p.group, kv_capacity(p.batch.table_width, p.page_shift));
+        return kv_visible(w.pos + j, kv_capacity(p.batch.table_width, p.page_shift));
     }
     // one past the last tile of the part that some row sees a key of
     __device__ __forceinline__ int last_tile(const Part &w) const {
         if constexpr (CHOSEN) {                              // the list is shorter where the sequence has fewer pages
-            const int64_t keys = (int64_t(p.token_pos[w.first_token]) >> p.page_shift) + 1 << p.page_shift;
+            const int64_t keys = ((w.pos >> p.page_shift) + 1) << p.page_shift;
             return int(min(int64_t(w.tile1), (keys + kKvTile - 1) / kKvTile));
         }
-        return min(w.tile1, (limit(w, w.rows - 1) + kKvTile - 1) / kKvTile);
+        return min(w.tile1, (limit(w, (w.row0 + w.rows - 1) / p.group) + kKvTile - 1) / kKvTile);
     }
 };
 
@@ -335,13 +335,12 @@ __global__ void __launch_bounds__(kAttendThreads, 2) kv_attend_kernel(const KvAt
     while (walk.next(w)) {
         const int last = walk.last_tile(w);
         uint32_t qf[D / 16][4];
-        auto q_row = [&](int r) -> const T * {
-            const int row = w.row0 + r;
-            return static_cast<const T *>(p.q.data) + int64_t(w.first_token + row / p.group) * p.q.token_stride +
-                   int64_t(w.h * p.group + row % p.group) * p.q.head_stride;
-        };
         const bool have0 = r0 < w.rows, have1 = r1 < w.rows;
-        const T *q0 = q_row(have0 ? r0 : 0), *q1 = q_row(have1 ? r1 : 0);
+        const int row0 = w.row0 + (have0 ? r0 : 0), row1 = w.row0 + (have1 ? r1 : 0);
+        const int j0 = row0 / p.group, j1 = row1 / p.group;              // tokens of the two rows, and their heads
+        const int head0 = w.h * p.group + row0 - j0 * p.group, head1 = w.h * p.group + row1 - j1 * p.group;
+        const T *q0 = static_cast<const T *>(p.q.data) + int64_t(w.first_token + j0) * p.q.token_stride + int64_t(head0) * p.q.head_stride;
+        const T *q1 = static_cast<const T *>(p.q.data) + int64_t(w.first_token + j1) * p.q.token_stride + int64_t(head1) * p.q.head_stride;
 #pragma unroll
         for (int i = 0; i < D / 16; ++i) {
             qf[i][0] = have0 ? *reinterpret_cast<const uint32_t *>(q0 + 16 * i + c2) : 0u;
@@ -349,8 +348,8 @@ __global__ void __launch_bounds__(kAttendThreads, 2) kv_attend_kernel(const KvAt
             qf[i][2] = have0 ? *reinterpret_cast<const uint32_t *>(q0 + 16 * i + 8 + c2) : 0u;
             qf[i][3] = have1 ? *reinterpret_cast<const uint32_t *>(q1 + 16 * i + 8 + c2) : 0u;
         }
-        const int lim0 = have0 ? walk.limit(w, r0) : 0, lim1 = have1 ? walk.limit(w, r1) : 0;
-        const int lim_first = walk.limit(w, 0), lim_last = walk.limit(w, w.rows - 1);
+        const int lim0 = have0 ? walk.limit(w, j0) : 0, lim1 = have1 ? walk.limit(w, j1) : 0;
+        const int lim_first = walk.limit(w, w.row0 / p.group), lim_last = walk.limit(w, (w.row0 + w.rows - 1) / p.group);
         float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.0f, l1 = 0.0f;
         float o[D / 8][4];
 #pragma unroll
@@ -479,51 +478,49 @@ __global__ void __launch_bounds__(kAttendThreads, 2) kv_attend_kernel(const KvAt
         }
         const float f0 = kv_exp2(m0 - base0), f1 = kv_exp2(m1 - base1);
 #pragma unroll
-        for (int j = 0; j < D / 8; ++j) { o[j][0] *= f0; o[j][1] *= f0; o[j][2] *= f1; o[j][3] *= f1; }
-#pragma unroll 1
-        for (int i = kConsumers - 1; i >= 0; --i) {
-            if (warp == i) {
-#pragma unroll
-                for (int j = 0; j < D / 8; ++j) {
-                    const int col = (8 * j + c2) ^ (r0 * 8);           // rows lie a multiple of 32 words apart: spread their banks
-                    float2 *a = reinterpret_cast<float2 *>(&sh.o[r0][col]), *b = reinterpret_cast<float2 *>(&sh.o[r1][col]);
-                    if (i < kConsumers - 1) {
-                        o[j][0] += a->x; o[j][1] += a->y;
-                        o[j][2] += b->x; o[j][3] += b->y;
-                    }
-                    if (i > 0) { *a = make_float2(o[j][0], o[j][1]); *b = make_float2(o[j][2], o[j][3]); }
-                }
-            }
-            consumers_sync();
+        for (int j = 0; j < D / 8; ++j) {
+            *reinterpret_cast<float2 *>(&sh.o[warp][r0][8 * j + c2]) = make_float2(o[j][0] * f0, o[j][1] * f0);
+            if (w.rows > 8) *reinterpret_cast<float2 *>(&sh.o[warp][r1][8 * j + c2]) = make_float2(o[j][2] * f1, o[j][3] * f1);
         }
-        if (warp != 0) continue;
+        // the sums for the rows, where a lane that writes a row's result finds them
+        if (warp == 0 && (lane & 3) == 0) { sh.total[r0] = make_float2(big0, sum0); sh.total[r1] = make_float2(big1, sum1); }
+        consumers_sync();
+        // row after row: a warp every fourth, a lane D / 32 channels
         const bool whole = w.tile0 == 0 && w.tile1 == w.item_tiles && p.prefix_len == 0;
         const int64_t slot = int64_t(w.item) + blockIdx.x;
-        auto finish = [&](int r, bool have, float big, float sum, int e) {
-            if (!have) return;
-            const int row = w.row0 + r;
-            const int64_t token = w.first_token + row / p.group, head = w.h * p.group + row % p.group;
-            if (whole) {
-                const float inv = sum > 0.0f || sum != sum ? 1.0f / sum : 0.0f;            // no key: zero
-                T *dst = static_cast<T *>(p.out.data) + token * p.out.token_stride + head * p.out.head_stride;
+        for (int r = warp; r < w.rows; r += kConsumers) {
+            constexpr int kPer = D / 32;
+            float x[kPer] = {};
 #pragma unroll
-                for (int j = 0; j < D / 8; ++j) *reinterpret_cast<uint32_t *>(dst + 8 * j + c2) = KvType<T>::pack(o[j][e] * inv, o[j][e + 1] * inv);
-                if (c2 == 0 && p.lse) p.lse[token * p.heads + head] = sum > 0.0f || sum != sum ? (big + log2f(sum)) * 0.6931471805599453f : -INFINITY;
-            } else if (slot < p.slots) {
-                float *dst = p.part_o + (slot * kKvRows + r) * D;
-#pragma unroll
-                for (int j = 0; j < D / 8; ++j) *reinterpret_cast<float2 *>(dst + 8 * j + c2) = make_float2(o[j][e], o[j][e + 1]);
-                if (c2 == 0) p.part_ml[slot * kKvRows + r] = make_float2(big, sum);
+            for (int i = 0; i < kConsumers; ++i) {
+                const float *src = &sh.o[i][r][lane * kPer];
+                if constexpr (kPer == 4) { const float4 y = *reinterpret_cast<const float4 *>(src); x[0] += y.x; x[1] += y.y; x[2] += y.z; x[3] += y.w; }
+                else { const float2 y = *reinterpret_cast<const float2 *>(src); x[0] += y.x; x[1] += y.y; }
             }
-            if (c2 == 0 && w.tile0 == 0) {                      // where the parts of the item lie, packed with the row within a slot
+            const float2 total = sh.total[r];
+            const int row = w.row0 + r, j = row / p.group;
+            const int64_t token = w.first_token + j, head = w.h * p.group + row - j * p.group;
+            if (whole) {
+                const bool any = total.y > 0.0f || total.y != total.y;
+                const float inv = any ? 1.0f / total.y : 0.0f;             // no key: zero
+                uint32_t *dst = reinterpret_cast<uint32_t *>(static_cast<T *>(p.out.data) + token * p.out.token_stride + head * p.out.head_stride + lane * kPer);
+#pragma unroll
+                for (int i = 0; i < kPer / 2; ++i) dst[i] = KvType<T>::pack(x[2 * i] * inv, x[2 * i + 1] * inv);
+                if (lane == 0 && p.lse) p.lse[token * p.heads + head] = any ? (total.x + log2f(total.y)) * 0.6931471805599453f : -INFINITY;
+            } else if (slot < p.slots) {
+                float *dst = p.part_o + (slot * kKvRows + r) * D + lane * kPer;
+                if constexpr (kPer == 4) *reinterpret_cast<float4 *>(dst) = make_float4(x[0], x[1], x[2], x[3]);
+                else *reinterpret_cast<float2 *>(dst) = make_float2(x[0], x[1]);
+                if (lane == 0) p.part_ml[slot * kKvRows + r] = total;
+            }
+            if (lane == 0 && w.tile0 == 0) {                               // where the parts of the item lie
                 const int64_t begin = divide(w.item_start, per), finish_at = divide(w.item_start + w.item_tiles - 1, per);
                 const KvPieces pc{(w.item + begin) * kKvRows + r, whole ? 0 : int(finish_at - begin + 1), 0};
                 (w.b < 0 ? p.prefix_pieces : p.own_pieces)[token * p.heads + head] = pc;
             }
-        };
-        finish(r0, have0, big0, sum0, 0);
-        finish(r1, have1, big1, sum1, 2);
+        }
     }
+    if (!CHOSEN && p.tensor_prefix) asm volatile("griddepcontrol.wait;" ::: "memory");
 }
 
 // Joins the parts of a row (token, head): WARPS warps each take every WARPS-th part.
