@@ -70,6 +70,9 @@ ATTEND = [
     (BF, 128, 128, 16, 2, [1] * 17, [2] * 17, 900, False, 0),               # 136: two row tiles
     (FP, 128, 32, 10, 1, [1, 3, 2] * 9, [4] * 27, 5000, True, 1),           # 540 rows, three pairs
     (BF, 64, 64, 24, 8, [2] * 50, [70] * 50, 2050, False, 0),               # 300 rows, eight key heads
+    (BF, 128, 64, 24, 2, [1] * 3, [9] * 3, 192, False, 0),                  # half a tile of keys at the end
+    (FP, 128, 32, 24, 2, [1] * 30, [9] * 30, 193, False, 0),
+    (FP, 64, 128, 24, 1, [1] * 3, [9] * 3, 40_000, False, 0),               # several tiles to a block
 ]
 
 

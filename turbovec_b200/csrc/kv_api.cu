@@ -90,22 +90,30 @@ KvRows rows_of(const tv_kv_rows *r) { return r ? KvRows{r->data, r->token_stride
 KvBatch batch_of(const tv_kv_batch *b) { return {b->table, b->lens, b->offsets, b->table_stride, int(b->table_width), int(b->sequences)}; }
 int shift_of(int page_size) { return page_size == 16 ? 4 : page_size == 32 ? 5 : page_size == 64 ? 6 : 7; }
 
-// Tensor map (channel, token, head, page) of K or V; boxes of 64 channels (128 bytes, swizzled) by `box_tokens` tokens.
-bool make_map(CUtensorMap *map, const tv_kv_cache *c, void *base, int64_t page, int64_t head, int64_t token, int box_tokens) {
+// Tensor map of four dimensions, channels first (strides of the others in elements); boxes of 64 channels (128 bytes, swizzled) by
+// box1 x 1 x box3.
+bool make_map(CUtensorMap *map, const tv_kv_cache *c, void *base, const int64_t (&dims)[3], const int64_t (&strides)[3], int box1, int box3) {
     typedef CUresult (*EncodeTiledFn)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *, const cuuint32_t *,
                                       const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
     const EncodeTiledFn enc = reinterpret_cast<EncodeTiledFn>(tensor_map_encoder());
     if (!enc) return false;
-    const cuuint64_t dims[4] = {cuuint64_t(c->head_dim), cuuint64_t(c->page_size), cuuint64_t(c->kv_heads), cuuint64_t(c->pages)};
-    const cuuint64_t strides[3] = {cuuint64_t(2 * token), cuuint64_t(2 * head), cuuint64_t(2 * page)};
-    const cuuint32_t box[4] = {64, cuuint32_t(box_tokens), 1, 1}, step[4] = {1, 1, 1, 1};
+    const cuuint64_t d[4] = {cuuint64_t(c->head_dim), cuuint64_t(dims[0]), cuuint64_t(dims[1]), cuuint64_t(dims[2])};
+    const cuuint64_t st[3] = {cuuint64_t(2 * strides[0]), cuuint64_t(2 * strides[1]), cuuint64_t(2 * strides[2])};
+    const cuuint32_t box[4] = {64, cuuint32_t(box1), 1, cuuint32_t(box3)}, step[4] = {1, 1, 1, 1};
     const CUtensorMapDataType type = c->dtype == TV_KV_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
-    return enc(map, type, 4, base, dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+    return enc(map, type, 4, base, d, st, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
+// (channel, token, key head, page) of K and V
 bool make_maps(KvMaps *m, const tv_kv_cache *c, int box_tokens) {
-    return make_map(&m->k, c, c->k, c->k_page_stride, c->k_head_stride, c->k_token_stride, box_tokens) &&
-           make_map(&m->v, c, c->v, c->v_page_stride, c->v_head_stride, c->v_token_stride, box_tokens);
+    const int64_t dims[3] = {c->page_size, c->kv_heads, c->pages};
+    return make_map(&m->k, c, c->k, dims, {c->k_token_stride, c->k_head_stride, c->k_page_stride}, box_tokens, 1) &&
+           make_map(&m->v, c, c->v, dims, {c->v_token_stride, c->v_head_stride, c->v_page_stride}, box_tokens, 1);
+}
+// (channel, head of the group, key head, token) of Q, whole tokens to a tile of rows
+bool make_query_map(KvMaps *m, const tv_kv_cache *c, const tv_kv_rows *q, int64_t tokens, int group, int rows) {
+    const int64_t dims[3] = {group, c->kv_heads, tokens};
+    return make_map(&m->q, c, q->data, dims, {q->head_stride, group * q->head_stride, q->token_stride}, group, rows / group);
 }
 
 // Cuts a workspace into arrays, each on a 256-byte boundary; with a null base it only counts.
@@ -122,9 +130,9 @@ struct Carver {
 // Rows (tokens x heads of a key head) from which a prefix goes to the tensor cores.
 constexpr int64_t kTensorRows = 17;
 void plan_prefix(KvAttendParams &p, const tv_kv_cache *c, int64_t tokens, int heads, int64_t prefix_len, int sm_count) {
-    const int64_t rows = tokens * (heads / c->kv_heads);
-    p.tensor_prefix = prefix_len > 0 && rows >= kTensorRows;
-    if (p.tensor_prefix) p.plan = kv_prefix_plan(rows, c->kv_heads, int(prefix_len), sm_count);
+    const int group = heads / c->kv_heads;
+    p.tensor_prefix = prefix_len > 0 && tokens * group >= kTensorRows && group <= kKvPrefixRows;     // a tile holds whole tokens
+    if (p.tensor_prefix) p.plan = kv_prefix_plan(tokens, group, c->kv_heads, int(prefix_len), sm_count);
 }
 size_t carve_attend(KvAttendParams &p, char *base, int64_t slots, int64_t rows, const tv_kv_cache *c, bool prefix) {
     Carver w{base};
@@ -261,7 +269,7 @@ int tv_kv_attend(const tv_kv_cache *c, const tv_kv_batch *b, int64_t tokens, int
     cudaError_t e;
     if (p.tensor_prefix) {
         KvMaps wide;
-        if (!make_maps(&wide, c, c->page_size)) return set_create_error(TV_ERR_CUDA, "the tensor maps of the cache cannot be made");
+        if (!make_maps(&wide, c, c->page_size) || !make_query_map(&wide, c, q, tokens, p.group, p.plan.rows)) return set_create_error(TV_ERR_CUDA, "the tensor maps of the cache cannot be made");
         e = launch_kv_prefix(p, wide, c->dtype, c->head_dim, c->device, static_cast<cudaStream_t>(stream));
         if (e != cudaSuccess) return cuda_error("prefix kernel", e);
     }

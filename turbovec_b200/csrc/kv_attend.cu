@@ -587,7 +587,7 @@ __global__ void __launch_bounds__(128) kv_join_kernel(const KvAttendParams p) {
         const int first = int(int64_t(h) * w.tiles / w.per), count = int((int64_t(h + 1) * w.tiles - 1) / w.per) - first + 1;
         const int64_t block = int64_t(kKvPrefixRows) * D;
         if (w.paired) {
-            const int64_t at = ((int64_t(h) + first) * w.units + r / (2 * kKvPrefixRows)) * 2 * kKvPrefixRows + r % (2 * kKvPrefixRows);
+            const int64_t at = ((int64_t(h) + first) * w.units * 2 + r / w.rows) * kKvPrefixRows + r % w.rows;
             add(p.pre_o + at * D, p.pre_ml + at, 2 * w.units * block, count);
         } else {
             const int64_t at = (int64_t(h) + first) * 2 * kKvPrefixRows + r;

@@ -182,16 +182,19 @@ struct KvPieces {
 constexpr int kKvPrefixRows = 128;           // M of tcgen05.mma
 constexpr int kKvPrefixTile = 128;           // keys of one step
 struct KvPrefixPlan {                        // the same on host and device but for `live_rows`
+    int rows;                                // rows of a tile: whole tokens
     bool paired;                             // two row tiles to a block, which share its keys; else one, its keys dealt to two streams
     int units;                               // row tiles (or pairs) of a key head
     int tiles;                               // key tiles
     int groups;                              // blocks of one unit: they share the (key head, tile) list
     int64_t per;                             // steps of a block
 };
-__host__ __device__ inline KvPrefixPlan kv_prefix_plan(int64_t rows, int kv_heads, int prefix_len, int sm_count) {
+inline KvPrefixPlan kv_prefix_plan(int64_t tokens, int group, int kv_heads, int prefix_len, int sm_count) {
     KvPrefixPlan w;
-    w.paired = rows > kKvPrefixRows;
-    w.units = int(w.paired ? (rows + 2 * kKvPrefixRows - 1) / (2 * kKvPrefixRows) : 1);
+    w.rows = kKvPrefixRows / group * group;
+    const int64_t row_tiles = (tokens * group + w.rows - 1) / w.rows;
+    w.paired = row_tiles > 1;
+    w.units = int(w.paired ? (row_tiles + 1) / 2 : 1);
     w.tiles = (prefix_len + kKvPrefixTile - 1) / kKvPrefixTile;
     const int64_t steps = int64_t(kv_heads) * w.tiles;
     int64_t groups = w.units < sm_count ? sm_count / w.units : 1;
@@ -228,6 +231,7 @@ struct KvAttendParams {
 };
 struct KvMaps {
     CUtensorMap k, v;                        // (channel, token, key head, page), boxes of 64 channels
+    CUtensorMap q;                           // (channel, head of the group, key head, token); for the prefix kernel alone
 };
 // Upper bound of the slots that `grid` blocks can use.
 inline int64_t kv_attend_slots(int64_t tokens, int64_t sequences, int group, int kv_heads, bool prefix, int grid) {

@@ -23,6 +23,7 @@ constexpr int kPrefixThreads = 12 * 32;          // 2 x 4 warps of weights, one 
 constexpr int kWeightRegs = 208, kOtherRegs = 88;   // registers a thread: 256 * 208 + 128 * 88 = 384 * 168, what the block starts with
 static_assert(256 * kWeightRegs + 128 * kOtherRegs <= kPrefixThreads * 168, "more registers than the block has");
 constexpr int kMmaWarp = 8, kCopyWarp = 9;
+constexpr int kHalfKeys = kKvPrefixTile / 2;
 constexpr float kRescaleAt = 8.0f;
 constexpr int kByPolynomial = 2;                 // pairs of weights of every eight
 
@@ -37,7 +38,7 @@ struct PrefixGeometry {
 template <int D>
 struct PrefixShared {
     uint64_t full[PrefixGeometry<D>::kSlots], empty[PrefixGeometry<D>::kSlots];
-    uint64_t s_full[2], p_ready[2], o_done[2], q_ready;
+    uint64_t s_full[2], p_ready[2][2], o_done[2], q_full[2], q_free[2];       // [stream], [stream][half of P]
     uint32_t tmem_base;
 };
 
@@ -170,26 +171,39 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) kv_prefix_kernel(const KvAt
     uint8_t *q_smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     uint8_t *ring = q_smem + G::kQBytes;
     PrefixShared<D> &sh = *reinterpret_cast<PrefixShared<D> *>(ring + G::kSlots * G::kTileBytes);
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    // the warp's number and the tensor-memory address come from lane 0, so that the compiler knows them to be the same in all lanes and keeps
+    // what follows from them (branches, descriptors) in uniform registers
+    const int tid = threadIdx.x, warp = __shfl_sync(kFullMask, tid >> 5, 0), lane = tid & 31;
     const KvPrefixPlan plan = p.plan;
     const int unit = blockIdx.x % plan.units, group = blockIdx.x / plan.units;
     if (tid == 0) {
         for (int s = 0; s < G::kSlots; ++s) { mbar_init(&sh.full[s], 1); mbar_init(&sh.empty[s], 1); }
-        for (int s = 0; s < 2; ++s) { mbar_init(&sh.s_full[s], 1); mbar_init(&sh.p_ready[s], 4); mbar_init(&sh.o_done[s], 1); }
-        mbar_init(&sh.q_ready, 8);
+        for (int s = 0; s < 2; ++s) {
+            mbar_init(&sh.s_full[s], 1); mbar_init(&sh.o_done[s], 1);
+            mbar_init(&sh.q_full[s], 1); mbar_init(&sh.q_free[s], 8);
+            for (int b = 0; b < 2; ++b) mbar_init(&sh.p_ready[s][b], 4);
+        }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == kMmaWarp) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sh.tmem_base)), "r"(512u) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
+    // rows of a tile that no copy writes
+    for (int i = tid; i < 2 * (D / 64) * (kKvPrefixRows - plan.rows) * 8; i += kPrefixThreads) {
+        const int half = i / ((kKvPrefixRows - plan.rows) * 8), rest = i % ((kKvPrefixRows - plan.rows) * 8);
+        *reinterpret_cast<uint4 *>(q_smem + half * G::kHalfBytes + plan.rows * 128 + rest * 16) = make_uint4(0, 0, 0, 0);
+    }
+    fence_shared_async();
     fence_before();
     __syncthreads();
     fence_after();
-    const uint32_t tmem = sh.tmem_base;
+    const uint32_t tmem = __shfl_sync(kFullMask, sh.tmem_base, 0);
     // the attention kernel that follows does not wait for this one before it reads: what both read must be there by now
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;");
+    const KvSpan all = kv_span(p.batch.offsets[0], p.batch.offsets[p.batch.sequences], p.tokens);
+    const int q_first = all.first, q_count = all.count;
     const int64_t steps = int64_t(p.kv_heads) * plan.tiles;
     int64_t at = min(steps, group * plan.per);
     const int64_t end = min(steps, at + plan.per);
@@ -223,7 +237,22 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) kv_prefix_kernel(const KvAt
                     tma_load_page(ring + s * G::kTileBytes + c * G::kHalfBytes + lane * box * 128, map, c * 64, int(key & ((1 << p.page_shift) - 1)), part.h, page, &sh.full[s]);
             ++n;
         };
+        uint32_t parts = 0;
         while (next_part(plan, at, end, w)) {
+            // rows of Q: whole tokens, plan.rows of them to a tile; those behind the last token are zeros
+            for (int s = 0; s < (plan.paired ? 2 : 1); ++s) {
+                if (ok && parts > 0) ok = mbar_wait(&sh.q_free[s], (parts - 1) & 1, p.timeouts);
+                ok = __all_sync(kFullMask, ok);
+                if (!ok) break;
+                if (lane == 0) {
+                    mbar_arrive_expect_tx(&sh.q_full[s], uint32_t(plan.rows * 128 * (D / 64)));
+                    const int token = q_first + (plan.paired ? 2 * unit + s : unit) * (plan.rows / p.group);
+                    for (int c = 0; c < D / 64; ++c)
+                        tma_load_page(q_smem + s * G::kTileBytes + c * G::kHalfBytes, &maps.q, c * 64, 0, w.h, token, &sh.q_full[s]);
+                }
+                __syncwarp();
+            }
+            ++parts;
             for (int i = 0; i < min(lookahead, w.count); ++i) load(w, i, &maps.k);
             for (int i = 0; i < w.count; ++i) {
                 load(w, i, &maps.v);
@@ -231,7 +260,10 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) kv_prefix_kernel(const KvAt
             }
         }
         if (!ok)                                                 // the copies in flight land before the block ends
+        {
             for (uint32_t i = n > G::kSlots ? n - G::kSlots : 0; i < n; ++i) mbar_wait(&sh.full[i % G::kSlots], (i / G::kSlots) & 1, p.timeouts);
+            for (int s = 0; s < (plan.paired ? 2 : 1) && parts > 0; ++s) mbar_wait(&sh.q_full[s], (parts - 1) & 1, p.timeouts);
+        }
     } else if (warp == kMmaWarp) {
         uint32_t parts = 0, p_count[2] = {0, 0};
         constexpr uint32_t kIdS = idesc<T>(128, false), kIdO = idesc<T>(D, true);
@@ -252,11 +284,17 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) kv_prefix_kernel(const KvAt
             }
             commit(leader, &sh.s_full[s]);
         };
-        auto sums = [&](int s, uint32_t slot, bool first) {      // O_s += P_s V
+        // O_s += P_s V, in two halves of the keys: the first begins while the weights of the second are being computed
+        auto sums = [&](int s, uint32_t slot, bool first) {
             const uint64_t b = ring_v + slot * uint32_t(G::kTileBytes >> 4);
+            for (int half = 0; half < 2; ++half) {
+                wait(&sh.p_ready[s][half], p_count[s] & 1);
+                fence_after();
 #pragma unroll
-            for (int i = 0; i < kKvPrefixTile / 16; ++i)
-                mma_ts(leader, tmem + 256 + G::kOColumns * s, tmem + 128 * s + 8 * i, b + i * (2048 >> 4), kIdO, !first || i > 0);
+                for (int i = 0; i < kHalfKeys / 16; ++i)
+                    mma_ts(leader, tmem + 256 + G::kOColumns * s, tmem + 128 * s + 8 * (4 * half + i), b + (4 * half + i) * (2048 >> 4), kIdO, !first || half + i > 0);
+            }
+            ++p_count[s];
             commit(leader, &sh.o_done[s]);
         };
         auto release = [&](uint32_t slot) { commit(leader, &sh.empty[slot]); };
@@ -269,7 +307,7 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) kv_prefix_kernel(const KvAt
             return slot;
         };
         while (next_part(plan, at, end, w)) {
-            wait(&sh.q_ready, parts & 1);
+            for (int s = 0; s < (plan.paired ? 2 : 1); ++s) wait(&sh.q_full[s], parts & 1);
             fence_after();
             ++parts;
             auto begin = [&](int i) {                            // logits of tile i
@@ -294,8 +332,6 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) kv_prefix_kernel(const KvAt
                     const bool more = i + 1 < w.count;
 #pragma unroll
                     for (int s = 0; s < 2; ++s) {
-                        wait(&sh.p_ready[s], p_count[s]++ & 1);
-                        fence_after();
                         sums(s, v_slot, i == 0);
                         if (s == 1) release(v_slot);
                         if (more) {
@@ -306,8 +342,6 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) kv_prefix_kernel(const KvAt
                     }
                 } else {
                     const int s = i & 1;
-                    wait(&sh.p_ready[s], p_count[s]++ & 1);
-                    fence_after();
                     sums(s, v_slot, i < 2);
                     release(v_slot);
                     if (i + 2 < w.count) begin(i + 2);
@@ -321,29 +355,12 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) kv_prefix_kernel(const KvAt
         const int s = warp >> 2, r = (warp & 3) * 32 + lane;
         const uint32_t quarter = uint32_t((warp & 3) * 32) << 16, s_addr = tmem + 128 * s + quarter, o_addr = tmem + 256 + G::kOColumns * s + quarter;
         uint32_t s_count = 0, o_count = 0;
-        const KvSpan all = kv_span(p.batch.offsets[0], p.batch.offsets[p.batch.sequences], p.tokens);
-        const int64_t live = int64_t(all.count) * p.group;
-        const int64_t row_base = int64_t(unit) * (plan.paired ? 2 * kKvPrefixRows : kKvPrefixRows) + (plan.paired ? s * kKvPrefixRows : 0);
+        const int64_t live = int64_t(q_count) * p.group;
+        const int64_t row_base = int64_t(plan.paired ? 2 * unit + s : unit) * plan.rows;
         auto wait = [&](uint64_t *bar, uint32_t parity) {
             if (ok) ok = mbar_wait(bar, parity, p.timeouts);
         };
         while (next_part(plan, at, end, w)) {
-            if (plan.paired || s == 0) {                         // this stream's rows of Q, swizzled as a copy would
-                uint8_t *dst = q_smem + s * G::kTileBytes;
-                for (int i = tid & 127; i < kKvPrefixRows * (D / 8); i += 128) {
-                    const int row = i / (D / 8), c = i % (D / 8);
-                    const int64_t at_row = row_base + row;
-                    uint4 x = make_uint4(0, 0, 0, 0);
-                    if (at_row < live)
-                        x = *reinterpret_cast<const uint4 *>(static_cast<const T *>(p.q.data) + (all.first + at_row / p.group) * p.q.token_stride +
-                                                             (int64_t(w.h) * p.group + at_row % p.group) * p.q.head_stride + 8 * c);
-                    *reinterpret_cast<uint4 *>(dst + (c >> 3) * G::kHalfBytes + row * 128 + (((c & 7) ^ (row & 7)) << 4)) = x;
-                }
-                fence_shared_async();
-            }
-            fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&sh.q_ready);
             float m = -INFINITY, l = 0.0f;
             int done = 0;                                        // tiles of this stream so far
             // pages outside the pool hold no keys: lane l < 8 looks after keys 16 l .. 16 l + 15 of a tile, if the part has any such page
@@ -374,8 +391,24 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) kv_prefix_kernel(const KvAt
                     for (int c = 0; c < 128; ++c)
                         if (c >= left || !((good >> (c >> 4)) & 1u)) x[c] = 0xff800000u;
                 }
-                float top = -INFINITY;
-                {
+                // the weights of columns c0 .. c0 + 31, under the maximum m, and their sum
+                const uint64_t scale2 = pair(p.scale_log2, p.scale_log2);
+                auto weights = [&](int c0, uint32_t (&pk)[16], uint64_t (&part)[2]) {
+                    const float base = m == -INFINITY ? 0.0f : -m;
+                    const uint64_t base2 = pair(base, base);
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) {
+                        const float2 z = unpair(fma2(pair(__uint_as_float(x[c0 + 2 * j]), __uint_as_float(x[c0 + 2 * j + 1])), scale2, base2));
+                        // some of the weights by the multiply-add pipe: the exponential unit gives 4 a cycle to each scheduler and
+                        // would take 2,048 cycles a step
+                        float2 e;
+                        if ((j & 7) < kByPolynomial) e = exp2_pair(z);
+                        else e = make_float2(kv_exp2(z.x), kv_exp2(z.y));
+                        part[j & 1] = add2(part[j & 1], pair(e.x, e.y));
+                        pk[j] = KvType<T>::pack(e.x, e.y);
+                    }
+                };
+                auto largest = [&] {
                     float t8[8];
 #pragma unroll
                     for (int j = 0; j < 8; ++j) t8[j] = __uint_as_float(x[j]);
@@ -385,59 +418,56 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) kv_prefix_kernel(const KvAt
                         for (int j = 0; j < 8; ++j) t8[j] = max3_nan(t8[j], __uint_as_float(x[c + j]), __uint_as_float(x[c + 8 + j]));
 #pragma unroll
                     for (int j = 0; j < 8; j += 2) t8[j] = max3_nan(max3_nan(t8[j], t8[j + 1], __uint_as_float(x[120 + j])), __uint_as_float(x[121 + j]), t8[j]);
-                    top = max3_nan(max3_nan(t8[0], t8[2], t8[4]), t8[6], t8[6]) * p.scale_log2;
-                }
-                top = top < INFINITY ? top : NAN;                // an infinite logit makes the row NaN, as inf - inf does
-                if (done == 0) {
-                    m = top;
-                } else if (__any_sync(kFullMask, !(top <= m + kRescaleAt))) {
-                    // (a NaN becomes the maximum: the polynomial below would lose it)
-                    const float next = max3_nan(m, top, top), f = next == -INFINITY ? 1.0f : kv_exp2(m - next);
-                    m = next;
-                    l *= f;
-                    wait(&sh.o_done[s], (o_count + done - 1) & 1);
-                    fence_after();
-#pragma unroll 1
-                    for (int c = 0; c < D; c += 32) {
-                        uint32_t y[32];
-                        tmem_ld32(o_addr + c, y);
-                        tmem_wait_ld();
-#pragma unroll
-                        for (int j = 0; j < 32; ++j) y[j] = __float_as_uint(__uint_as_float(y[j]) * f);
-                        tmem_st32(o_addr + c, y);
-                    }
-                    tmem_wait_st();
-                }
-                const float base = m == -INFINITY ? 0.0f : -m;
-                const uint64_t scale2 = pair(p.scale_log2, p.scale_log2), base2 = pair(base, base);
+                    const float top = max3_nan(max3_nan(t8[0], t8[2], t8[4]), t8[6], t8[6]) * p.scale_log2;
+                    return top < INFINITY ? top : NAN;           // an infinite logit makes the row NaN, as inf - inf does
+                };
+                // The first half is computed under the maximum so far, before it is known whether that still holds: it mostly does, and then
+                // looking for it costs no time of its own.
+                if (done == 0) m = largest();
+                uint32_t pk[2][16];
                 uint64_t part[2] = {0, 0};
+                weights(0, pk[0], part);
+                weights(32, pk[1], part);
+                if (done > 0) {
+                    const float top = largest();
+                    if (__any_sync(kFullMask, !(top <= m + kRescaleAt))) {
+                        // (a NaN becomes the maximum: the polynomial would lose it)
+                        const float next = max3_nan(m, top, top), f = next == -INFINITY ? 1.0f : kv_exp2(m - next);
+                        m = next;
+                        l *= f;
+                        wait(&sh.o_done[s], (o_count + done - 1) & 1);
+                        fence_after();
+#pragma unroll 1
+                        for (int c = 0; c < D; c += 32) {
+                            uint32_t y[32];
+                            tmem_ld32(o_addr + c, y);
+                            tmem_wait_ld();
 #pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    uint32_t pk[16];
-#pragma unroll
-                    for (int j = 0; j < 16; ++j) {
-                        const int at = 32 * c + 2 * j;
-                        const float2 z = unpair(fma2(pair(__uint_as_float(x[at]), __uint_as_float(x[at + 1])), scale2, base2));
-                        // some of the weights by the multiply-add pipe: the exponential unit gives 4 a cycle to each scheduler and
-                        // would take 2,048 cycles a step
-                        float2 e;
-                        if ((j & 7) < kByPolynomial) e = exp2_pair(z);
-                        else e = make_float2(kv_exp2(z.x), kv_exp2(z.y));
-                        part[j & 1] = add2(part[j & 1], pair(e.x, e.y));
-                        pk[j] = KvType<T>::pack(e.x, e.y);
+                            for (int j = 0; j < 32; ++j) y[j] = __float_as_uint(__uint_as_float(y[j]) * f);
+                            tmem_st32(o_addr + c, y);
+                        }
+                        tmem_wait_st();
+                        part[0] = part[1] = 0;
+                        weights(0, pk[0], part);
+                        weights(32, pk[1], part);
                     }
-                    tmem_st16(s_addr + 16 * c, pk);
+                }
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                    if (half == 1) { weights(64, pk[0], part); weights(96, pk[1], part); }
+                    tmem_st16(s_addr + 32 * half, pk[0]);
+                    tmem_st16(s_addr + 32 * half + 16, pk[1]);
+                    tmem_wait_st();
+                    fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&sh.p_ready[s][half]);
                 }
                 const float2 sums = unpair(add2(part[0], part[1]));
                 l += sums.x + sums.y;
-                tmem_wait_st();
-                fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&sh.p_ready[s]);
             }
             // ---- the part's result
             const int64_t block = ((int64_t(w.h) + group) * plan.units + unit) * 2 + s;
-            const bool have = row_base + r < live;
+            const bool have = r < plan.rows && row_base + r < live;
             if (done > 0) {
                 wait(&sh.o_done[s], (o_count + done - 1) & 1);
                 fence_after();
@@ -455,6 +485,10 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) kv_prefix_kernel(const KvAt
             }
             o_count += done;
             if (have) p.pre_ml[block * kKvPrefixRows + r] = make_float2(m, l);
+            // Q, S and O may be written anew
+            fence_before();
+            __syncwarp();
+            if (lane == 0) { mbar_arrive(&sh.q_free[0]); mbar_arrive(&sh.q_free[1]); }
         }
     }
 
