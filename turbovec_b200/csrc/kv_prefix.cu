@@ -1,28 +1,35 @@
 // Attention of many query rows over a shared prefix, on the tensor cores (tcgen05, accumulators in tensor memory).
 //
 // All rows of a batch (tokens x heads of a key head) see all keys of the prefix, so the prefix is read once for 256 rows instead of
-// once for every sequence.  S = Q K^T and O += P V are MMAs of 128 rows by 128 keys; four warps turn a tile of S into P, a row
-// to a thread: running maximum, weights in powers of two, their sum.  O is rescaled only when a row's maximum grows by more than
-// 2^8 (weights then stay below 2^8, which neither type nor the sums mind).  P replaces S in tensor memory and is the A operand
-// of the second MMA.
+// once for every sequence.  S = Q K^T and O += P V are MMAs of 128 rows; four warps turn S into P, a row to a thread: running
+// maximum, weights in powers of two, their sum.  O is rescaled only when a row's maximum grows by more than 2^8 (weights then
+// stay below 2^8, which neither type nor the sums mind).  P replaces S in tensor memory and is the A operand of the second MMA.
 //
-// Two streams of such tiles keep the tensor cores busy while the other's weights are computed.  With more than 128 rows the streams
-// are two row tiles that share each tile of keys and values; with fewer they are one row tile over every other tile of keys.
+// Two streams keep the tensor cores and the other units busy at once.  With more than one tile of rows the streams are two such tiles
+// that share each tile of keys and values; else they are one tile of rows over every other tile of keys.  A stream's S has two
+// halves of 64 keys: while the weights of one are computed, P of the other goes through its MMAs and becomes the next logits.
 // 128 channels: 256 columns of S and 256 of O fill tensor memory.
 //
 // Blocks of one unit of rows share the list of (key head, tile) steps evenly; the units of one group of blocks go over the same keys at
-// the same time, so that the second and later ones find them in L2.  A step is 2 * 128 * 128 * 128 * 2 multiply-adds = 2,048 cycles
-// of the tensor cores and as many of the exponential unit: that is what bounds it.
+// the same time, so that the second and later ones find them in L2.
+//
+// What bounds it is the weights.  A step (256 rows x 128 keys x 128 channels) is 2,048 cycles of MMAs (2,480 measured: halves of S
+// are MMAs of N = 64, which shared memory feeds in 48 cycles and not in 32), and it takes 3,800; with the MMAs left out 3,630, with
+// the weights left out 2,500.  1,536 cycles of it are the exponential unit (8 cycles an instruction; a quarter of the weights go by the
+// multiply-add pipe, 0, 1/8 and 3/8 are 5, 1 and 1 % slower), 960 multiply-adds, 770 maxima and conversions, per scheduler, and two
+// warps do not overlap them well.  Tried and slower: tiles of 128 keys without halves (3,650 a step, but 8,000 cycles
+// more around the loop), two threads to a row on 16 warps (4,600), one warp for all MMAs with halves (4,300).
+// attend_128_prefix_32768 (1,024 rows of 8 key heads, 32,768 keys): 129 us of 202.
 #include "kv_cache.cuh"
 #include "scan_tc_common.cuh"
 
 namespace tv {
 namespace {
 
-constexpr int kPrefixThreads = 12 * 32;          // 2 x 4 warps of weights, one of MMAs, one of copies, two that complete the group
-constexpr int kWeightRegs = 208, kOtherRegs = 88;   // registers a thread: 256 * 208 + 128 * 88 = 384 * 168, what the block starts with
+constexpr int kPrefixThreads = 12 * 32;          // 2 x 4 warps of weights, two of MMAs, one of copies, one that completes the group
+constexpr int kWeightRegs = 184, kOtherRegs = 136;   // registers a thread: 256 * 184 + 128 * 136 = 384 * 168, what the block starts with
 static_assert(256 * kWeightRegs + 128 * kOtherRegs <= kPrefixThreads * 168, "more registers than the block has");
-constexpr int kMmaWarp = 8, kCopyWarp = 9;
+constexpr int kMmaWarp = 8, kCopyWarp = 10;      // MMAs of stream s: warp kMmaWarp + s
 constexpr int kHalfKeys = kKvPrefixTile / 2;
 constexpr float kRescaleAt = 8.0f;
 constexpr int kByPolynomial = 2;                 // pairs of weights of every eight
@@ -38,7 +45,7 @@ struct PrefixGeometry {
 template <int D>
 struct PrefixShared {
     uint64_t full[PrefixGeometry<D>::kSlots], empty[PrefixGeometry<D>::kSlots];
-    uint64_t s_full[2], p_ready[2][2], o_done[2], q_full[2], q_free[2];       // [stream], [stream][half of P]
+    uint64_t s_full[2][2], p_ready[2][2], o_done[2], q_full[2], q_free[2];    // [stream][half of a tile], [stream]
     uint32_t tmem_base;
 };
 
@@ -177,11 +184,11 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) kv_prefix_kernel(const KvAt
     const KvPrefixPlan plan = p.plan;
     const int unit = blockIdx.x % plan.units, group = blockIdx.x / plan.units;
     if (tid == 0) {
-        for (int s = 0; s < G::kSlots; ++s) { mbar_init(&sh.full[s], 1); mbar_init(&sh.empty[s], 1); }
+        for (int s = 0; s < G::kSlots; ++s) { mbar_init(&sh.full[s], 1); mbar_init(&sh.empty[s], plan.paired ? 2 : 1); }
         for (int s = 0; s < 2; ++s) {
-            mbar_init(&sh.s_full[s], 1); mbar_init(&sh.o_done[s], 1);
+            mbar_init(&sh.o_done[s], 1);
             mbar_init(&sh.q_full[s], 1); mbar_init(&sh.q_free[s], 8);
-            for (int b = 0; b < 2; ++b) mbar_init(&sh.p_ready[s][b], 4);
+            for (int b = 0; b < 2; ++b) { mbar_init(&sh.s_full[s][b], 1); mbar_init(&sh.p_ready[s][b], 4); }
         }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -264,89 +271,79 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) kv_prefix_kernel(const KvAt
             for (uint32_t i = n > G::kSlots ? n - G::kSlots : 0; i < n; ++i) mbar_wait(&sh.full[i % G::kSlots], (i / G::kSlots) & 1, p.timeouts);
             for (int s = 0; s < (plan.paired ? 2 : 1) && parts > 0; ++s) mbar_wait(&sh.q_full[s], (parts - 1) & 1, p.timeouts);
         }
-    } else if (warp == kMmaWarp) {
-        uint32_t parts = 0, p_count[2] = {0, 0};
-        constexpr uint32_t kIdS = idesc<T>(128, false), kIdO = idesc<T>(D, true);
-        const uint32_t ring_addr = smem_u32(ring), q_addr = smem_u32(q_smem);
+    } else if (warp < kMmaWarp + 2) {
+        // ---- MMAs of stream s.  One warp for both would be what bounds the kernel: waiting for a barrier that has completed takes it some 200
+        // cycles, six times a tile, and an MMA 30 to issue (3,000 cycles a step with weights that cost nothing; 2,048 are the MMAs').
+        const int s = warp - kMmaWarp, first = plan.paired ? 0 : s, stride = plan.paired ? 1 : 2, qs = plan.paired ? s : 0;
+        uint32_t parts = 0, p_count = 0, base = 0;               // tiles of the ring before this part
+        constexpr uint32_t kIdS = idesc<T>(kHalfKeys, false), kIdO = idesc<T>(D, true);
         auto wait = [&](uint64_t *bar, uint32_t parity) {
             if (ok) ok = mbar_wait(bar, parity, p.timeouts);
+            fence_after();
         };
         const uint32_t leader = elected();
-        const uint64_t q_desc = umma_desc(q_addr), ring_k = umma_desc(ring_addr), ring_v = desc_mn(ring_addr, G::kHalfBytes);
-        // descriptors of other addresses: 16-byte units added to the address field, which has room for all of shared memory
-        auto logits = [&](int s, uint32_t slot) {                // S_s = Q_s K^T
-            const uint64_t a = q_desc + (plan.paired ? uint32_t(s * (G::kTileBytes >> 4)) : 0u), b = ring_k + slot * uint32_t(G::kTileBytes >> 4);
-            mma_ss<false>(leader, tmem + 128 * s, a, b, kIdS);
-#pragma unroll
-            for (int i = 1; i < D / 16; ++i) {
-                const uint32_t off = ((i >> 2) * G::kHalfBytes + (i & 3) * 32) >> 4;
-                mma_ss<true>(leader, tmem + 128 * s, a + off, b + off, kIdS);
-            }
-            commit(leader, &sh.s_full[s]);
-        };
-        // O_s += P_s V, in two halves of the keys: the first begins while the weights of the second are being computed
-        auto sums = [&](int s, uint32_t slot, bool first) {
-            const uint64_t b = ring_v + slot * uint32_t(G::kTileBytes >> 4);
-            for (int half = 0; half < 2; ++half) {
-                wait(&sh.p_ready[s][half], p_count[s] & 1);
-                fence_after();
-#pragma unroll
-                for (int i = 0; i < kHalfKeys / 16; ++i)
-                    mma_ts(leader, tmem + 256 + G::kOColumns * s, tmem + 128 * s + 8 * (4 * half + i), b + (4 * half + i) * (2048 >> 4), kIdO, !first || half + i > 0);
-            }
-            ++p_count[s];
-            commit(leader, &sh.o_done[s]);
-        };
-        auto release = [&](uint32_t slot) { commit(leader, &sh.empty[slot]); };
-        uint32_t ring_slot = 0, ring_round = 0;
-        auto next_tile = [&] {                                   // waits for the next tile of the ring
-            const uint32_t slot = ring_slot;
-            wait(&sh.full[slot], ring_round & 1);
-            fence_after();
-            if (++ring_slot == G::kSlots) { ring_slot = 0; ++ring_round; }
-            return slot;
-        };
+        const uint64_t q_desc = umma_desc(smem_u32(q_smem) + qs * G::kTileBytes), ring_k = umma_desc(smem_u32(ring)), ring_v = desc_mn(smem_u32(ring), G::kHalfBytes);
+        const uint32_t s_tmem = tmem + 128 * s, o_tmem = tmem + 256 + G::kOColumns * s;
         while (next_part(plan, at, end, w)) {
-            for (int s = 0; s < (plan.paired ? 2 : 1); ++s) wait(&sh.q_full[s], parts & 1);
-            fence_after();
-            ++parts;
-            auto begin = [&](int i) {                            // logits of tile i
-                const uint32_t slot = next_tile();
-                if (plan.paired) { logits(0, slot); logits(1, slot); }
-                else logits(i & 1, slot);
-                release(slot);
+            const int ahead = min(lookahead, w.count);
+            // places in the ring: `ahead` tiles of keys, then values and keys in turn
+            auto place_v = [&](int i) { return base + uint32_t(ahead + i + min(i, w.count - ahead)); };
+            auto place_k = [&](int i) { return i < lookahead ? base + uint32_t(i) : place_v(i - lookahead) + 1; };
+            // descriptors of other addresses: 16-byte units added to the address field, which has room for all of shared memory
+            auto logits = [&](int b, uint32_t slot) {            // S of half b = Q K^T
+                const uint64_t k = ring_k + slot * uint32_t(G::kTileBytes >> 4) + uint32_t(b * (kHalfKeys * 128 >> 4));
+                const uint32_t d = s_tmem + kHalfKeys * b;
+                mma_ss<false>(leader, d, q_desc, k, kIdS);
+#pragma unroll
+                for (int c = 1; c < D / 16; ++c) {
+                    const uint32_t off = ((c >> 2) * G::kHalfBytes + (c & 3) * 32) >> 4;
+                    mma_ss<true>(leader, d, q_desc + off, k + off, kIdS);
+                }
+                commit(leader, &sh.s_full[s][b]);
             };
-            for (int i = 0; i < min(lookahead, w.count); ++i) begin(i);
-            for (int i = 0; i < w.count; ++i) {
-                const uint32_t v_slot = next_tile();
+            auto tile_of = [&](uint32_t n) {                     // waits for place n of the ring
+                const uint32_t slot = n % G::kSlots;
+                wait(&sh.full[slot], (n / G::kSlots) & 1);
+                return slot;
+            };
+            if (first < w.count) {
+                wait(&sh.q_full[qs], parts & 1);
+                const uint32_t slot = tile_of(place_k(first));
+                logits(0, slot);
+                logits(1, slot);
+                commit(leader, &sh.empty[slot]);
+            }
+            for (int i = first; i < w.count; i += stride) {
+                const uint32_t slot = tile_of(place_v(i));
                 const int64_t left = int64_t(p.prefix_len) - int64_t(w.tile0 + i) * kKvPrefixTile;
-                if (left < kKvPrefixTile) {                      // places behind the prefix may hold anything, and 0 * NaN is not 0
-                    uint8_t *v = ring + v_slot * G::kTileBytes;
+                if (left < kKvPrefixTile) {                      // places behind the prefix may hold anything, and 0 * NaN is not 0 (the other
+                    uint8_t *v = ring + slot * G::kTileBytes;    // stream's warp writes the same zeros)
                     for (int row = int(left); row < kKvPrefixTile; ++row)
                         if (lane < D / 8) *reinterpret_cast<uint4 *>(v + (lane >> 3) * G::kHalfBytes + row * 128 + (lane & 7) * 16) = make_uint4(0, 0, 0, 0);
                     fence_shared_async();
                     __syncwarp();
                 }
-                if (plan.paired) {
-                    uint32_t k_slot = 0;
-                    const bool more = i + 1 < w.count;
+                const uint64_t v = ring_v + slot * uint32_t(G::kTileBytes >> 4);
+                const bool more = i + stride < w.count;
+                uint32_t k_slot = 0;
 #pragma unroll
-                    for (int s = 0; s < 2; ++s) {
-                        sums(s, v_slot, i == 0);
-                        if (s == 1) release(v_slot);
-                        if (more) {
-                            if (s == 0) k_slot = next_tile();
-                            logits(s, k_slot);
-                            if (s == 1) release(k_slot);
-                        }
+                for (int b = 0; b < 2; ++b) {                    // O += P V, and the next logits where this P was
+                    wait(&sh.p_ready[s][b], p_count & 1);
+#pragma unroll
+                    for (int c = 0; c < kHalfKeys / 16; ++c)
+                        mma_ts(leader, o_tmem, s_tmem + kHalfKeys * b + 8 * c, v + (4 * b + c) * (2048 >> 4), kIdO, i != first || b + c > 0);
+                    commit(leader, &sh.o_done[s]);
+                    if (more) {
+                        if (b == 0) k_slot = tile_of(place_k(i + stride));
+                        logits(b, k_slot);
                     }
-                } else {
-                    const int s = i & 1;
-                    sums(s, v_slot, i < 2);
-                    release(v_slot);
-                    if (i + 2 < w.count) begin(i + 2);
                 }
+                ++p_count;
+                commit(leader, &sh.empty[slot]);
+                if (more) commit(leader, &sh.empty[k_slot]);
             }
+            base += 2 * uint32_t(w.count);
+            ++parts;
         }
     }
     } else {
@@ -362,8 +359,8 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) kv_prefix_kernel(const KvAt
         };
         while (next_part(plan, at, end, w)) {
             float m = -INFINITY, l = 0.0f;
-            int done = 0;                                        // tiles of this stream so far
-            // pages outside the pool hold no keys: lane l < 8 looks after keys 16 l .. 16 l + 15 of a tile, if the part has any such page
+            int done = 0;                                        // halves of tiles of this stream so far
+            // pages outside the pool hold no keys: lane l < 4 looks after keys 16 l .. 16 l + 15 of a half, if the part has any such page
             auto page_is_good = [&](int64_t key) {
                 const int64_t entry = key >> p.page_shift;
                 const int page = key < p.prefix_len && entry < p.prefix_width ? __ldg(p.prefix_pages + entry) : -1;
@@ -376,19 +373,21 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) kv_prefix_kernel(const KvAt
                 all_good = __all_sync(kFullMask, all_good);
             }
             const int stride = plan.paired ? 1 : 2;
-            for (int i = plan.paired ? 0 : s; i < w.count; i += stride, ++done) {
-                wait(&sh.s_full[s], s_count++ & 1);
+            for (int i = plan.paired ? 0 : s; i < w.count; i += stride, ++s_count)
+#pragma unroll 1
+            for (int b = 0; b < 2; ++b, ++done) {
+                wait(&sh.s_full[s][b], s_count & 1);
                 fence_after();
-                uint32_t x[128];
-#pragma unroll
-                for (int c = 0; c < 4; ++c) tmem_ld32(s_addr + 32 * c, reinterpret_cast<uint32_t (&)[32]>(x[32 * c]));
+                const uint32_t half_addr = s_addr + kHalfKeys * b;
+                uint32_t x[kHalfKeys];
+                tmem_ld32(half_addr, reinterpret_cast<uint32_t (&)[32]>(x[0]));
+                tmem_ld32(half_addr + 32, reinterpret_cast<uint32_t (&)[32]>(x[32]));
                 tmem_wait_ld();
-                const int64_t left = int64_t(p.prefix_len) - int64_t(w.tile0 + i) * kKvPrefixTile;
-                const bool border = !all_good || left < kKvPrefixTile;
-                if (border) {
-                    const uint32_t good = __ballot_sync(kFullMask, page_is_good(int64_t(w.tile0 + i) * kKvPrefixTile + 16 * (lane & 7)));
+                const int first_key = (w.tile0 + i) * kKvPrefixTile + kHalfKeys * b, left = p.prefix_len - first_key;     // below 2^30 + 128
+                if (!all_good || left < kHalfKeys) {
+                    const uint32_t good = __ballot_sync(kFullMask, page_is_good(first_key + 16 * (lane & 3)));
 #pragma unroll
-                    for (int c = 0; c < 128; ++c)
+                    for (int c = 0; c < kHalfKeys; ++c)
                         if (c >= left || !((good >> (c >> 4)) & 1u)) x[c] = 0xff800000u;
                 }
                 // the weights of columns c0 .. c0 + 31, under the maximum m, and their sum
@@ -413,15 +412,15 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) kv_prefix_kernel(const KvAt
 #pragma unroll
                     for (int j = 0; j < 8; ++j) t8[j] = __uint_as_float(x[j]);
 #pragma unroll
-                    for (int c = 8; c < 120; c += 16)
+                    for (int c = 8; c < 56; c += 16)
 #pragma unroll
                         for (int j = 0; j < 8; ++j) t8[j] = max3_nan(t8[j], __uint_as_float(x[c + j]), __uint_as_float(x[c + 8 + j]));
 #pragma unroll
-                    for (int j = 0; j < 8; j += 2) t8[j] = max3_nan(max3_nan(t8[j], t8[j + 1], __uint_as_float(x[120 + j])), __uint_as_float(x[121 + j]), t8[j]);
+                    for (int j = 0; j < 8; j += 2) t8[j] = max3_nan(max3_nan(t8[j], t8[j + 1], __uint_as_float(x[56 + j])), __uint_as_float(x[57 + j]), t8[j]);
                     const float top = max3_nan(max3_nan(t8[0], t8[2], t8[4]), t8[6], t8[6]) * p.scale_log2;
                     return top < INFINITY ? top : NAN;           // an infinite logit makes the row NaN, as inf - inf does
                 };
-                // The first half is computed under the maximum so far, before it is known whether that still holds: it mostly does, and then
+                // The weights are computed under the maximum so far, before it is known whether that still holds: it mostly does, and then
                 // looking for it costs no time of its own.
                 if (done == 0) m = largest();
                 uint32_t pk[2][16];
@@ -435,7 +434,7 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) kv_prefix_kernel(const KvAt
                         const float next = max3_nan(m, top, top), f = next == -INFINITY ? 1.0f : kv_exp2(m - next);
                         m = next;
                         l *= f;
-                        wait(&sh.o_done[s], (o_count + done - 1) & 1);
+                        wait(&sh.o_done[s], (o_count + done - 1) & 1);      // (the half before that had ended when these logits were there)
                         fence_after();
 #pragma unroll 1
                         for (int c = 0; c < D; c += 32) {
@@ -446,24 +445,22 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) kv_prefix_kernel(const KvAt
                             for (int j = 0; j < 32; ++j) y[j] = __float_as_uint(__uint_as_float(y[j]) * f);
                             tmem_st32(o_addr + c, y);
                         }
-                        tmem_wait_st();
                         part[0] = part[1] = 0;
                         weights(0, pk[0], part);
                         weights(32, pk[1], part);
                     }
                 }
-#pragma unroll
-                for (int half = 0; half < 2; ++half) {
-                    if (half == 1) { weights(64, pk[0], part); weights(96, pk[1], part); }
-                    tmem_st16(s_addr + 32 * half, pk[0]);
-                    tmem_st16(s_addr + 32 * half + 16, pk[1]);
-                    tmem_wait_st();
-                    fence_before();
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(&sh.p_ready[s][half]);
-                }
+                tmem_st16(half_addr, pk[0]);
+                tmem_st16(half_addr + 16, pk[1]);
                 const float2 sums = unpair(add2(part[0], part[1]));
                 l += sums.x + sums.y;
+                tmem_wait_st();
+                // A wait tells a phase from the one before it only.  At the end of the part the last half's product is waited for, so the one
+                // before must be known to have ended; it has, or is under way, while the last one cannot have begun.
+                if (b == 1 && i + stride >= w.count) wait(&sh.o_done[s], (o_count + done - 1) & 1);
+                fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&sh.p_ready[s][b]);
             }
             // ---- the part's result
             const int64_t block = ((int64_t(w.h) + group) * plan.units + unit) * 2 + s;
