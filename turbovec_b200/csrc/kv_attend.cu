@@ -33,6 +33,7 @@ struct Geometry {
 template <int D>
 struct AttendShared {
     float o[kConsumers][kKvRows][D + 4];
+    uint16_t q[kKvRows][D + 8];                          // rows of Q, a row's banks four words from the one before it
     float2 ml[kConsumers][kKvRows], total[kKvRows];
     int first_key[Geometry<D>::kStages][kConsumers];
     int64_t scratch[2 * (kAttendThreads / 32) + 3];
@@ -223,10 +224,10 @@ __device__ __forceinline__ void ldmatrix4_trans(uint32_t addr, uint32_t (&r)[4])
 template <typename T>
 __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     if constexpr (std::is_same<T, __nv_bfloat16>::value)
-        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
     else
-        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 __device__ __forceinline__ void consumers_sync() { asm volatile("bar.sync 1, %0;" ::"n"(kConsumers * 32) : "memory"); }
@@ -335,19 +336,20 @@ __global__ void __launch_bounds__(kAttendThreads, 2) kv_attend_kernel(const KvAt
     while (walk.next(w)) {
         const int last = walk.last_tile(w);
         uint32_t qf[D / 16][4];
-        const bool have0 = r0 < w.rows, have1 = r1 < w.rows;
-        const int row0 = w.row0 + (have0 ? r0 : 0), row1 = w.row0 + (have1 ? r1 : 0);
-        const int j0 = row0 / p.group, j1 = row1 / p.group;              // tokens of the two rows, and their heads
-        const int head0 = w.h * p.group + row0 - j0 * p.group, head1 = w.h * p.group + row1 - j1 * p.group;
-        const T *q0 = static_cast<const T *>(p.q.data) + int64_t(w.first_token + j0) * p.q.token_stride + int64_t(head0) * p.q.head_stride;
-        const T *q1 = static_cast<const T *>(p.q.data) + int64_t(w.first_token + j1) * p.q.token_stride + int64_t(head1) * p.q.head_stride;
-#pragma unroll
-        for (int i = 0; i < D / 16; ++i) {
-            qf[i][0] = have0 ? *reinterpret_cast<const uint32_t *>(q0 + 16 * i + c2) : 0u;
-            qf[i][1] = have1 ? *reinterpret_cast<const uint32_t *>(q1 + 16 * i + c2) : 0u;
-            qf[i][2] = have0 ? *reinterpret_cast<const uint32_t *>(q0 + 16 * i + 8 + c2) : 0u;
-            qf[i][3] = have1 ? *reinterpret_cast<const uint32_t *>(q1 + 16 * i + 8 + c2) : 0u;
+        // Q through shared memory: every warp needs all of it, and eight 16-byte loads are under way where 32 of 4 bytes were
+        for (int i = tid; i < kKvRows * (D / 8); i += kConsumers * 32) {
+            const int r = i / (D / 8), c = i % (D / 8), row = w.row0 + r, j = row / p.group;
+            uint4 x = make_uint4(0, 0, 0, 0);
+            if (r < w.rows)
+                x = *reinterpret_cast<const uint4 *>(static_cast<const T *>(p.q.data) + int64_t(w.first_token + j) * p.q.token_stride +
+                                                     int64_t(w.h * p.group + row - j * p.group) * p.q.head_stride + 8 * c);
+            *reinterpret_cast<uint4 *>(&sh.q[r][8 * c]) = x;
         }
+        const bool have0 = r0 < w.rows, have1 = r1 < w.rows;
+        const int j0 = have0 ? (w.row0 + r0) / p.group : 0, j1 = have1 ? (w.row0 + r1) / p.group : 0;       // tokens of the two rows
+        consumers_sync();
+#pragma unroll
+        for (int i = 0; i < D / 16; ++i) ldmatrix4(smem_u32(&sh.q[((lane >> 3) & 1) * 8 + (lane & 7)][16 * i + ((lane >> 4) & 1) * 8]), qf[i]);
         const int lim0 = have0 ? walk.limit(w, j0) : 0, lim1 = have1 ? walk.limit(w, j1) : 0;
         const int lim_first = walk.limit(w, w.row0 / p.group), lim_last = walk.limit(w, (w.row0 + w.rows - 1) / p.group);
         float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.0f, l1 = 0.0f;
@@ -360,15 +362,23 @@ __global__ void __launch_bounds__(kAttendThreads, 2) kv_attend_kernel(const KvAt
             if (ok) ok = mbar_wait(&sh.full[s], (n / G::kStages) & 1, p.timeouts);
             const uint32_t k_addr = ring_addr + s * G::kStageBytes, v_addr = k_addr + G::kOperandBytes;
             const int first = sh.first_key[s][warp];
-            float sc[2][4] = {};
+            // all of K's fragments first, so that their loads overlap; two accumulators to a product halve the chain of MMAs
+            uint32_t kf[D / 16][4];
 #pragma unroll
             for (int i = 0; i < D / 16; ++i) {
-                uint32_t kf[4];
                 const int chunk = 2 * i + k_chunk;
-                ldmatrix4(k_addr + (chunk >> 3) * G::kHalfBytes + k_row * 128 + (((chunk & 7) ^ (k_row & 7)) << 4), kf);
-                mma16816<T>(sc[0], qf[i], kf[0], kf[1]);
-                mma16816<T>(sc[1], qf[i], kf[2], kf[3]);
+                ldmatrix4(k_addr + (chunk >> 3) * G::kHalfBytes + k_row * 128 + (((chunk & 7) ^ (k_row & 7)) << 4), kf[i]);
             }
+            float sc[2][4] = {}, sd[2][4] = {};
+#pragma unroll
+            for (int i = 0; i < D / 16; i += 2) {
+                mma16816<T>(sc[0], qf[i], kf[i][0], kf[i][1]);
+                mma16816<T>(sc[1], qf[i], kf[i][2], kf[i][3]);
+                mma16816<T>(sd[0], qf[i + 1], kf[i + 1][0], kf[i + 1][1]);
+                mma16816<T>(sd[1], qf[i + 1], kf[i + 1][2], kf[i + 1][3]);
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) { sc[0][e] += sd[0][e]; sc[1][e] += sd[1][e]; }
             // logits in powers of two; keys that a row does not see count for nothing, whatever they hold
             const bool border = first + 16 > lim_first;
 #pragma unroll
@@ -417,11 +427,15 @@ __global__ void __launch_bounds__(kAttendThreads, 2) kv_attend_kernel(const KvAt
                 const bool all = first + 16 <= limit;
                 const uint32_t x0 = all ? ~0u : live_mask(first + c2, limit), x1 = all ? ~0u : live_mask(first + 8 + c2, limit);
 #pragma unroll
-                for (int i = 0; i < D / 16; ++i) {
-                    uint32_t vf[4];
-                    values(i, vf);
-                    mma16816<T>(o[2 * i], a, vf[0] & x0, vf[1] & x1);
-                    mma16816<T>(o[2 * i + 1], a, vf[2] & x0, vf[3] & x1);
+                for (int i0 = 0; i0 < D / 16; i0 += 4) {
+                    uint32_t vf[4][4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) values(i0 + i, vf[i]);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        mma16816<T>(o[2 * (i0 + i)], a, vf[i][0] & x0, vf[i][1] & x1);
+                        mma16816<T>(o[2 * (i0 + i) + 1], a, vf[i][2] & x0, vf[i][3] & x1);
+                    }
                 }
             };
             bool apart = false;
