@@ -425,7 +425,7 @@ int tv_kv_attend(const tv_kv_cache *cache, const tv_kv_batch *batch, int64_t tok
  * the largest over its query heads of s * sum over channels of max(q8 lo, q8 hi), times the page's scale: lo and hi its bounds, q8 =
  * q / s to the nearest whole number (ties to even) and s the smallest of 2^-24 .. 2^40 with |q| <= 127 s.  A page outside the pool comes
  * last.  pages_out [token][key head][budget] receives the chosen page numbers of the sequence, ascending, then -1.  first + recent <=
- * budget; table_width <= 49,152. */
+ * budget; table_width <= 32,768. */
 size_t tv_kv_attend_selected_workspace(const tv_kv_cache *cache, const tv_kv_batch *batch, int64_t tokens, int heads, int64_t budget);
 int tv_kv_attend_selected(const tv_kv_cache *cache, const tv_kv_batch *batch, int64_t tokens, int heads, const tv_kv_rows *q,
                           int64_t budget, int64_t first, int64_t recent, float scale, const tv_kv_rows *out, float *lse,

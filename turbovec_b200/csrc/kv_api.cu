@@ -291,8 +291,8 @@ int tv_kv_attend_selected(const tv_kv_cache *c, const tv_kv_batch *b, int64_t to
     if (rc != TV_OK) return rc;
     if (!c->bounds) return refuse("the cache has no bounds to choose pages by");
     if (budget < 1 || budget > kKvMaxScored || first < 0 || recent < 0 || first > budget || recent > budget - first)
-        return refuse("budget must be between 1 and 49,152, and first + recent at most budget");
-    if (b->table_width > kKvMaxScored) return unsupported("table_width must be at most 49,152 pages");
+        return refuse("budget must be between 1 and 32,768, and first + recent at most budget");
+    if (b->table_width > kKvMaxScored) return unsupported("table_width must be at most 32,768 pages");
     if (tokens == 0 || b->sequences == 0) return TV_OK;
     if (!pages_out) return refuse("pages_out must be given");
     KvAttendParams p{};

@@ -246,7 +246,7 @@ cudaError_t launch_kv_attend(const KvAttendParams &p, const KvMaps &maps, int dt
 cudaError_t launch_kv_prefix(const KvAttendParams &p, const KvMaps &maps, int dtype, int head_dim, int device, cudaStream_t s);
 uint32_t *kv_timeouts_symbol(int device);    // address on `device`, which is the current one; null if it cannot be had
 
-constexpr int kKvMaxScored = 49152;          // pages of a sequence whose scores fit a block's shared memory
+constexpr int kKvMaxScored = 32768;          // pages of a sequence whose scores fit a block's shared memory
 struct KvSelectParams {
     KvBatch batch;
     KvRows q;
