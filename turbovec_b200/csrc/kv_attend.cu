@@ -18,6 +18,7 @@ namespace {
 
 constexpr int kConsumers = 4;
 constexpr int kAttendThreads = (kConsumers + 1) * 32;
+constexpr float kRescaleAt = 8.0f;
 constexpr int kLeastTiles = 3;                           // tiles of a run: joining more parts takes longer than these
 constexpr int kNothing = INT_MAX - kKvTile;              // first position of a group of keys that nobody sees
 
@@ -396,7 +397,8 @@ __global__ void __launch_bounds__(kAttendThreads, 2) kv_attend_kernel(const KvAt
             float t0 = fmaxf(fmaxf(sc[0][0], sc[0][1]), fmaxf(sc[1][0], sc[1][1])), t1 = fmaxf(fmaxf(sc[0][2], sc[0][3]), fmaxf(sc[1][2], sc[1][3]));
             t0 = fmaxf(t0, __shfl_xor_sync(kFullMask, t0, 1)); t1 = fmaxf(t1, __shfl_xor_sync(kFullMask, t1, 1));
             t0 = fmaxf(t0, __shfl_xor_sync(kFullMask, t0, 2)); t1 = fmaxf(t1, __shfl_xor_sync(kFullMask, t1, 2));
-            if (__any_sync(kFullMask, t0 > m0 || t1 > m1)) {
+            // a maximum that grows by less than 2^8 stays: weights are below 2^8 then, which neither type nor the sums mind
+            if (__any_sync(kFullMask, t0 > m0 + kRescaleAt || t1 > m1 + kRescaleAt)) {
                 const float n0 = fmaxf(m0, t0), n1 = fmaxf(m1, t1);
                 const float a0 = n0 == -INFINITY ? 1.0f : kv_exp2(m0 - n0), a1 = n1 == -INFINITY ? 1.0f : kv_exp2(m1 - n1);
                 m0 = n0; m1 = n1;

@@ -105,11 +105,12 @@ __global__ void __launch_bounds__(kSelectThreads, 2) kv_select_kernel(const KvSe
         return;
     }
     const int begin = p.first, end = n - p.recent, want = p.budget - p.first - p.recent;
-    if (rank == 0) {
+    auto put_taken = [&] {
         for (int i = tid; i < p.first; i += kSelectThreads) put(i, i);
         for (int i = tid; i < p.recent; i += kSelectThreads) put(p.budget - p.recent + i, end + i);
-    }
+    };
     if (want == 0) {
+        if (rank == 0) put_taken();
         others_begun();
         return;
     }
@@ -233,6 +234,7 @@ __global__ void __launch_bounds__(kSelectThreads, 2) kv_select_kernel(const KvSe
         __syncthreads();
     }
 
+    put_taken();
     // The want-th largest key.  Between the smallest and the largest key the leading digit of kBinBits bits mostly leaves a handful of candidates,
     // which are ranked by comparing them all; where it leaves more, the next digit of the bin that holds the key is looked at.
     const int m = end - begin;
