@@ -430,6 +430,12 @@ size_t tv_kv_attend_selected_workspace(const tv_kv_cache *cache, const tv_kv_bat
 int tv_kv_attend_selected(const tv_kv_cache *cache, const tv_kv_batch *batch, int64_t tokens, int heads, const tv_kv_rows *q,
                           int64_t budget, int64_t first, int64_t recent, float scale, const tv_kv_rows *out, float *lse,
                           int32_t *pages_out, void *workspace, size_t workspace_bytes, void *stream);
+/* Options of these calls, for the whole process; results stay within the same rounding.  Workspace sizes follow them: ask anew. */
+enum {
+    TV_KV_OPT_TENSOR_PREFIX = 1     /* -1 (default): a prefix is read by the tensor-memory kernel where that was measured to be faster
+                                     * (keys * key heads * (rows - 29) > 2.6 million); 0: never; 1: always (testing) */
+};
+int tv_kv_set_option(int option, int64_t value);
 /* Waits for the device and tells whether a kernel of these calls gave up a wait since the last time it was asked (its results are
  * then worthless): TV_OK or TV_ERR_DEVICE_TIMEOUT.  Not for a stream that is being captured. */
 int tv_kv_status(int device);

@@ -76,8 +76,18 @@ ATTEND = [
 ]
 
 
+@pytest.fixture
+def prefix_kernel():
+    """Sets which kernel reads prefixes, and puts the rule back."""
+    from turbovec_b200 import kvcache
+    yield lambda value: kvcache.set_option(kvcache.OPT_TENSOR_PREFIX, value)
+    kvcache.set_option(kvcache.OPT_TENSOR_PREFIX, -1)
+
+
+@pytest.mark.parametrize("tensor", [0, 1])
 @pytest.mark.parametrize("case", range(len(ATTEND)))
-def test_attend(case):
+def test_attend(case, tensor, prefix_kernel):
+    prefix_kernel(tensor)
     dtype, dim, page, heads, kv_heads, new, lens, prefix, first, padding = ATTEND[case]
     s = R.Setup(case, dtype=dtype, dim=dim, page=page, heads=heads, kv_heads=kv_heads, new=new, lens=lens, prefix=prefix, tokens_first=first,
                 padding=padding, leading=1 if padding else 0)

@@ -143,6 +143,7 @@ SIGNATURES.update({
     "tv_kv_attend_selected_workspace": (C.c_size_t, [_cachep, _batchp, C.c_int64, C.c_int, C.c_int64]),
     "tv_kv_attend_selected": (C.c_int, [_cachep, _batchp, C.c_int64, C.c_int, _rowsp, C.c_int64, C.c_int64, C.c_int64, C.c_float, _rowsp,
                                         C.c_void_p, C.c_void_p, C.c_void_p, C.c_size_t, C.c_void_p]),
+    "tv_kv_set_option": (C.c_int, [C.c_int, C.c_int64]),
     "tv_kv_status": (C.c_int, [C.c_int]),
 })
 

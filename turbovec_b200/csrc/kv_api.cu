@@ -127,11 +127,18 @@ struct Carver {
         return p;
     }
 };
-// Rows (tokens x heads of a key head) from which a prefix goes to the tensor cores.
-constexpr int64_t kTensorRows = 17;
+// Whether a prefix goes to the tensor-memory kernel.  The warp-level kernel reads it once for every 16 rows, which costs 3.1 us for a million
+// (row, key, key head) triples; the other costs 8 us more to begin with and 0.09 us for a thousand (key, key head) pairs, up to 128
+// rows.  They meet where keys * key heads * (rows - 29) is 2.6 million.  Measured (8 key heads of 128 channels, us, warp-level / tensor):
+// 32 rows, 16,000 keys 27 / 29; 64 rows 41 / 33; 128 rows, 4,000 keys 31 / 31; 256 rows, 500 keys 29 / 33, 2,000 keys 38 / 36, 8,000
+// keys 72 / 42; 64 channels: 64 rows, 8,000 keys 25 / 25, 256 rows, 2,000 keys 27 / 28.
+constexpr int64_t kTensorFrom = 2600000;
+std::atomic<int64_t> g_tensor_prefix{-1};                 // TV_KV_OPT_TENSOR_PREFIX
 void plan_prefix(KvAttendParams &p, const tv_kv_cache *c, int64_t tokens, int heads, int64_t prefix_len, int sm_count) {
     const int group = heads / c->kv_heads;
-    p.tensor_prefix = prefix_len > 0 && tokens * group >= kTensorRows && group <= kKvPrefixRows;     // a tile holds whole tokens
+    const int64_t option = g_tensor_prefix.load(std::memory_order_relaxed);
+    const bool worth = option < 0 ? tokens * group > 29 && prefix_len * c->kv_heads > kTensorFrom / (tokens * group - 29) : option > 0;
+    p.tensor_prefix = prefix_len > 0 && worth && group <= kKvPrefixRows;     // a tile holds whole tokens
     if (p.tensor_prefix) p.plan = kv_prefix_plan(tokens, group, c->kv_heads, int(prefix_len), sm_count);
 }
 size_t carve_attend(KvAttendParams &p, char *base, int64_t slots, int64_t rows, const tv_kv_cache *c, bool prefix) {
@@ -180,7 +187,7 @@ int fill_attend(KvAttendParams &p, const tv_kv_cache *c, const tv_kv_batch *b, i
     p.page_shift = shift_of(c->page_size);
     p.pages = int(c->pages);
     p.scale_log2 = scale * 1.4426950408889634f;
-    p.item_cost = 3;
+    p.item_cost = 4;
     return TV_OK;
 }
 int check_workspace(const void *ws, size_t have, size_t need) {
@@ -319,6 +326,12 @@ int tv_kv_attend_selected(const tv_kv_cache *c, const tv_kv_batch *b, int64_t to
     if (e != cudaSuccess) return cuda_error("selection kernel", e);
     e = launch_kv_attend(p, maps, c->dtype, c->head_dim, true, c->device, sms, static_cast<cudaStream_t>(stream));
     return e == cudaSuccess ? int(TV_OK) : cuda_error("attention kernel", e);
+}
+
+int tv_kv_set_option(int option, int64_t value) {
+    if (option != TV_KV_OPT_TENSOR_PREFIX || value < -1 || value > 1) return refuse("no such option, or no such value of it");
+    g_tensor_prefix.store(value, std::memory_order_relaxed);
+    return TV_OK;
 }
 
 int tv_kv_status(int device) {

@@ -19,7 +19,7 @@ namespace {
 constexpr int kConsumers = 4;
 constexpr int kAttendThreads = (kConsumers + 1) * 32;
 constexpr float kRescaleAt = 8.0f;
-constexpr int kLeastTiles = 3;                           // tiles of a run: joining more parts takes longer than these
+constexpr int kLeastTiles = 2;                           // tiles of a run: joining more parts takes longer than these
 constexpr int kNothing = INT_MAX - kKvTile;              // first position of a group of keys that nobody sees
 
 __device__ uint32_t g_kv_timeouts;

@@ -20,7 +20,10 @@ import torch
 
 from . import _native
 
-__all__ = ["PagedKVCache", "KVBatch"]
+__all__ = ["PagedKVCache", "KVBatch", "OPT_TENSOR_PREFIX", "set_option"]
+
+OPT_TENSOR_PREFIX = 1
+_options = 0                                            # how often an option was set: workspace sizes follow options
 
 _DTYPES = {torch.bfloat16: 0, torch.float16: 1}
 
@@ -54,6 +57,16 @@ def _tensor(name: str, t, dtype, ndim: int, device=None) -> torch.Tensor:
 def _last_adjacent(name: str, t: torch.Tensor) -> None:
     if t.shape[-1] > 1 and t.stride(-1) != 1:
         raise ValueError(f"{name}: the elements of the last dimension must be adjacent")
+
+
+def set_option(option: int, value: int) -> None:
+    """An option of the cache's calls, for the whole process (TV_KV_OPT_* of include/turbovec_b200.h)."""
+    global _options
+    lib = _native.load()
+    rc = lib.tv_kv_set_option(int(option), int(value))
+    if rc:
+        _fail(lib, rc)
+    _options += 1
 
 
 class KVBatch:
@@ -197,7 +210,7 @@ class PagedKVCache:
 
     def _workspace(self, op: str, batch, *sizes) -> torch.Tensor:
         """A workspace for an operator; its size for these sizes is asked for once."""
-        key = (op, batch._view.sequences, *sizes)
+        key = (op, _options, batch._view.sequences, *sizes)
         n = self._sizes.get(key)
         if n is None:
             n = getattr(self._lib, f"tv_kv_{op}_workspace")(self._view, batch._view, *sizes)
