@@ -43,7 +43,7 @@ struct PrefixGeometry {
     static constexpr int kOColumns = D;
 };
 template <int D>
-struct PrefixShared {
+struct alignas(16) PrefixShared {
     uint64_t full[PrefixGeometry<D>::kSlots], empty[PrefixGeometry<D>::kSlots];
     uint64_t s_full[2][2], p_ready[2][2], o_done[2], q_full[2], q_free[2];    // [stream][half of a tile], [stream]
     uint32_t tmem_base;
@@ -468,17 +468,34 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) kv_prefix_kernel(const KvAt
             if (done > 0) {
                 wait(&sh.o_done[s], (o_count + done - 1) & 1);
                 fence_after();
-                float *dst = p.pre_o + (block * kKvPrefixRows + r) * D;
+                // a row to a thread as it comes from tensor memory, rows of 128 bytes as it goes out: each warp turns its 32 rows in 4 KB of
+                // shared memory (stores of 16 bytes in 32 rows at once took 7,000 cycles).  Q has been read by now: its place is used where
+                // there is no other; a stream without a tile of rows of its own uses the second tile's.
+                uint8_t *stage = (D == 64 ? reinterpret_cast<uint8_t *>(&sh + 1) + s * 16384
+                                          : q_smem + (plan.paired ? s * G::kTileBytes : G::kTileBytes + s * 16384)) + (warp & 3) * 4096;
+                const int64_t first_row = row_base + (warp & 3) * 32;
+                const int rows = int(max(int64_t(0), min(live - first_row, int64_t(min(32, plan.rows - (warp & 3) * 32)))));     // of this warp that are there
+                float *dst = p.pre_o + (block * kKvPrefixRows + (warp & 3) * 32) * D;
 #pragma unroll 1
                 for (int c = 0; c < D; c += 32) {
                     uint32_t y[32];
                     tmem_ld32(o_addr + c, y);
                     tmem_wait_ld();
-                    if (have)
 #pragma unroll
-                        for (int j = 0; j < 8; ++j)
-                            *reinterpret_cast<uint4 *>(dst + c + 4 * j) = make_uint4(y[4 * j], y[4 * j + 1], y[4 * j + 2], y[4 * j + 3]);
+                    for (int j = 0; j < 8; ++j)
+                        *reinterpret_cast<uint4 *>(stage + lane * 128 + ((j ^ (lane & 7)) << 4)) = make_uint4(y[4 * j], y[4 * j + 1], y[4 * j + 2], y[4 * j + 3]);
+                    __syncwarp();
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        const int row = 4 * j + (lane >> 3), piece = lane & 7;
+                        if (row < rows) *reinterpret_cast<uint4 *>(dst + row * D + c + 4 * piece) = *reinterpret_cast<const uint4 *>(stage + row * 128 + ((piece ^ (row & 7)) << 4));
+                    }
+                    __syncwarp();
                 }
+                if (D == 128 && plan.paired)                     // the rows of Q's tile that no copy writes are zeros again
+                    for (int row = max((warp & 3) * 32, plan.rows); row < (warp & 3) * 32 + 32; ++row)
+                        if (lane < 8) *reinterpret_cast<uint4 *>(stage + (row - (warp & 3) * 32) * 128 + lane * 16) = make_uint4(0, 0, 0, 0);
+                fence_shared_async();
             }
             o_count += done;
             if (have) p.pre_ml[block * kKvPrefixRows + r] = make_float2(m, l);
@@ -500,8 +517,8 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) kv_prefix_kernel(const KvAt
 template <typename T, int D>
 cudaError_t launch(const KvAttendParams &p, const KvMaps &maps, int device, cudaStream_t s) {
     using G = PrefixGeometry<D>;
-    const size_t smem = G::kQBytes + size_t(G::kSlots) * G::kTileBytes + sizeof(PrefixShared<D>) + 1024;
-    static_assert(G::kQBytes + G::kSlots * G::kTileBytes + sizeof(PrefixShared<D>) + 1024 <= kBlockSharedBytes, "more shared memory than a block can have");
+    constexpr size_t smem = G::kQBytes + G::kSlots * G::kTileBytes + sizeof(PrefixShared<D>) + (D == 64 ? 32768 : 0) + 1024;
+    static_assert(smem <= kBlockSharedBytes, "more shared memory than a block can have");
     auto *kern = kv_prefix_kernel<T, D>;
     static std::atomic<uint64_t> allowed{0};
     const cudaError_t e = kv_allow_shared(kern, allowed, device);
