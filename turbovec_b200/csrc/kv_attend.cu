@@ -552,67 +552,68 @@ __global__ void __launch_bounds__(128) kv_join_kernel(const KvAttendParams p) {
     const int token = int(row / p.heads), head = int(row % p.heads);
     const KvSpan all = kv_span(p.batch.offsets[0], p.batch.offsets[p.batch.sequences], p.tokens);
     if (token < all.first || token >= all.first + all.count) return;       // behind the last sequence: as it was
-    float big = -INFINITY, sum = 0.0f, acc[kPer] = {};
-    // parts at o + i * step, (largest logit, sum) at ml + i * step / D
-    auto add = [&](const float *o, const float2 *ml_at, int64_t step, int count) {
-        if (WARPS > 1) {                             // this warp's parts
-            o += turn * step;
-            ml_at += turn * (step / D);
-            step *= WARPS;
-            count = (count - turn + WARPS - 1) / WARPS;
-        }
-        for (int i0 = 0; i0 < count; i0 += 32) {
-            const int left = min(32, count - i0);
-            const float2 ml = lane < left ? ml_at[(i0 + lane) * (step / D)] : make_float2(-INFINITY, 0.0f);
-            float top = ml.x;
-#pragma unroll
-            for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(kFullMask, top, d));
-            const float next = fmaxf(big, top), base = next == -INFINITY ? 0.0f : next;
-            const float old = kv_exp2(big - base), mine = kv_exp2(ml.x - base);
-            float part = mine * ml.y;
-#pragma unroll
-            for (int d = 16; d > 0; d >>= 1) part += __shfl_xor_sync(kFullMask, part, d);
-            sum = fmaf(sum, old, part);
-            big = next;
-#pragma unroll
-            for (int j = 0; j < kPer; ++j) acc[j] *= old;
-#pragma unroll 8
-            for (int i = 0; i < left; ++i) {
-                const float f = __shfl_sync(kFullMask, mine, i);
-                const float *src = o + (i0 + i) * step + lane * kPer;
-                float x[kPer] = {};
-                if (f != 0.0f) {                     // a part without keys may have no sums
-                    if constexpr (kPer == 4) { const float4 y = *reinterpret_cast<const float4 *>(src); x[0] = y.x; x[1] = y.y; x[2] = y.z; x[3] = y.w; }
-                    else { const float2 y = *reinterpret_cast<const float2 *>(src); x[0] = y.x; x[1] = y.y; }
-                }
-#pragma unroll
-                for (int j = 0; j < kPer; ++j) acc[j] = fmaf(f, x[j], acc[j]);
-            }
-        }
-    };
-    auto add_items = [&](const KvPieces &pc) {
-        if (pc.first_row < 0 || pc.count < 0 || pc.first_row / kKvRows + pc.count > p.slots) return;
-        add(p.part_o + pc.first_row * D, p.part_ml + pc.first_row, int64_t(kKvRows) * D, pc.count);
-    };
     const KvPieces own = p.own_pieces[row];
     if (own.count == 0 && p.prefix_len == 0) return;
+    // Two lists of parts, n1 of a prefix and n2 of the row's own keys: sums o at step floats, (largest logit, sum of weights) at step / D.
+    const float *o1 = nullptr, *o2 = nullptr;
+    const float2 *ml1 = nullptr, *ml2 = nullptr;
+    int64_t step1 = 0;
+    int n1 = 0, n2 = 0;
+    auto of_items = [&](const KvPieces &pc, const float *&o, const float2 *&ml) {
+        if (pc.first_row < 0 || pc.count < 0 || pc.first_row / kKvRows + pc.count > p.slots) return 0;
+        o = p.part_o + pc.first_row * D;
+        ml = p.part_ml + pc.first_row;
+        return pc.count;
+    };
     if (p.tensor_prefix) {
         const int h = head / p.group;                // rows of a key head lie together, token after token
         const int64_t r = int64_t(token - all.first) * p.group + head - h * p.group;
         const KvPrefixPlan &w = p.plan;
-        const int first = int(int64_t(h) * w.tiles / w.per), count = int((int64_t(h + 1) * w.tiles - 1) / w.per) - first + 1;
-        const int64_t block = int64_t(kKvPrefixRows) * D;
-        if (w.paired) {
-            const int64_t at = ((int64_t(h) + first) * w.units * 2 + r / w.rows) * kKvPrefixRows + r % w.rows;
-            add(p.pre_o + at * D, p.pre_ml + at, 2 * w.units * block, count);
-        } else {
-            const int64_t at = (int64_t(h) + first) * 2 * kKvPrefixRows + r;
-            add(p.pre_o + at * D, p.pre_ml + at, block, 2 * count);
-        }
+        const int first = int(divide(h * w.places, w.per)), count = int(divide(h * w.places + w.tiles - 1, w.per)) - first + 1;
+        const int tile = w.paired ? int(uint32_t(r) / uint32_t(w.rows)) : 0, in_tile = int(r) - tile * w.rows;     // r < 2^31: tokens * heads are
+        const int64_t at = ((int64_t(h) + first) * w.units * 2 + tile) * kKvPrefixRows + in_tile;
+        o1 = p.pre_o + at * D;
+        ml1 = p.pre_ml + at;
+        step1 = (w.paired ? 2 * int64_t(w.units) : 1) * kKvPrefixRows * D;       // not paired: both streams of a block, one after the other
+        n1 = w.paired ? count : 2 * count;
     } else if (p.prefix_len > 0) {
-        add_items(p.prefix_pieces[row]);
+        step1 = int64_t(kKvRows) * D;
+        n1 = of_items(p.prefix_pieces[row], o1, ml1);
     }
-    add_items(own);
+    n2 = of_items(own, o2, ml2);
+    constexpr int64_t kStep2 = int64_t(kKvRows) * D;
+    float big = -INFINITY, sum = 0.0f, acc[kPer] = {};
+    const int n = (n1 + n2 - turn + WARPS - 1) / WARPS;                         // parts turn, turn + WARPS, ... are this warp's
+    for (int k0 = 0; k0 < n; k0 += 32) {
+        const int left = min(32, n - k0), mine_at = turn + (k0 + lane) * WARPS;
+        float2 ml = make_float2(-INFINITY, 0.0f);
+        if (lane < left) ml = mine_at < n1 ? ml1[mine_at * (step1 / D)] : ml2[(mine_at - n1) * (kStep2 / D)];
+        float top = ml.x;
+#pragma unroll
+        for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(kFullMask, top, d));
+        const float next = fmaxf(big, top), base = next == -INFINITY ? 0.0f : next;
+        const float old = kv_exp2(big - base), mine = kv_exp2(ml.x - base);
+        float part = mine * ml.y;
+#pragma unroll
+        for (int d = 16; d > 0; d >>= 1) part += __shfl_xor_sync(kFullMask, part, d);
+        sum = fmaf(sum, old, part);
+        big = next;
+#pragma unroll
+        for (int j = 0; j < kPer; ++j) acc[j] *= old;
+#pragma unroll 8
+        for (int k = 0; k < left; ++k) {
+            const float f = __shfl_sync(kFullMask, mine, k);
+            const int i = turn + (k0 + k) * WARPS;
+            const float *src = (i < n1 ? o1 + i * step1 : o2 + (i - n1) * kStep2) + lane * kPer;
+            float x[kPer] = {};
+            if (f != 0.0f) {                         // a part without keys may have no sums
+                if constexpr (kPer == 4) { const float4 y = *reinterpret_cast<const float4 *>(src); x[0] = y.x; x[1] = y.y; x[2] = y.z; x[3] = y.w; }
+                else { const float2 y = *reinterpret_cast<const float2 *>(src); x[0] = y.x; x[1] = y.y; }
+            }
+#pragma unroll
+            for (int j = 0; j < kPer; ++j) acc[j] = fmaf(f, x[j], acc[j]);
+        }
+    }
     if constexpr (WARPS > 1) {
         static_assert(WARPS == 4, "a block is one row");
         if (turn > 0) {

@@ -187,7 +187,8 @@ struct KvPrefixPlan {                        // the same on host and device but 
     int units;                               // row tiles (or pairs) of a key head
     int tiles;                               // key tiles
     int groups;                              // blocks of one unit: they share the (key head, tile) list
-    int64_t per;                             // steps of a block
+    int64_t places;                          // places of a key head in the list: its tiles, and none behind them
+    int64_t per;                             // places of a block
 };
 inline KvPrefixPlan kv_prefix_plan(int64_t tokens, int group, int kv_heads, int prefix_len, int sm_count) {
     KvPrefixPlan w;
@@ -196,11 +197,19 @@ inline KvPrefixPlan kv_prefix_plan(int64_t tokens, int group, int kv_heads, int 
     w.paired = row_tiles > 1;
     w.units = int(w.paired ? (row_tiles + 1) / 2 : 1);
     w.tiles = (prefix_len + kKvPrefixTile - 1) / kKvPrefixTile;
-    const int64_t steps = int64_t(kv_heads) * w.tiles;
     int64_t groups = w.units < sm_count ? sm_count / w.units : 1;
+    const int64_t steps = int64_t(kv_heads) * w.tiles;
     if (groups > steps) groups = steps;
-    w.groups = int(groups);
+    w.places = w.tiles;
     w.per = (steps + groups - 1) / groups;
+    // A block whose run crosses from one key head to the next has a second part: loading Q, starting and ending cost it about four
+    // steps.  If the runs are hardly longer when each lies within a head, they do.
+    const int64_t per_head = groups / kv_heads;
+    if (per_head > 0) {
+        const int64_t within = (w.tiles + per_head - 1) / per_head;
+        if (within <= w.per + 4) { w.per = within; w.places = per_head * within; groups = per_head * kv_heads; }
+    }
+    w.groups = int(groups);
     return w;
 }
 struct KvAttendParams {

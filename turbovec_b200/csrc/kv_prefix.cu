@@ -163,12 +163,15 @@ struct PrefixPart {
     int h, tile0, count;
 };
 __device__ __forceinline__ bool next_part(const KvPrefixPlan &plan, int64_t &at, int64_t end, PrefixPart &w) {
-    if (at >= end) return false;
-    w.h = int(at / plan.tiles);
-    w.tile0 = int(at - int64_t(w.h) * plan.tiles);
-    w.count = int(min(end - at, int64_t(plan.tiles - w.tile0)));
-    at += w.count;
-    return true;
+    while (at < end) {
+        w.h = int(at / plan.places);
+        const int64_t begin = int64_t(w.h) * plan.places, stop = min(end, begin + plan.tiles);
+        w.tile0 = int(at - begin);
+        w.count = int(stop - at);
+        at = min(end, begin + plan.places);
+        if (w.count > 0) return true;
+    }
+    return false;
 }
 
 template <typename T, int D>
@@ -211,7 +214,7 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) kv_prefix_kernel(const KvAt
     asm volatile("griddepcontrol.launch_dependents;");
     const KvSpan all = kv_span(p.batch.offsets[0], p.batch.offsets[p.batch.sequences], p.tokens);
     const int q_first = all.first, q_count = all.count;
-    const int64_t steps = int64_t(p.kv_heads) * plan.tiles;
+    const int64_t steps = int64_t(p.kv_heads) * plan.places;
     int64_t at = min(steps, group * plan.per);
     const int64_t end = min(steps, at + plan.per);
     const int lookahead = plan.paired ? 1 : 2;                   // tiles of keys whose logits are under way
