@@ -399,8 +399,9 @@ __global__ void __launch_bounds__(kAttendThreads, 2) kv_attend_kernel(const KvAt
             t0 = fmaxf(t0, __shfl_xor_sync(kFullMask, t0, 2)); t1 = fmaxf(t1, __shfl_xor_sync(kFullMask, t1, 2));
             // a maximum that grows by less than 2^8 stays: weights are below 2^8 then, which neither type nor the sums mind
             if (__any_sync(kFullMask, t0 > m0 + kRescaleAt || t1 > m1 + kRescaleAt)) {
-                const float n0 = fmaxf(m0, t0), n1 = fmaxf(m1, t1);
-                const float a0 = n0 == -INFINITY ? 1.0f : kv_exp2(m0 - n0), a1 = n1 == -INFINITY ? 1.0f : kv_exp2(m1 - n1);
+                // (for the rows that need it: what the others give must not depend on their neighbours)
+                const float n0 = t0 > m0 + kRescaleAt ? t0 : m0, n1 = t1 > m1 + kRescaleAt ? t1 : m1;
+                const float a0 = n0 == m0 ? 1.0f : kv_exp2(m0 - n0), a1 = n1 == m1 ? 1.0f : kv_exp2(m1 - n1);
                 m0 = n0; m1 = n1;
                 l0 *= a0; l1 *= a1;
 #pragma unroll

@@ -433,8 +433,9 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) kv_prefix_kernel(const KvAt
                 if (done > 0) {
                     const float top = largest();
                     if (__any_sync(kFullMask, !(top <= m + kRescaleAt))) {
-                        // (a NaN becomes the maximum: the polynomial would lose it)
-                        const float next = max3_nan(m, top, top), f = next == -INFINITY ? 1.0f : kv_exp2(m - next);
+                        // For the rows that need it: what the others give must not depend on their neighbours.  (A NaN becomes the maximum: the
+                        // polynomial would lose it.)
+                        const float next = top <= m + kRescaleAt ? m : max3_nan(m, top, top), f = next == m ? 1.0f : kv_exp2(m - next);
                         m = next;
                         l *= f;
                         wait(&sh.o_done[s], (o_count + done - 1) & 1);      // (the half before that had ended when these logits were there)
