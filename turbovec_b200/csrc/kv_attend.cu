@@ -219,8 +219,13 @@ __device__ __forceinline__ void tma_load_page(void *dst, const CUtensorMap *map,
 __device__ __forceinline__ void ldmatrix4(uint32_t addr, uint32_t (&r)[4]) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
 }
-__device__ __forceinline__ void ldmatrix4_trans(uint32_t addr, uint32_t (&r)[4]) {
-    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+// (a constant offset is part of the instruction)
+template <int OFFSET, bool TRANS>
+__device__ __forceinline__ void ldmatrix4_at(uint32_t addr, uint32_t (&r)[4]) {
+    if constexpr (TRANS)
+        asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4 + %5];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr), "n"(OFFSET) : "memory");
+    else
+        asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4 + %5];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr), "n"(OFFSET) : "memory");
 }
 template <typename T>
 __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
@@ -334,6 +339,9 @@ __global__ void __launch_bounds__(kAttendThreads, 2) kv_attend_kernel(const KvAt
     // row of this lane's ldmatrix address, and its 16-byte chunk before the swizzle
     const int k_row = warp * 16 + ((lane >> 4) & 1) * 8 + (lane & 7), k_chunk = (lane >> 3) & 1;
     const int v_row = warp * 16 + ((lane >> 3) & 1) * 8 + (lane & 7), v_chunk = (lane >> 4) & 1;
+    // Piece 2 i + chunk of row r lies at place (2 i + chunk) ^ (r & 7) of its 128 bytes: the place of i = 0, of which 2 i flips bits that no other part
+    // of the address has.
+    const uint32_t k_at = ring_addr + k_row * 128 + ((k_chunk ^ (k_row & 7)) << 4), v_at = ring_addr + G::kOperandBytes + v_row * 128 + ((v_chunk ^ (v_row & 7)) << 4);
     while (walk.next(w)) {
         const int last = walk.last_tile(w);
         uint32_t qf[D / 16][4];
@@ -361,14 +369,14 @@ __global__ void __launch_bounds__(kAttendThreads, 2) kv_attend_kernel(const KvAt
         for (int tile = w.tile0; tile < last; ++tile, ++n) {
             const int s = n % G::kStages;
             if (ok) ok = mbar_wait(&sh.full[s], (n / G::kStages) & 1, p.timeouts);
-            const uint32_t k_addr = ring_addr + s * G::kStageBytes, v_addr = k_addr + G::kOperandBytes;
+            const uint32_t k_addr = k_at + s * G::kStageBytes, v_addr = v_at + s * G::kStageBytes;
             const int first = sh.first_key[s][warp];
             // all of K's fragments first, so that their loads overlap; two accumulators to a product halve the chain of MMAs
             uint32_t kf[D / 16][4];
 #pragma unroll
-            for (int i = 0; i < D / 16; ++i) {
-                const int chunk = 2 * i + k_chunk;
-                ldmatrix4(k_addr + (chunk >> 3) * G::kHalfBytes + k_row * 128 + (((chunk & 7) ^ (k_row & 7)) << 4), kf[i]);
+            for (int i = 0; i < 4; ++i) {
+                ldmatrix4_at<0, false>(k_addr ^ (i << 5), kf[i]);
+                if constexpr (D == 128) ldmatrix4_at<G::kHalfBytes, false>(k_addr ^ (i << 5), kf[i + 4]);
             }
             float sc[2][4] = {}, sd[2][4] = {};
 #pragma unroll
@@ -431,8 +439,8 @@ __global__ void __launch_bounds__(kAttendThreads, 2) kv_attend_kernel(const KvAt
             // values of keys that no row sees: zero, for 0 * NaN is not 0
             auto live_mask = [&](int key, int limit) { return (key < limit ? 0xffffu : 0u) | (key + 1 < limit ? 0xffff0000u : 0u); };
             auto values = [&](int i, uint32_t (&vf)[4]) {
-                const int chunk = 2 * i + v_chunk;
-                ldmatrix4_trans(v_addr + (chunk >> 3) * G::kHalfBytes + v_row * 128 + (((chunk & 7) ^ (v_row & 7)) << 4), vf);
+                if (i < 4) ldmatrix4_at<0, true>(v_addr ^ ((i & 3) << 5), vf);
+                else ldmatrix4_at<G::kHalfBytes, true>(v_addr ^ ((i & 3) << 5), vf);
             };
             auto product = [&](const uint32_t (&a)[4], const uint32_t (&rest)[4], int limit) {
                 const bool all = first + 16 <= limit;
@@ -443,7 +451,7 @@ __global__ void __launch_bounds__(kAttendThreads, 2) kv_attend_kernel(const KvAt
 #pragma unroll
                     for (int i = 0; i < 4; ++i) values(i0 + i, vf[i]);
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) { vf[i][0] &= x0; vf[i][1] &= x1; vf[i][2] &= x0; vf[i][3] &= x1; }
+                    for (int i = 0; i < 4 && !all; ++i) { vf[i][0] &= x0; vf[i][1] &= x1; vf[i][2] &= x0; vf[i][3] &= x1; }
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         mma16816<T>(o[2 * (i0 + i)], a, vf[i][0], vf[i][1]);
@@ -469,26 +477,41 @@ __global__ void __launch_bounds__(kAttendThreads, 2) kv_attend_kernel(const KvAt
                 }
                 apart = __any_sync(kFullMask, odd);
             }
-            if (!apart) {
-                product(pf, pr, lim_last);
-            } else {
+            if (apart) {
+                // They are taken out of the tile, this warp's 16 rows of which nobody else reads, and added where they belong: to the rows that
+                // see them they give what they are.  (The sums to add wait where the part's result goes later.)
+                for (int i = lane; i < kKvRows * (D + 4); i += 32) (&sh.o[warp][0][0])[i] = 0.0f;
+                __syncwarp();
 #pragma unroll 1
-                for (int limit = lim_first; limit <= lim_last; ++limit) {   // one token's rows after the other
-                    const bool on0 = have0 && lim0 == limit, on1 = have1 && lim1 == limit;
-                    if (!__any_sync(kFullMask, on0 || on1)) continue;
-                    const uint32_t a[4] = {on0 ? pf[0] : 0u, on1 ? pf[1] : 0u, on0 ? pf[2] : 0u, on1 ? pf[3] : 0u};
-                    float keep[D / 8][4];
-#pragma unroll
-                    for (int j = 0; j < D / 8; ++j)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) keep[j][e] = o[j][e];
-                    const uint32_t rest[4] = {on0 ? pr[0] : 0u, on1 ? pr[1] : 0u, on0 ? pr[2] : 0u, on1 ? pr[3] : 0u};
-                    product(a, rest, limit);
-#pragma unroll
-                    for (int j = 0; j < D / 8; ++j) {
-                        if (!on0) { o[j][0] = keep[j][0]; o[j][1] = keep[j][1]; }
-                        if (!on1) { o[j][2] = keep[j][2]; o[j][3] = keep[j][3]; }
+                for (int r = 0; r < 16; ++r) {
+                    const int key = first + r;
+                    if (key < lim_first || key >= lim_last) continue;
+#pragma unroll 1
+                    for (int word = lane; word < D / 2; word += 32) {
+                        uint32_t *at = reinterpret_cast<uint32_t *>(ring + s * G::kStageBytes + G::kOperandBytes + (word >> 5) * G::kHalfBytes + (warp * 16 + r) * 128 +
+                                                                    ((((word >> 2) & 7) ^ (r & 7)) << 4)) + (word & 3);
+                        const uint32_t x = *at;
+                        if (!not_finite<T>(x)) continue;
+                        const bool low = not_finite<T>(x & 0xffffu), high = not_finite<T>(x & 0xffff0000u);
+                        const float2 z = KvType<T>::unpack(x);
+                        *at = (low ? 0u : x & 0xffffu) | (high ? 0u : x & 0xffff0000u);
+                        for (int row = 0; row < w.rows; ++row) {
+                            if (key >= walk.limit(w, (w.row0 + row) / p.group)) continue;
+                            if (low) sh.o[warp][row][2 * word] += z.x;
+                            if (high) sh.o[warp][row][2 * word + 1] += z.y;
+                        }
                     }
+                    __syncwarp();
+                }
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");      // before the next copy into the tile
+            }
+            product(pf, pr, lim_last);
+            if (apart) {
+#pragma unroll
+                for (int j = 0; j < D / 8; ++j) {
+                    const float2 x = *reinterpret_cast<const float2 *>(&sh.o[warp][r0][8 * j + c2]), y = *reinterpret_cast<const float2 *>(&sh.o[warp][r1][8 * j + c2]);
+                    o[j][0] += x.x; o[j][1] += x.y;
+                    o[j][2] += y.x; o[j][3] += y.y;
                 }
             }
             __syncwarp();
