@@ -33,7 +33,7 @@ struct Geometry {
 };
 template <int D>
 struct AttendShared {
-    float o[kConsumers][kKvRows][D + 4];
+    float o[kConsumers][kKvRows][D + 8];
     uint16_t q[kKvRows][D + 8];                          // rows of Q, a row's banks four words from the one before it
     float2 ml[kConsumers][kKvRows], total[kKvRows];
     int first_key[Geometry<D>::kStages][kConsumers];
@@ -480,7 +480,7 @@ __global__ void __launch_bounds__(kAttendThreads, 2) kv_attend_kernel(const KvAt
             if (apart) {
                 // They are taken out of the tile, this warp's 16 rows of which nobody else reads, and added where they belong: to the rows that
                 // see them they give what they are.  (The sums to add wait where the part's result goes later.)
-                for (int i = lane; i < kKvRows * (D + 4); i += 32) (&sh.o[warp][0][0])[i] = 0.0f;
+                for (int i = lane; i < kKvRows * (D + 8); i += 32) (&sh.o[warp][0][0])[i] = 0.0f;
                 __syncwarp();
 #pragma unroll 1
                 for (int r = 0; r < 16; ++r) {

@@ -60,7 +60,7 @@ __global__ void __launch_bounds__(kSelectThreads, 2) kv_select_kernel(const KvSe
     uint32_t *keys = reinterpret_cast<uint32_t *>(dynamic + kRingBytes<D>);     // scores in ascending order of their bits; 0: no such page in the pool
     __shared__ __align__(16) int8_t q8[kKvRows][2 * D];
     __shared__ SelectShared sh;
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, token = blockIdx.x / blocks, h = blockIdx.y;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, item = blockIdx.x / blocks, token = item / p.kv_heads, h = item % p.kv_heads;
     const int rank = blocks > 1 ? int(cluster_ctarank()) : 0;              // clusters lie along x
 
     if (blocks > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");   // this block has begun: others may write into it
@@ -348,7 +348,7 @@ cudaError_t launch(const KvSelectParams &p, int device, int sm_count, cudaStream
     attrs[1].id = cudaLaunchAttributeClusterDimension;
     attrs[1].val.clusterDim.x = unsigned(blocks); attrs[1].val.clusterDim.y = 1; attrs[1].val.clusterDim.z = 1;
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(unsigned(p.tokens) * unsigned(blocks), unsigned(p.kv_heads));
+    cfg.gridDim = dim3(unsigned(items * blocks));       // the heads of a token side by side: their bounds lie side by side in every page
     cfg.blockDim = dim3(kSelectThreads);
     cfg.dynamicSmemBytes = kRingBytes<D> + size_t(p.batch.table_width) * 4;
     cfg.stream = s;
