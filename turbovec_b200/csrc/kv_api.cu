@@ -46,6 +46,7 @@ int refuse(const char *message) { return set_create_error(TV_ERR_INVALID_ARGUMEN
 int unsupported(const char *message) { return set_create_error(TV_ERR_UNSUPPORTED, message); }
 int cuda_error(const char *what, cudaError_t e) {
     char text[256];
+    cudaGetLastError();                                        // reported here: it does not wait for the caller's next call
     std::snprintf(text, sizeof text, "%s: %s", what, cudaGetErrorString(e));
     return set_create_error(TV_ERR_CUDA, text);
 }
