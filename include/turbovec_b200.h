@@ -373,6 +373,8 @@ int tv_v7_plan_sync(size_t n_synced, size_t n, const size_t *pending, size_t n_p
  * caller's current device is left as it was.  Failures that the host can see are returned, with a message in
  * tv_last_error(NULL).
  *
+ * Of `heads` query heads, head j reads key head j / (heads / kv_heads).
+ *
  * A pool has `pages` pages of page_size (16, 32, 64 or 128) tokens for each of kv_heads key heads; head_dim is 64 or 128; dtype
  * holds for keys, values, queries and outputs.  K and V are views [page][key head][token][channel] with channels adjacent and
  * the other strides in elements, positive multiples of 8; 16-byte aligned.  bounds [page][key head][lowest, highest][channel]
@@ -414,9 +416,9 @@ int tv_kv_append(const tv_kv_cache *cache, const tv_kv_batch *batch, int64_t tok
                  int64_t positions, int rotary, int interleaved, int64_t position_offset, void *stream);
 /* out = softmax(scale * q k) v over the first prefix_len keys of the pages prefix_pages (prefix_width of them; none: 0) and the
  * keys of the row's own sequence at positions up to p.  lse (may be null): natural logarithm of the sum of exponentials,
- * [token][head].  A row that sees no key gives zeros and -infinity.  What a row does not see never
- * reaches it, NaN and infinities included; an infinite value that it sees gives an infinity or NaN.  The workspace needs tv_kv_attend_workspace bytes (256-byte
- * aligned), belongs to the call until its work is done, and need not be cleared. */
+ * [token][head].  A row that sees no key gives zeros and -infinity.  What a row does not see never reaches it, NaN and infinities
+ * included; an infinite value that it sees gives an infinity or NaN.  out must not overlap q.  The workspace needs
+ * tv_kv_attend_workspace bytes (256-byte aligned), belongs to the call until its work is done, and need not be cleared. */
 size_t tv_kv_attend_workspace(const tv_kv_cache *cache, const tv_kv_batch *batch, int64_t tokens, int heads, int64_t prefix_len);
 int tv_kv_attend(const tv_kv_cache *cache, const tv_kv_batch *batch, int64_t tokens, int heads, const tv_kv_rows *q,
                  const int32_t *prefix_pages, int64_t prefix_width, int64_t prefix_len, float scale, const tv_kv_rows *out,

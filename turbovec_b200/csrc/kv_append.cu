@@ -1,8 +1,12 @@
 // Appending keys and values to the pages of a cache, with the position rotation and the pages' bounds.
 //
-// A block takes one page that a sequence's new tokens touch, and one key head: it rotates the page's new keys and the queries of
-// that head's group, copies the values, and brings the page's bounds up to date.  A page belongs to one block, so bounds need no
-// atomics and no order matters.
+// A block takes one page that a sequence's new tokens touch, and one to eight key heads (whole warps each): it rotates the page's new
+// keys and the queries of the heads' groups, copies the values, and brings the page's bounds up to date.  A page and head belongs to
+// one block, so bounds need no atomics and no order matters.  A thread takes 16 channels of a token: key, value and the group's
+// queries, whose angles it reads once.
+//
+// Bound by memory where there are many tokens (append_prompts_4, 32,818 tokens of 8 + 32 heads of 128 channels, 824 MB: 149 us, 5.5 TB/s),
+// by dependent loads where there are few (place in the batch, page, rows: 6.1 us for one token).
 //
 // Rotation: (y1, y2) = (x1 cos - x2 sin, x2 cos + x1 sin) in 32 bits, each product and sum rounded by itself, then to the type.
 // Bounds: for every channel the lowest and highest key of the page, as int8 multiples of one power of two 2^e per page and key head,

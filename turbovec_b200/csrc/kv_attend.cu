@@ -6,8 +6,11 @@
 // ends inside an item leaves partial results, (largest logit, sum of weights, weighted sum of values), in slot
 // item + block, a number that is different for every pair of the two that meet; a second kernel joins them.
 //
-// Bound by memory: a tile of 128 channels is 32 KB and 4 * 64 * 128 * 16 multiply-adds of which 16 / rows are padding.  One warp keeps the
-// ring of tiles full by tensor copies; four warps take 16 keys of each tile: no exchange between warps until the end of a part.
+// Bound by memory: a tile of 128 channels is 32 KB and 4 * 64 * 128 * 16 multiply-adds, most of them padding where rows are few.  One warp
+// keeps the ring of tiles full by tensor copies; four warps take 16 keys of each tile: no exchange between warps until the end of a
+// part.  What a part costs beside its tiles is weighed as four tiles when the list is divided (2, 3, 4, 5, 6: attend_48_ragged 60.0, 54.2, 54.8,
+// 55.4, 55.7 us a call, attend_24_drafts_prefix_8200 57.1, 55.4, 52.8, 53.0, 52.5).  attend_48_ragged, 48 sequences of 1 to 12,000 keys,
+// 274 MB: 52.6 us for this kernel, 5.2 TB/s.
 #include <cfloat>
 
 #include "kv_cache.cuh"

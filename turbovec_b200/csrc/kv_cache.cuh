@@ -181,7 +181,7 @@ struct KvPieces {
 // Partial results of the tensor-memory form for a prefix (kv_prefix.cu): blocks of 128 rows.
 constexpr int kKvPrefixRows = 128;           // M of tcgen05.mma
 constexpr int kKvPrefixTile = 128;           // keys of one step
-struct KvPrefixPlan {                        // the same on host and device but for `live_rows`
+struct KvPrefixPlan {                        // computed alike on host and device
     int rows;                                // rows of a tile: whole tokens
     bool paired;                             // two row tiles to a block, which share its keys; else one, its keys dealt to two streams
     int units;                               // row tiles (or pairs) of a key head
