@@ -418,7 +418,8 @@ int tv_kv_append(const tv_kv_cache *cache, const tv_kv_batch *batch, int64_t tok
  * keys of the row's own sequence at positions up to p.  lse (may be null): natural logarithm of the sum of exponentials,
  * [token][head].  A row that sees no key gives zeros and -infinity.  What a row does not see never reaches it, NaN and infinities
  * included; an infinite value that it sees gives an infinity or NaN.  out must not overlap q.  The workspace needs
- * tv_kv_attend_workspace bytes (256-byte aligned), belongs to the call until its work is done, and need not be cleared. */
+ * tv_kv_attend_workspace bytes (256-byte aligned; 0 with a message in tv_last_error(NULL): the sizes are refused), belongs to the
+ * call until its work is done, and need not be cleared. */
 size_t tv_kv_attend_workspace(const tv_kv_cache *cache, const tv_kv_batch *batch, int64_t tokens, int heads, int64_t prefix_len);
 int tv_kv_attend(const tv_kv_cache *cache, const tv_kv_batch *batch, int64_t tokens, int heads, const tv_kv_rows *q,
                  const int32_t *prefix_pages, int64_t prefix_width, int64_t prefix_len, float scale, const tv_kv_rows *out,

@@ -130,3 +130,18 @@ def test_bounds_do_not_depend_on_how_keys_arrive(seed):
         both, step = torch.stack([torch.minimum(torch.floor(old[0]), lo), torch.maximum(torch.ceil(old[1]), hi)]), wide
     want, s = R.bounds_of(keys)
     assert s == step and torch.equal(both, want)
+
+
+def test_workspace_sizes_that_cannot_be_are_refused_with_a_message(lib):
+    _, _, cache, batch, _ = views()
+    assert call(lib, "attend", scale=-1.0) == 90                        # a message that must not be met again below
+    for prefix_len in (-1, (1 << 30) + 1, 1 << 32, 1 << 62):
+        assert lib.tv_kv_attend_workspace(cache, batch, 1, 4, prefix_len) == 0
+        assert b"prefix_len" in lib.tv_last_error(None), prefix_len
+    for budget in (0, -1, 40_000, 1 << 40):
+        assert lib.tv_kv_attend_selected_workspace(cache, batch, 1, 4, budget) == 0
+        assert b"budget" in lib.tv_last_error(None), budget
+    cache.device = 63                                                   # no machine has so many
+    for size in (lib.tv_kv_attend_workspace(cache, batch, 1, 4, 20), lib.tv_kv_attend_selected_workspace(cache, batch, 1, 4, 2)):
+        assert size == 0
+        assert b"no such CUDA device" in lib.tv_last_error(None)

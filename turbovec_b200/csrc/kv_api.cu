@@ -240,8 +240,9 @@ int tv_kv_append(const tv_kv_cache *c, const tv_kv_batch *b, int64_t tokens, int
 
 size_t tv_kv_attend_workspace(const tv_kv_cache *c, const tv_kv_batch *b, int64_t tokens, int heads, int64_t prefix_len) {
     if (check_common(c, b, tokens, heads) != TV_OK) return 0;
+    if (prefix_len < 0 || prefix_len > kMaxCount) { refuse("prefix_len must be between 0 and 2^30"); return 0; }
     const int sms = sm_count_of(c->device);
-    if (sms == 0) return 0;
+    if (sms == 0) { set_create_error(TV_ERR_CUDA, "no such CUDA device"); return 0; }
     KvAttendParams p{};
     plan_prefix(p, c, tokens, heads, prefix_len, sms);
     const bool items = prefix_len > 0 && !p.tensor_prefix;
@@ -286,10 +287,13 @@ int tv_kv_attend(const tv_kv_cache *c, const tv_kv_batch *b, int64_t tokens, int
 }
 
 size_t tv_kv_attend_selected_workspace(const tv_kv_cache *c, const tv_kv_batch *b, int64_t tokens, int heads, int64_t budget) {
-    if (check_common(c, b, tokens, heads) != TV_OK || budget < 1 || budget > kKvMaxScored) return 0;
+    if (check_common(c, b, tokens, heads) != TV_OK) return 0;
+    if (budget < 1 || budget > kKvMaxScored) { refuse("budget must be between 1 and 32,768"); return 0; }
+    const int sms = sm_count_of(c->device);
+    if (sms == 0) { set_create_error(TV_ERR_CUDA, "no such CUDA device"); return 0; }
     KvAttendParams p{};
     KvSelectParams s{};
-    return carve_chosen(p, s, nullptr, chosen_slots(c, tokens, heads, sm_count_of(c->device)), tokens, tokens * heads, tokens * c->kv_heads * budget, c);
+    return carve_chosen(p, s, nullptr, chosen_slots(c, tokens, heads, sms), tokens, tokens * heads, tokens * c->kv_heads * budget, c);
 }
 
 int tv_kv_attend_selected(const tv_kv_cache *c, const tv_kv_batch *b, int64_t tokens, int heads, const tv_kv_rows *q, int64_t budget, int64_t first,
