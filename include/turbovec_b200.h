@@ -384,7 +384,8 @@ int tv_v7_plan_sync(size_t n_synced, size_t n, const size_t *pending, size_t n_p
  * numbers), and stands at position p = lens[b] - (offsets[b + 1] - offsets[b]) + j of the sequence's own pages, so lens counts the
  * tokens of the call.  table[b] lists the pages of sequence b.  Rows outside [offsets[0], offsets[sequences]) are left as they are.
  * What the host cannot see is checked on the device: a page number outside the pool holds no keys and stores none, positions
- * below 0 or behind the table do not exist, offsets are cut to the call's rows.  Two sequences may share pages that are
+ * below 0 or behind the table do not exist, offsets are cut to the call's rows (where they do not ascend, rows of the call and pages
+ * of the table may hold anything afterwards, and nothing else changes).  Two sequences may share pages that are
  * read; no two tokens of one tv_kv_append may go into the same place, nor new tokens of two sequences into one page. ---- */
 enum { TV_KV_BF16 = 0, TV_KV_F16 = 1 };
 typedef struct tv_kv_cache {

@@ -602,3 +602,28 @@ def test_equal_calls_give_equal_bits():
     for _ in range(3):
         out, lse = attend(s)
         assert torch.equal(out, first) and torch.equal(lse, first_lse)
+
+
+@pytest.mark.parametrize("tensor", [0, 1])
+@pytest.mark.parametrize("offsets", [[2, 6, 3, 9], [9, 5, 4, 2], [-4, 100, 1, 2 ** 31 - 1], [-2 ** 31, 8, -1, 8]])
+def test_offsets_that_do_not_ascend_stay_within_the_call(offsets, tensor, prefix_kernel):
+    """Such rows have no meaning, but the calls end, and write to their own rows and to pages of the table alone."""
+    prefix_kernel(tensor)
+    s = R.Setup(35, dtype=BF, dim=128, page=16, heads=4, kv_heads=2, new=[4, 3, 2], lens=[100, 300, 20], prefix=400)
+    cache, batch = handles(s)
+    batch.offsets.copy_(torch.tensor(offsets, dtype=torch.int32))
+    heads, rows = s.heads, s.tokens
+    around = torch.full((rows + 16, heads, s.dim), 7.0, dtype=s.dtype, device="cuda")
+    out, lse_around = around[8:8 + rows], torch.full((rows + 16, heads), 7.0, device="cuda")
+    q = s.q.cuda()
+    cache.attend(batch, q, out=out, lse=lse_around[8:8 + rows], prefix_pages=s.prefix_pages.cuda(), prefix_len=s.prefix)
+    cache.attend_selected(batch, q, budget=3, out=out, lse=lse_around[8:8 + rows])
+    used = set(s.table.flatten().tolist())
+    unused = torch.tensor([p for p in range(s.pages) if p not in used], device="cuda")
+    before = cache.k[unused].clone(), cache.v[unused].clone(), cache.bounds[unused].clone(), cache.scales[unused].clone()
+    cache.append(batch, s.k_new.cuda(), s.v_new.cuda(), q=q, q_out=out)
+    cache.check()
+    assert unused.numel() > 0 and (around[:8] == 7).all() and (around[8 + rows:] == 7).all()
+    assert (lse_around[:8] == 7).all() and (lse_around[8 + rows:] == 7).all()
+    for got, want in zip((cache.k, cache.v, cache.bounds, cache.scales), before):
+        assert torch.equal(got[unused], want)

@@ -566,7 +566,7 @@ __global__ void __launch_bounds__(kAttendThreads, 2) kv_attend_kernel(const KvAt
 #pragma unroll
                 for (int i = 0; i < kPer / 2; ++i) dst[i] = KvType<T>::pack(x[2 * i] * inv, x[2 * i + 1] * inv);
                 if (lane == 0 && p.lse) p.lse[token * p.heads + head] = any ? (total.x + log2f(total.y)) * 0.6931471805599453f : -INFINITY;
-            } else if (slot < p.slots) {
+            } else if (uint64_t(slot) < uint64_t(p.slots)) {               // (offsets that do not ascend can give more items than there are slots)
                 float *dst = p.part_o + (slot * kKvRows + r) * D + lane * kPer;
                 if constexpr (kPer == 4) *reinterpret_cast<float4 *>(dst) = make_float4(x[0], x[1], x[2], x[3]);
                 else *reinterpret_cast<float2 *>(dst) = make_float2(x[0], x[1]);

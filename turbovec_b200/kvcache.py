@@ -12,7 +12,7 @@ offsets[b]) + j of the sequence's own pages, table[b][position // page_size].  R
 
 Everything runs on torch's current stream of the cache's device, without a synchronisation, and may be captured into a CUDA graph;
 results and workspaces come from torch's allocator.  Tensors are read when the kernels run: table, lens and offsets may be changed
-in place between calls, and a captured graph sees the new values.  There is no CPU path.
+in place between calls, and a captured graph sees the new values.  There is no CPU path, and no gradient passes through.
 """
 from __future__ import annotations
 
