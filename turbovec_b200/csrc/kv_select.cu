@@ -8,7 +8,7 @@
 //
 // The kernel is a chain of dependent steps (sequence, quantised queries, scores, histogram, list), each a latency of its own; the bounds alone
 // (2 D bytes a page and head) would be a fraction of its time.  selected_48x65536, 830 pages to each of 192 (token, head) pairs, 41 MB of
-// bounds: 22.8 us, 1.8 TB/s; selected_16_ragged, 23 MB: 23.6 us; selected_1x32000, 1 MB: 8.3 us.
+// bounds: 21.8 us, 1.9 TB/s; selected_16_ragged, 23 MB: 22.4 us; selected_1x32000, 1 MB: 7.7 us.
 //
 // A cluster of blocks takes one token and key head: all of them score pages, into the shared memory of the first, which chooses.
 // Scores: int8 MMAs, query heads on the M side, 8 pages on the N side; a lane's 16-byte
@@ -44,7 +44,9 @@ __device__ __forceinline__ uint32_t load_cluster(uint32_t addr) {
 __device__ __forceinline__ void copy16(uint32_t to, const void *from) { asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory"); }
 
 constexpr int kBinBits = 11, kBins = 1 << kBinBits;
-constexpr int kDepth = 4;                                 // runs of 8 pages that a warp has under way
+// Runs of 8 pages that a warp has under way.  1, 2, 3, 4: selected_1x32000 18.3, 18.5, 18.9, 19.2 us a call, selected_16_ragged 51.8, 49.3, 49.8, 50.4,
+// selected_48x65536 93.3, 90.7, 91.5, 91.6: 16 warps on a multiprocessor hide the latency with two, and more is more to begin.
+constexpr int kDepth = 2;
 template <int D>
 constexpr int kRingBytes = kSelectWarps * kDepth * 8 * 2 * D;   // bounds on their way: [warp][run][8 pages][2 D]
 struct SelectShared {
