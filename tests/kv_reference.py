@@ -162,3 +162,57 @@ def rotate(x, cos, sin, interleaved):
     mag[:, i1] = mag[:, i2] = (x1.abs() + x2.abs())
     # two products and a sum, each half a step of 2^-23 off, then half a step of the type
     return y, y.abs() * torch.finfo(x.dtype).eps / 2 + mag * 2 * 2.0 ** -24 * (1 + torch.finfo(x.dtype).eps) + 2.0 ** -25
+
+
+def attend_sequence(s, scale=None, weight_step=None):
+    """attend() for a setup of one sequence, all rows of a head at once: (out [new, heads, dim], lse [new, heads], their tolerances) of the
+    sequence's rows in order.  weight_step: half a step of what the weights are rounded to (None: the type's)."""
+    assert len(s.lens) == 1
+    scale = s.dim ** -0.5 if scale is None else scale
+    pre, own = s.prefix_keys(), s.own_keys(0, s.lens[0] - 1)
+    pp, oo = [p for p, _ in pre + own], [o for _, o in pre + own]
+    place = [i * s.page + o for i in range(s.table.shape[1]) if s.page_at(0, i) is not None for o in range(s.page) if i * s.page + o < s.lens[0]]
+    rows = [(t, p) for t, _, p in s.rows()]
+    at = [t for t, _ in rows]
+    pos = torch.tensor([p for _, p in rows])
+    hidden = torch.cat([torch.zeros(len(rows), len(pre), dtype=torch.bool), torch.tensor(place, dtype=torch.long)[None] > pos[:, None]], 1)
+    group, half = s.heads // s.kv_heads, torch.finfo(s.dtype).eps / 2
+    step = half if weight_step is None else weight_step
+    out, lse = torch.zeros(len(rows), s.heads, s.dim, dtype=torch.float64), torch.zeros(len(rows), s.heads, dtype=torch.float64)
+    tol, ltol = out.clone(), lse.clone()
+    for h in range(s.kv_heads):
+        k, v = s.k[pp, h, oo].double(), s.v[pp, h, oo].double()
+        for j in range(h * group, (h + 1) * group):
+            q = s.q[at, j].double()
+            logits = (q @ k.T * scale).masked_fill(hidden, -math.inf)
+            lse[:, j] = torch.logsumexp(logits, -1)
+            w = torch.exp(logits - lse[:, j, None])
+            out[:, j] = w @ v
+            # the tolerances of attention() above
+            delta = (q.abs() @ k.abs().T).masked_fill(hidden, 0.0).amax(-1) * scale * (s.dim + 4) * 2.0 ** -23 + 2.0 ** -18
+            tol[:, j] = out[:, j].abs() * half + (w @ v.abs()) * (step + 2 * delta)[:, None] * (1 + half) + torch.finfo(s.dtype).tiny
+            ltol[:, j] = delta + lse[:, j].abs() * 2.0 ** -22
+    return out, lse, tol, ltol
+
+
+def prefix_parts(tokens, group, kv_heads, prefix, multiprocessors):
+    """What the tensor-memory kernel for a prefix makes of these sizes (kv_prefix_plan of csrc/kv_cache.cuh, restated): whether two tiles of
+    rows share a block, and for each group of blocks the (key head, tiles of keys) of its parts."""
+    rows = 128 // group * group
+    row_tiles = -(-tokens * group // rows)
+    paired = row_tiles > 1
+    units, tiles = ((row_tiles + 1) // 2 if paired else 1), -(-prefix // 128)
+    groups = min(multiprocessors // units if units < multiprocessors else 1, kv_heads * tiles)
+    places, per = tiles, -(-kv_heads * tiles // groups)
+    of_head = groups // kv_heads
+    if of_head > 0 and -(-tiles // of_head) <= per + 4:
+        per, groups = -(-tiles // of_head), of_head * kv_heads
+        places = of_head * per
+    parts = []
+    for g in range(groups):
+        mine = {}
+        for at in range(g * per, min((g + 1) * per, kv_heads * places)):
+            if at % places < tiles:
+                mine[at // places] = mine.get(at // places, 0) + 1
+        parts.append(list(mine.items()))
+    return paired, units, parts

@@ -145,3 +145,14 @@ def test_workspace_sizes_that_cannot_be_are_refused_with_a_message(lib):
     for size in (lib.tv_kv_attend_workspace(cache, batch, 1, 4, 20), lib.tv_kv_attend_selected_workspace(cache, batch, 1, 4, 2)):
         assert size == 0
         assert b"no such CUDA device" in lib.tv_last_error(None)
+
+
+def test_the_restatement_of_one_sequence_is_that_of_many():
+    for prefix, lens, padding in ((0, 40, 0), (70, 23, 2), (33, 7, 0)):
+        s = R.Setup(81, dtype=torch.bfloat16, dim=64, page=16, heads=6, kv_heads=2, new=[7], lens=[lens], prefix=prefix, padding=padding, leading=1)
+        out, lse, tol, ltol = R.attend_sequence(s)
+        want = R.attend(s)
+        for i, (t, _, _) in enumerate(s.rows()):
+            for j, (o, l, to, tl) in enumerate(want[t]):
+                assert torch.allclose(out[i, j], o, rtol=1e-12, atol=1e-12) and abs(float(lse[i, j]) - l) < 1e-12
+                assert torch.allclose(tol[i, j], to, rtol=1e-9) and abs(float(ltol[i, j]) - tl) < 1e-12

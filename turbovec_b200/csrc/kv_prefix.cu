@@ -195,7 +195,7 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) kv_prefix_kernel(const KvAt
         for (int s = 0; s < G::kSlots; ++s) { mbar_init(&sh.full[s], 1); mbar_init(&sh.empty[s], plan.paired ? 2 : 1); }
         for (int s = 0; s < 2; ++s) {
             mbar_init(&sh.o_done[s], 1);
-            mbar_init(&sh.q_full[s], 1); mbar_init(&sh.q_free[s], 8);
+            mbar_init(&sh.q_full[s], 1); mbar_init(&sh.q_free[s], 10);
             for (int b = 0; b < 2; ++b) { mbar_init(&sh.s_full[s][b], 1); mbar_init(&sh.p_ready[s][b], 4); }
         }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -314,8 +314,12 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) kv_prefix_kernel(const KvAt
                 wait(&sh.full[slot], (n / G::kSlots) & 1);
                 return slot;
             };
+            // Q of the part, also where this stream has no tile of it: a wait tells a phase from the one before it only, so nobody may be
+            // more than one behind, and Q is not loaded anew before both streams have seen it
+            wait(&sh.q_full[qs], parts & 1);
+            if (lane == 0) { mbar_arrive(&sh.q_free[0]); mbar_arrive(&sh.q_free[1]); }
+            __syncwarp();
             if (first < w.count) {
-                wait(&sh.q_full[qs], parts & 1);
                 const uint32_t slot = tile_of(place_k(first));
                 logits(0, slot);
                 logits(1, slot);
@@ -359,7 +363,7 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) kv_prefix_kernel(const KvAt
         // ---- weights: stream `s`, a row to a thread
         const int s = warp >> 2, r = (warp & 3) * 32 + lane;
         const uint32_t quarter = uint32_t((warp & 3) * 32) << 16, s_addr = tmem + 128 * s + quarter, o_addr = tmem + 256 + G::kOColumns * s + quarter;
-        uint32_t s_count = 0, o_count = 0;
+        uint32_t s_count = 0, o_count = 0, parts = 0;
         const int64_t live = int64_t(q_count) * p.group;
         const int64_t row_base = int64_t(plan.paired ? 2 * unit + s : unit) * plan.rows;
         auto wait = [&](uint64_t *bar, uint32_t parity) {
@@ -505,8 +509,13 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) kv_prefix_kernel(const KvAt
                     for (int row = max((warp & 3) * 32, plan.rows); row < (warp & 3) * 32 + 32; ++row)
                         if (lane < 8) *reinterpret_cast<uint4 *>(stage + (row - (warp & 3) * 32) * 128 + lane * 16) = make_uint4(0, 0, 0, 0);
                 fence_shared_async();
+            } else {
+                // no tile of this part (one tile of keys, and it is the other stream's): without this wait the stream could be a part ahead and
+                // give Q back twice, in the other one's place
+                wait(&sh.q_full[0], parts & 1);
             }
             o_count += done;
+            ++parts;
             if (have) p.pre_ml[block * kKvPrefixRows + r] = make_float2(m, l);
             // Q, S and O may be written anew
             fence_before();
