@@ -48,3 +48,58 @@ def test_parts_of_one_tile(case, prefix_kernel):  # noqa: F811
     for _ in range(3):
         out, lse = attend(s)
         assert torch.equal(out, first) and torch.equal(lse, first_lse)
+
+
+MANY_TILES = [
+    # dtype, dim, page, group, kv_heads, tokens, prefix: one tile of rows, many of keys
+    (BF, 128, 16, 3, 1, 40, 60_000),            # pages all over the pool
+    (FP, 64, 16, 7, 2, 18, 50_000),
+    (BF, 128, 128, 1, 149, 20, 1_500),          # more key heads than multiprocessors: runs of 12 tiles and more
+    (FP, 128, 64, 2, 150, 64, 700),
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("case", range(len(MANY_TILES)))
+def test_tiles_that_are_dealt_to_two_streams(case, prefix_kernel):  # noqa: F811
+    """Each stream waits for the tiles that it uses, whatever has become of the other one's."""
+    dtype, dim, page, group, kv_heads, tokens, prefix = MANY_TILES[case]
+    prefix_kernel(1)
+    s = R.Setup(320 + case, dtype=dtype, dim=dim, page=page, heads=group * kv_heads, kv_heads=kv_heads, new=[tokens], lens=[tokens], prefix=prefix)
+    first, first_lse = attend(s)
+    check(s, first, first_lse)
+    for _ in range(10):
+        out, lse = attend(s)
+        assert torch.equal(out, first) and torch.equal(lse, first_lse)
+
+
+PAIRED = [
+    # dtype, dim, page, group, kv_heads, tokens, prefix: two tiles of rows and more to a block
+    (BF, 128, 64, 3, 160, 60, 300),             # 126 rows to a tile: Q's rows that no copy writes are zeroed again after each part
+    (FP, 128, 16, 5, 151, 40, 640),
+    (BF, 64, 32, 7, 152, 30, 1_000),
+    (FP, 128, 64, 1, 150, 129, 260),            # one row in the second tile
+    (BF, 128, 128, 7, 75, 90, 700),             # five tiles of rows: three units, the last with one
+]
+
+
+def test_sizes_whose_blocks_have_several_parts():
+    for dtype, dim, page, group, kv_heads, tokens, prefix in MANY_TILES[2:]:
+        paired, units, parts = R.prefix_parts(tokens, group, kv_heads, prefix, MULTIPROCESSORS)
+        assert not paired and any(len(p) > 1 for p in parts)
+    for dtype, dim, page, group, kv_heads, tokens, prefix in PAIRED:
+        paired, units, parts = R.prefix_parts(tokens, group, kv_heads, prefix, MULTIPROCESSORS)
+        assert paired and any(len(p) > 1 for p in parts)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("case", range(len(PAIRED)))
+def test_parts_of_two_tiles_of_rows(case, prefix_kernel):  # noqa: F811
+    dtype, dim, page, group, kv_heads, tokens, prefix = PAIRED[case]
+    prefix_kernel(1)
+    s = R.Setup(340 + case, dtype=dtype, dim=dim, page=page, heads=group * kv_heads, kv_heads=kv_heads, new=[tokens], lens=[tokens], prefix=prefix, padding=2)
+    first, first_lse = attend(s)
+    check(s, first, first_lse)
+    for _ in range(3):
+        out, lse = attend(s)
+        assert torch.equal(out, first) and torch.equal(lse, first_lse)

@@ -49,7 +49,7 @@ struct PrefixGeometry {
 };
 template <int D>
 struct alignas(16) PrefixShared {
-    uint64_t full[PrefixGeometry<D>::kSlots], empty[PrefixGeometry<D>::kSlots];
+    uint64_t full[2][PrefixGeometry<D>::kSlots], empty[PrefixGeometry<D>::kSlots];     // [stream; 0 where both use a tile][slot]
     uint64_t s_full[2][2], p_ready[2][2], o_done[2], q_full[2], q_free[2];    // [stream][half of a tile], [stream]
     uint32_t tmem_base;
 };
@@ -192,7 +192,7 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) kv_prefix_kernel(const KvAt
     const KvPrefixPlan plan = p.plan;
     const int unit = blockIdx.x % plan.units, group = blockIdx.x / plan.units;
     if (tid == 0) {
-        for (int s = 0; s < G::kSlots; ++s) { mbar_init(&sh.full[s], 1); mbar_init(&sh.empty[s], plan.paired ? 2 : 1); }
+        for (int s = 0; s < G::kSlots; ++s) { mbar_init(&sh.full[0][s], 1); mbar_init(&sh.full[1][s], 1); mbar_init(&sh.empty[s], plan.paired ? 2 : 1); }
         for (int s = 0; s < 2; ++s) {
             mbar_init(&sh.o_done[s], 1);
             mbar_init(&sh.q_full[s], 1); mbar_init(&sh.q_free[s], 10);
@@ -231,10 +231,12 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) kv_prefix_kernel(const KvAt
     if (warp == kCopyWarp) {
         // ---- tiles in the order of their use: the keys `lookahead` tiles ahead of the values
         const int box = min(kKvPrefixTile, 1 << p.page_shift), boxes = kKvPrefixTile / box;
-        uint32_t n = 0;
+        uint32_t n = 0, armed = 0;                               // a bit per stream and slot: the phase that its next copy completes
         auto load = [&](const PrefixPart &part, int i, const CUtensorMap *map) {
             if (!ok) return;
-            const int s = n % G::kSlots;
+            // A wait tells a phase from the one before it only, so a barrier's phases are all waited for by those who wait for it: tiles of
+            // keys that are dealt to the streams complete barriers of the stream that uses them.
+            const int s = n % G::kSlots, owner = plan.paired ? 0 : i & 1;
             const int64_t key = int64_t(part.tile0 + i) * kKvPrefixTile + lane * box;
             const int64_t entry = key >> p.page_shift;
             int page = -1;
@@ -244,12 +246,14 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) kv_prefix_kernel(const KvAt
             if (n >= G::kSlots) ok = mbar_wait(&sh.empty[s], ((n / G::kSlots) - 1) & 1, p.timeouts);
             ok = __all_sync(kFullMask, ok);
             if (!ok) return;
-            if (lane == 0) mbar_arrive_expect_tx(&sh.full[s], G::kTileBytes);
+            uint64_t *bar = &sh.full[owner][s];
+            armed ^= 1u << (16 * owner + s);
+            if (lane == 0) mbar_arrive_expect_tx(bar, G::kTileBytes);
             __syncwarp();
             if (lane < boxes)
 #pragma unroll
                 for (int c = 0; c < D / 64; ++c)
-                    tma_load_page(ring + s * G::kTileBytes + c * G::kHalfBytes + lane * box * 128, map, c * 64, int(key & ((1 << p.page_shift) - 1)), part.h, page, &sh.full[s]);
+                    tma_load_page(ring + s * G::kTileBytes + c * G::kHalfBytes + lane * box * 128, map, c * 64, int(key & ((1 << p.page_shift) - 1)), part.h, page, bar);
             ++n;
         };
         uint32_t parts = 0;
@@ -276,14 +280,17 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) kv_prefix_kernel(const KvAt
         }
         if (!ok)                                                 // the copies in flight land before the block ends
         {
-            for (uint32_t i = n > G::kSlots ? n - G::kSlots : 0; i < n; ++i) mbar_wait(&sh.full[i % G::kSlots], (i / G::kSlots) & 1, p.timeouts);
+            for (int i = 0; i < 2 * G::kSlots; ++i) {
+                const int owner = i & 1, slot = i >> 1;
+                mbar_wait(&sh.full[owner][slot], ((armed >> (16 * owner + slot)) & 1) ^ 1, p.timeouts);
+            }
             for (int s = 0; s < (plan.paired ? 2 : 1) && parts > 0; ++s) mbar_wait(&sh.q_full[s], (parts - 1) & 1, p.timeouts);
         }
     } else if (warp < kMmaWarp + 2) {
         // ---- MMAs of stream s.  One warp for both would be what bounds the kernel: waiting for a barrier that has completed takes it some 200
         // cycles, six times a tile, and an MMA 30 to issue (3,000 cycles a step with weights that cost nothing; 2,048 are the MMAs').
-        const int s = warp - kMmaWarp, first = plan.paired ? 0 : s, stride = plan.paired ? 1 : 2, qs = plan.paired ? s : 0;
-        uint32_t parts = 0, p_count = 0, base = 0;               // tiles of the ring before this part
+        const int s = warp - kMmaWarp, first = plan.paired ? 0 : s, stride = plan.paired ? 1 : 2, qs = plan.paired ? s : 0;    // `first`: its full barriers, too
+        uint32_t parts = 0, p_count = 0, base = 0, seen = 0;     // tiles of the ring before this part; a bit per slot: the phase to wait for
         constexpr uint32_t kIdS = idesc<T>(kHalfKeys, false), kIdO = idesc<T>(D, true);
         auto wait = [&](uint64_t *bar, uint32_t parity) {
             if (ok) ok = mbar_wait(bar, parity, p.timeouts);
@@ -311,7 +318,8 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) kv_prefix_kernel(const KvAt
             };
             auto tile_of = [&](uint32_t n) {                     // waits for place n of the ring
                 const uint32_t slot = n % G::kSlots;
-                wait(&sh.full[slot], (n / G::kSlots) & 1);
+                wait(&sh.full[first][slot], (seen >> slot) & 1);
+                seen ^= 1u << slot;
                 return slot;
             };
             // Q of the part, also where this stream has no tile of it: a wait tells a phase from the one before it only, so nobody may be
