@@ -10,8 +10,8 @@ BF, FP = torch.bfloat16, torch.float16
 MULTIPROCESSORS = 148
 
 
-def check(s, out, lse, weight_step=None):
-    want, want_lse, tol, ltol = R.attend_sequence(s, weight_step=weight_step)
+def check(s, out, lse, **steps):
+    want, want_lse, tol, ltol = R.attend_sequence(s, **steps)
     at = [t for t, _, _ in s.rows()]
     bad = (out.cpu().double()[at] - want).abs() - tol
     assert (bad <= 0).all(), (int((bad > 0).sum()), float(bad.max()))

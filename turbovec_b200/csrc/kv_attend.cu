@@ -3,7 +3,7 @@
 // An item is up to 16 query rows of one key head (the heads that share it, times the tokens of one sequence; for a prefix the
 // rows of all sequences) and the keys they read, in tiles of 64.  All items' tiles are laid end to end and every block takes an equal
 // run of them, so that batches of any lengths fill the device evenly: lengths are known on the device alone.  A run that begins or
-// ends inside an item leaves partial results, (largest logit, sum of weights, weighted sum of values), in slot
+// ends inside an item leaves partial results, (base of the weights, their sum, weighted sum of values), in slot
 // item + block, a number that is different for every pair of the two that meet; a second kernel joins them.
 //
 // Bound by memory: a tile of 128 channels is 32 KB and 4 * 64 * 128 * 16 multiply-adds, most of them padding where rows are few.  One warp
@@ -21,7 +21,6 @@ namespace {
 
 constexpr int kConsumers = 4;
 constexpr int kAttendThreads = (kConsumers + 1) * 32;
-constexpr float kRescaleAt = 8.0f;
 constexpr int kLeastTiles = 2;                           // tiles of a run: joining more parts takes longer than these
 constexpr int kNothing = INT_MAX - kKvTile;              // first position of a group of keys that nobody sees
 
@@ -408,10 +407,11 @@ __global__ void __launch_bounds__(kAttendThreads, 2) kv_attend_kernel(const KvAt
             float t0 = fmaxf(fmaxf(sc[0][0], sc[0][1]), fmaxf(sc[1][0], sc[1][1])), t1 = fmaxf(fmaxf(sc[0][2], sc[0][3]), fmaxf(sc[1][2], sc[1][3]));
             t0 = fmaxf(t0, __shfl_xor_sync(kFullMask, t0, 1)); t1 = fmaxf(t1, __shfl_xor_sync(kFullMask, t1, 1));
             t0 = fmaxf(t0, __shfl_xor_sync(kFullMask, t0, 2)); t1 = fmaxf(t1, __shfl_xor_sync(kFullMask, t1, 2));
-            // a maximum that grows by less than 2^8 stays: weights are below 2^8 then, which neither type nor the sums mind
-            if (__any_sync(kFullMask, t0 > m0 + kRescaleAt || t1 > m1 + kRescaleAt)) {
+            // a base (KvType) that logits are not far above stays
+            constexpr float kLift = KvType<T>::kLift, kUpTo = kLift + KvType<T>::kRescaleAt;
+            if (__any_sync(kFullMask, t0 > m0 + kUpTo || t1 > m1 + kUpTo)) {
                 // (for the rows that need it: what the others give must not depend on their neighbours)
-                const float n0 = t0 > m0 + kRescaleAt ? t0 : m0, n1 = t1 > m1 + kRescaleAt ? t1 : m1;
+                const float n0 = t0 > m0 + kUpTo ? t0 - kLift : m0, n1 = t1 > m1 + kUpTo ? t1 - kLift : m1;
                 const float a0 = n0 == m0 ? 1.0f : kv_exp2(m0 - n0), a1 = n1 == m1 ? 1.0f : kv_exp2(m1 - n1);
                 m0 = n0; m1 = n1;
                 l0 *= a0; l1 *= a1;
@@ -597,7 +597,7 @@ __global__ void __launch_bounds__(128) kv_join_kernel(const KvAttendParams p) {
     if (token < all.first || token >= all.first + all.count) return;       // behind the last sequence: as it was
     const KvPieces own = p.own_pieces[row];
     if (own.count == 0 && p.prefix_len == 0) return;
-    // Two lists of parts, n1 of a prefix and n2 of the row's own keys: sums o at step floats, (largest logit, sum of weights) at step / D.
+    // Two lists of parts, n1 of a prefix and n2 of the row's own keys: sums o at step floats, (base, sum of weights) at step / D.
     const float *o1 = nullptr, *o2 = nullptr;
     const float2 *ml1 = nullptr, *ml2 = nullptr;
     int64_t step1 = 0;

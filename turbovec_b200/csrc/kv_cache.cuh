@@ -51,8 +51,13 @@ __host__ __device__ inline int kv_visible(int64_t pos, int64_t capacity) {
     return n < 0 ? 0 : (n > INT_MAX - 2 * kKvTile ? INT_MAX - 2 * kKvTile : int(n));
 }
 
+// Weights of a softmax are 2^(logit - base) in the type, with a running base that is set to kLift below the largest logit and stays until a
+// logit is more than kLift + kRescaleAt above it.  bfloat16 has float's range: 2^8 is no matter to it.  float16 ends at 2^-24, with few bits below 2^-14:
+// under a base that is the largest logit itself, keys of less than 2^-25 of its weight would count for nothing, however many there are
+// of them (as beside a first key that takes most of the weight); times 2^11, and up to 2^15, they have all their bits down to 2^-25 of the largest.
 template <typename T> struct KvType;
 template <> struct KvType<__nv_bfloat16> {
+    static constexpr float kLift = 0.0f, kRescaleAt = 8.0f;
     static __device__ __forceinline__ float2 unpack(uint32_t x) { return {__uint_as_float(x << 16), __uint_as_float(x & 0xffff0000u)}; }
     static __device__ __forceinline__ uint32_t pack(float lo, float hi) {
         uint32_t d;
@@ -63,6 +68,7 @@ template <> struct KvType<__nv_bfloat16> {
     static constexpr CUtensorMapDataType kMapType = CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
 };
 template <> struct KvType<__half> {
+    static constexpr float kLift = 11.0f, kRescaleAt = 4.0f;
     static __device__ __forceinline__ float2 unpack(uint32_t x) { return __half22float2(*reinterpret_cast<const __half2 *>(&x)); }
     static __device__ __forceinline__ uint32_t pack(float lo, float hi) {
         uint32_t d;
@@ -226,7 +232,7 @@ struct KvAttendParams {
     const int32_t *token_pos;
     int budget;
     int item_cost;                           // what an item costs beside its tiles, in tiles
-    // partial results: unnormalised sums, and (largest logit, sum of weights) in powers of two
+    // partial results: unnormalised sums, and (base, sum of weights) in powers of two
     float *part_o;                           // [slot][kKvRows][head_dim]
     float2 *part_ml;                         // [slot][kKvRows]
     KvPieces *own_pieces, *prefix_pieces;    // [token][head]

@@ -2,8 +2,8 @@
 //
 // All rows of a batch (tokens x heads of a key head) see all keys of the prefix, so the prefix is read once for 256 rows instead of
 // once for every sequence.  S = Q K^T and O += P V are MMAs of 128 rows; four warps turn S into P, a row to a thread: running
-// maximum, weights in powers of two, their sum.  O is rescaled only when a row's maximum grows by more than 2^8 (weights then
-// stay below 2^8, which neither type nor the sums mind).  P replaces S in tensor memory and is the A operand of the second MMA.
+// base, weights in powers of two, their sum.  O is rescaled only when a row's logits go well above the base (KvType in kv_cache.cuh).  P
+// replaces S in tensor memory and is the A operand of the second MMA.
 //
 // Weights are rounded to the type once, half a step each, while their sum keeps what is rounded off: with the result's own rounding
 // the relative error is 1.35 times that of the latter alone.  Carrying the rest of each weight along, as kv_attend.cu does, would be half
@@ -36,7 +36,6 @@ constexpr int kWeightRegs = 184, kOtherRegs = 136;   // registers a thread: 256 
 static_assert(256 * kWeightRegs + 128 * kOtherRegs <= kPrefixThreads * 168, "more registers than the block has");
 constexpr int kMmaWarp = 8, kCopyWarp = 10;      // MMAs of stream s: warp kMmaWarp + s
 constexpr int kHalfKeys = kKvPrefixTile / 2;
-constexpr float kRescaleAt = 8.0f;
 constexpr int kByPolynomial = 2;                 // pairs of weights of every eight
 
 template <int D>
@@ -410,7 +409,7 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) kv_prefix_kernel(const KvAt
                     for (int c = 0; c < kHalfKeys; ++c)
                         if (c >= left || !((good >> (c >> 4)) & 1u)) x[c] = 0xff800000u;
                 }
-                // the weights of columns c0 .. c0 + 31, under the maximum m, and their sum
+                // the weights of columns c0 .. c0 + 31, over the base m, and their sum
                 const uint64_t scale2 = pair(p.scale_log2, p.scale_log2);
                 auto weights = [&](int c0, uint32_t (&pk)[16], uint64_t (&part)[2]) {
                     const float base = m == -INFINITY ? 0.0f : -m;
@@ -440,19 +439,20 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) kv_prefix_kernel(const KvAt
                     const float top = max3_nan(max3_nan(t8[0], t8[2], t8[4]), t8[6], t8[6]) * p.scale_log2;
                     return top < INFINITY ? top : NAN;           // an infinite logit makes the row NaN, as inf - inf does
                 };
-                // The weights are computed under the maximum so far, before it is known whether that still holds: it mostly does, and then
-                // looking for it costs no time of its own.
-                if (done == 0) m = largest();
+                // The weights are computed over the base so far, before it is known whether that still holds: it mostly does, and then
+                // looking for the largest logit costs no time of its own.
+                constexpr float kLift = KvType<T>::kLift, kUpTo = kLift + KvType<T>::kRescaleAt;
+                if (done == 0) m = largest() - kLift;
                 uint32_t pk[2][16];
                 uint64_t part[2] = {0, 0};
                 weights(0, pk[0], part);
                 weights(32, pk[1], part);
                 if (done > 0) {
                     const float top = largest();
-                    if (__any_sync(kFullMask, !(top <= m + kRescaleAt))) {
+                    if (__any_sync(kFullMask, !(top <= m + kUpTo))) {
                         // For the rows that need it: what the others give must not depend on their neighbours.  (A NaN becomes the maximum: the
                         // polynomial would lose it.)
-                        const float next = top <= m + kRescaleAt ? m : max3_nan(m, top, top), f = next == m ? 1.0f : kv_exp2(m - next);
+                        const float next = top <= m + kUpTo ? m : max3_nan(m, top - kLift, top - kLift), f = next == m ? 1.0f : kv_exp2(m - next);
                         m = next;
                         l *= f;
                         wait(&sh.o_done[s], (o_count + done - 1) & 1);      // (the half before that had ended when these logits were there)
