@@ -418,7 +418,10 @@ int tv_kv_append(const tv_kv_cache *cache, const tv_kv_batch *batch, int64_t tok
 /* out = softmax(scale * q k) v over the first prefix_len keys of the pages prefix_pages (prefix_width of them; none: 0) and the
  * keys of the row's own sequence at positions up to p.  lse (may be null): natural logarithm of the sum of exponentials,
  * [token][head].  A row that sees no key gives zeros and -infinity.  What a row does not see never reaches it, NaN and infinities
- * included; an infinite value that it sees gives an infinity or NaN.  out must not overlap q.  The workspace needs
+ * included; an infinite value that it sees gives an infinity or NaN.  Sums and logits are held in 32 bits and the result is rounded
+ * once, but for a prefix that the tensor-memory kernel reads (many rows on a long prefix: TV_KV_OPT_TENSOR_PREFIX has the rule, and 0 turns it
+ * off): its weights are rounded to the type before they meet the values, and the error of a result is 1.4 times that of rounding it once.
+ * out must not overlap q.  The workspace needs
  * tv_kv_attend_workspace bytes (256-byte aligned; 0 with a message in tv_last_error(NULL): the sizes are refused), belongs to the
  * call until its work is done, and need not be cleared. */
 size_t tv_kv_attend_workspace(const tv_kv_cache *cache, const tv_kv_batch *batch, int64_t tokens, int heads, int64_t prefix_len);
@@ -435,10 +438,11 @@ size_t tv_kv_attend_selected_workspace(const tv_kv_cache *cache, const tv_kv_bat
 int tv_kv_attend_selected(const tv_kv_cache *cache, const tv_kv_batch *batch, int64_t tokens, int heads, const tv_kv_rows *q,
                           int64_t budget, int64_t first, int64_t recent, float scale, const tv_kv_rows *out, float *lse,
                           int32_t *pages_out, void *workspace, size_t workspace_bytes, void *stream);
-/* Options of these calls, for the whole process; results stay within the same rounding.  Workspace sizes follow them: ask anew. */
+/* Options of these calls, for the whole process.  Workspace sizes follow them: set them before calls begin, for a call whose workspace was
+ * asked for under another option may be refused as having too small a one. */
 enum {
     TV_KV_OPT_TENSOR_PREFIX = 1     /* -1 (default): a prefix is read by the tensor-memory kernel where that was measured to be faster
-                                     * (keys * key heads * (rows - 29) > 2.6 million); 0: never; 1: always (testing) */
+                                     * (keys * key heads * (rows - 29) > 2.6 million); 0: never (one rounding: tv_kv_attend); 1: always (testing) */
 };
 int tv_kv_set_option(int option, int64_t value);
 /* Waits for the device and tells whether a kernel of these calls gave up a wait since the last time it was asked (its results are

@@ -164,10 +164,10 @@ def rotate(x, cos, sin, interleaved):
     return y, y.abs() * torch.finfo(x.dtype).eps / 2 + mag * 2 * 2.0 ** -24 * (1 + torch.finfo(x.dtype).eps) + 2.0 ** -25
 
 
-def attend_sequence(s, scale=None, weight_step=None, least=0.0):
+def attend_sequence(s, scale=None, weight_step=None, least=0.0, terms=None):
     """attend() for a setup of one sequence, all rows of a head at once: (out [new, heads, dim], lse [new, heads], their tolerances) of the
     sequence's rows in order.  weight_step: half a step of what the weights are rounded to (None: the type's); least:
-    half of the smallest step that a weight has, relative to the row's largest."""
+    half of the smallest step that a weight has, relative to the row's largest; terms: channels of the queries that are not zero (None: all)."""
     assert len(s.lens) == 1
     scale = s.dim ** -0.5 if scale is None else scale
     pre, own = s.prefix_keys(), s.own_keys(0, s.lens[0] - 1)
@@ -190,8 +190,8 @@ def attend_sequence(s, scale=None, weight_step=None, least=0.0):
             w = torch.exp(logits - lse[:, j, None])
             out[:, j] = w @ v
             # the tolerances of attention() above
-            delta = (q.abs() @ k.abs().T).masked_fill(hidden, 0.0).amax(-1) * scale * (s.dim + 4) * 2.0 ** -23 + 2.0 ** -18
-            tol[:, j] = out[:, j].abs() * half + (w @ v.abs()) * (step + 2 * delta)[:, None] * (1 + half) + torch.finfo(s.dtype).tiny
+            delta = (q.abs() @ k.abs().T).masked_fill(hidden, 0.0).amax(-1) * scale * ((s.dim if terms is None else terms) + 4) * 2.0 ** -23 + 2.0 ** -18
+            tol[:, j] = out[:, j].abs() * half + (w @ v.abs()) * (step + 2 * delta)[:, None] * (1 + half) + torch.finfo(s.dtype).tiny * half
             tol[:, j] += least * w.amax(-1, keepdim=True) * ((~hidden).double() @ v.abs())
             ltol[:, j] = delta + lse[:, j].abs() * 2.0 ** -22
     return out, lse, tol, ltol

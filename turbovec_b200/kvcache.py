@@ -60,7 +60,7 @@ def _last_adjacent(name: str, t: torch.Tensor) -> None:
 
 
 def set_option(option: int, value: int) -> None:
-    """An option of the cache's calls, for the whole process (TV_KV_OPT_* of include/turbovec_b200.h)."""
+    """An option of the cache's calls, for the whole process (TV_KV_OPT_* of include/turbovec_b200.h).  Not while another thread is in a call."""
     global _options
     lib = _native.load()
     rc = lib.tv_kv_set_option(int(option), int(value))
@@ -259,7 +259,8 @@ class PagedKVCache:
         """Attention of the rows of q [tokens, heads, head_dim] over the first prefix_len keys of prefix_pages (int32 [n], read once for the
         whole batch) and the keys of their own sequence up to their position.  Returns out (a new tensor by default); lse, where given,
         receives the logarithm of each row's sum of exponentials.  scale: head_dim ** -0.5 by default.  Rows that see no key: zeros
-        and -inf."""
+        and -inf.  Many rows on a long prefix go to a kernel that rounds the weights to the type (1.4 times the error of one rounding of the
+        result); set_option(OPT_TENSOR_PREFIX, 0) keeps to the other one."""
         b = self._batch(batch)
         tokens, heads, qr = self._query(q)
         if out is None:
