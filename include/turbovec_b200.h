@@ -410,8 +410,8 @@ typedef struct tv_kv_rows {                         /* [row][head][channel]: str
  * and sin are [positions][rotary / 2] floats (16-byte aligned); rotary is a multiple of 16 up to head_dim, 0 = no rotation.
  * interleaved = 0 pairs channels i and i + rotary / 2, 1 pairs 2i and 2i + 1.  y1 = x1 cos - x2 sin, y2 = x2 cos + x1 sin in
  * 32 bits.  A token whose angle is outside the tables, or whose position is below 0, is neither stored nor rotated.  Brings bounds
- * and scales of the pages up to date: a page whose first token is appended starts anew, others are widened, also when
- * tokens are overwritten. */
+ * and scales of the pages that tokens are stored in up to date: a page whose first token is appended starts anew, others are widened, also
+ * when tokens are overwritten. */
 int tv_kv_append(const tv_kv_cache *cache, const tv_kv_batch *batch, int64_t tokens, int heads, const tv_kv_rows *k_new,
                  const tv_kv_rows *v_new, const tv_kv_rows *q, const tv_kv_rows *q_out, const float *cos, const float *sin,
                  int64_t positions, int rotary, int interleaved, int64_t position_offset, void *stream);

@@ -162,6 +162,13 @@ __global__ void __launch_bounds__(kAppendThreads, 3) kv_append_kernel(const KvAp
         }
     }
     if (p.bounds == nullptr || !stored) return;
+    // places of the page that the tokens with an angle took: without any, the page and its bounds are as they were
+    int64_t first_place = at0, last_place = at0 + count - 1;
+    if (p.rotary > 0) {
+        first_place = max(first_place, -p.position_offset - page_from);
+        last_place = min(last_place, p.positions - 1 - p.position_offset - page_from);
+    }
+    if (first_place > last_place) return;
 
     // lowest and highest new key of every channel: over the rows of a warp, then over the head's warps
 #pragma unroll
@@ -201,7 +208,7 @@ __global__ void __launch_bounds__(kAppendThreads, 3) kv_append_kernel(const KvAp
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(kFullMask, top, o));
     const int64_t at = page * p.kv_heads + mine;
-    const bool widen = at0 > 0;                             // the page holds earlier keys
+    const bool widen = first_place > 0;                     // the page holds earlier keys
     const float old_scale = widen ? p.scales[at] : 0.0f;
     const float scale = fmaxf(kv_pow2(kv_exponent(top)), old_scale), ratio = old_scale / scale;
     int8_t *row = p.bounds + at * 2 * D;
