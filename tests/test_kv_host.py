@@ -156,3 +156,20 @@ def test_the_restatement_of_one_sequence_is_that_of_many():
             for j, (o, l, to, tl) in enumerate(want[t]):
                 assert torch.allclose(out[i, j], o, rtol=1e-12, atol=1e-12) and abs(float(lse[i, j]) - l) < 1e-12
                 assert torch.allclose(tol[i, j], to, rtol=1e-9) and abs(float(ltol[i, j]) - tl) < 1e-12
+
+
+def test_addresses_that_no_kernel_could_read_are_refused(lib):
+    """32-bit numbers at an odd address would be an error on the device."""
+    buf, at, cache, batch, rows = views()
+    for op in ("append", "attend", "selected"):
+        for change in (dict(table=at + 2), dict(lens=at + 1), dict(offsets=at + 3)):
+            assert call(lib, op, **change) == 90, (op, change)
+            assert b"4-byte aligned" in lib.tv_last_error(None)
+    out = type(rows)(at + 16384, 512, 128)
+    assert call(lib, "attend", prefix_pages=at + 2) == 90 and b"4-byte aligned" in lib.tv_last_error(None)
+    assert call(lib, "selected", pages_out=at + 1) == 90 and b"4-byte aligned" in lib.tv_last_error(None)
+    for lse in (at + 1, at + 2):
+        assert lib.tv_kv_attend(cache, batch, 1, 4, rows, at, 2, 20, 0.1, out, lse, at, 1 << 40, None) == 90
+        assert b"4-byte aligned" in lib.tv_last_error(None)
+        assert lib.tv_kv_attend_selected(cache, batch, 1, 4, rows, 2, 1, 1, 0.1, out, lse, at, at, 1 << 40, None) == 90
+        assert b"4-byte aligned" in lib.tv_last_error(None)

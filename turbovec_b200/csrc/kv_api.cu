@@ -70,6 +70,7 @@ int check_common(const tv_kv_cache *c, const tv_kv_batch *b, int64_t tokens, int
     if (b->sequences < 0 || b->sequences > kMaxCount || b->table_width < 0 || b->table_width > kMaxCount || b->table_stride < b->table_width)
         return refuse("sequences and table_width must be at most 2^30, and table_stride at least table_width");
     if (b->sequences > 0 && (!b->lens || !b->offsets || (b->table_width > 0 && !b->table))) return refuse("table, lens and offsets must be given");
+    if (!aligned(b->table, 4) || !aligned(b->lens, 4) || !aligned(b->offsets, 4)) return refuse("table, lens and offsets must be 4-byte aligned");
     if (tokens < 0 || tokens > kMaxCount) return refuse("tokens must be between 0 and 2^30");
     if (heads < c->kv_heads || heads % c->kv_heads != 0 || heads > 65535) return refuse("heads must be a positive multiple of kv_heads, at most 65535");
     if (int64_t(tokens) * heads > (int64_t(1) << 31)) return unsupported("tokens * heads must be at most 2^31");
@@ -176,6 +177,7 @@ int fill_attend(KvAttendParams &p, const tv_kv_cache *c, const tv_kv_batch *b, i
     if (rc == TV_OK) rc = check_rows(out, "out must be given, 16-byte aligned, with strides that are positive multiples of 8 elements");
     if (rc != TV_OK) return rc;
     if (overlap(q->data, extent(q, tokens, heads, c->head_dim), out->data, extent(out, tokens, heads, c->head_dim))) return refuse("out must not overlap q");
+    if (!aligned(lse, 4)) return refuse("lse must be 4-byte aligned");
     if (!(scale > 0.0f) || !std::isfinite(scale)) return refuse("scale must be positive and finite");
     p.batch = batch_of(b);
     p.q = rows_of(q);
@@ -257,6 +259,7 @@ int tv_kv_attend(const tv_kv_cache *c, const tv_kv_batch *b, int64_t tokens, int
     if (prefix_len < 0 || prefix_width < 0 || prefix_width > kMaxCount || prefix_len > prefix_width * c->page_size || prefix_len > kMaxCount)
         return refuse("prefix_len must be between 0 and prefix_width pages of tokens, at most 2^30");
     if (prefix_len > 0 && !prefix_pages) return refuse("prefix_pages must be given with prefix_len");
+    if (!aligned(prefix_pages, 4)) return refuse("prefix_pages must be 4-byte aligned");
     if (tokens == 0 || b->sequences == 0) return TV_OK;
     KvAttendParams p{};
     rc = fill_attend(p, c, b, tokens, heads, q, out, lse, scale);
@@ -306,7 +309,7 @@ int tv_kv_attend_selected(const tv_kv_cache *c, const tv_kv_batch *b, int64_t to
         return refuse("budget must be between 1 and 32,768, and first + recent at most budget");
     if (b->table_width > kKvMaxScored) return unsupported("table_width must be at most 32,768 pages");
     if (tokens == 0 || b->sequences == 0) return TV_OK;
-    if (!pages_out) return refuse("pages_out must be given");
+    if (!pages_out || !aligned(pages_out, 4)) return refuse("pages_out must be given and 4-byte aligned");
     KvAttendParams p{};
     KvSelectParams s{};
     rc = fill_attend(p, c, b, tokens, heads, q, out, lse, scale);
