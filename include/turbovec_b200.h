@@ -406,12 +406,12 @@ typedef struct tv_kv_rows {                         /* [row][head][channel]: str
     int64_t token_stride, head_stride;
 } tv_kv_rows;
 /* Appends `tokens` keys and values (kv_heads heads each) to the pages of their sequences and rotates keys and, where q is given
- * (heads heads, a multiple of kv_heads), queries into q_out (which may be q) by the angles of position p + position_offset: cos
- * and sin are [positions][rotary / 2] floats (16-byte aligned); rotary is a multiple of 16 up to head_dim, 0 = no rotation.
- * interleaved = 0 pairs channels i and i + rotary / 2, 1 pairs 2i and 2i + 1.  y1 = x1 cos - x2 sin, y2 = x2 cos + x1 sin in
- * 32 bits.  A token whose angle is outside the tables, or whose position is below 0, is neither stored nor rotated.  Brings bounds
- * and scales of the pages that tokens are stored in up to date: a page whose first token is appended starts anew, others are widened, also
- * when tokens are overwritten. */
+ * (heads heads, a multiple of kv_heads), queries into q_out by the angles of position p + position_offset: cos and sin are
+ * [positions][rotary / 2] floats (16-byte aligned); rotary is a multiple of 16 up to head_dim, 0 = no rotation.  interleaved = 0 pairs
+ * channels i and i + rotary / 2, 1 pairs 2i and 2i + 1.  y1 = x1 cos - x2 sin, y2 = x2 cos + x1 sin in 32 bits.  q_out may be q;
+ * otherwise it must not overlap q, k_new or v_new.  None of them may lie in pages that the call writes.  A token whose angle
+ * is outside the tables, or whose position is below 0, is neither stored nor rotated.  Brings bounds and scales of the pages that tokens
+ * are stored in up to date: a page whose first token is appended starts anew, others are widened, also when tokens are overwritten. */
 int tv_kv_append(const tv_kv_cache *cache, const tv_kv_batch *batch, int64_t tokens, int heads, const tv_kv_rows *k_new,
                  const tv_kv_rows *v_new, const tv_kv_rows *q, const tv_kv_rows *q_out, const float *cos, const float *sin,
                  int64_t positions, int rotary, int interleaved, int64_t position_offset, void *stream);
@@ -421,7 +421,7 @@ int tv_kv_append(const tv_kv_cache *cache, const tv_kv_batch *batch, int64_t tok
  * included; an infinite value that it sees gives an infinity or NaN.  Sums and logits are held in 32 bits and the result is rounded
  * once, but for a prefix that the tensor-memory kernel reads (many rows on a long prefix: TV_KV_OPT_TENSOR_PREFIX has the rule, and 0 turns it
  * off): its weights are rounded to the type before they meet the values, and the error of a result is 1.4 times that of rounding it once.
- * out must not overlap q.  The workspace needs
+ * q, out, lse and, below, pages_out must not overlap one another.  The workspace needs
  * tv_kv_attend_workspace bytes (256-byte aligned; 0 with a message in tv_last_error(NULL): the sizes are refused), belongs to the
  * call until its work is done, and need not be cleared. */
 size_t tv_kv_attend_workspace(const tv_kv_cache *cache, const tv_kv_batch *batch, int64_t tokens, int heads, int64_t prefix_len);

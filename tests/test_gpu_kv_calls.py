@@ -1,0 +1,56 @@
+"""Calls of the paged key/value cache that its documents allow or forbid and that nothing else makes."""
+import pytest
+import torch
+
+from tests import kv_reference as R
+from tests.test_gpu_kv import check_rows, handles
+
+pytestmark = pytest.mark.gpu
+
+BF, FP = torch.bfloat16, torch.float16
+
+
+def fused(s):
+    """q, k and v as heads of one projection's output, with room for results behind them."""
+    buf = torch.full((s.tokens, 2 * s.heads + 2 * s.kv_heads, s.dim), 3.0, dtype=s.dtype, device="cuda")
+    q, k, v, out = buf.split([s.heads, s.kv_heads, s.kv_heads, s.heads], 1)
+    q.copy_(s.q), k.copy_(s.k_new), v.copy_(s.v_new)
+    return buf, q, k, v, out
+
+
+def test_results_beside_their_inputs_in_one_buffer():
+    s = R.Setup(600, dtype=BF, dim=64, page=16, heads=6, kv_heads=2, new=[2, 1, 3], lens=[2, 100, 64], prefix=90)
+    cache, batch = handles(s)
+    buf, q, k, v, out = fused(s)
+    before = buf.clone()
+    cache.attend(batch, q, prefix_pages=s.prefix_pages.cuda(), prefix_len=s.prefix, out=out)
+    check_rows(s, out, None, R.attend(s))
+    _, pages = cache.attend_selected(batch, q, budget=2, out=out)
+    want, picks = R.attend_selected(s, 2, 1, 1)
+    check_rows(s, out, None, want)
+    assert torch.equal(buf[:, :-s.heads], before[:, :-s.heads])
+    angle = torch.rand(200, 32) * 6.28
+    cos, sin = torch.cos(angle).cuda(), torch.sin(angle).cuda()
+    cache.append(batch, k, v, q=q, q_out=out, cos=cos, sin=sin)
+    assert torch.equal(buf[:, :-s.heads], before[:, :-s.heads])
+    apart = out.clone()
+    cache.append(batch, k, v, q=q, q_out=q, cos=cos, sin=sin)       # in place, between the keys and values it reads
+    assert torch.equal(q, apart) and torch.equal(buf[:, s.heads:-s.heads], before[:, s.heads:-s.heads])
+
+
+def test_results_over_one_another_are_refused():
+    s = R.Setup(601, dtype=BF, dim=64, page=16, heads=4, kv_heads=4, new=[1, 1], lens=[5, 40])
+    cache, batch = handles(s)
+    q, k, v = s.q.cuda(), s.k_new.cuda(), s.v_new.cuda()
+    out, lse = torch.zeros_like(q), torch.zeros(2, 4, device="cuda")
+
+    def numbers(t, n):
+        return t.view(-1).view(torch.int32)[:n]
+    for call in (lambda: cache.append(batch, k, v, q=q, q_out=k), lambda: cache.append(batch, k, v, q=q, q_out=v),
+                 lambda: cache.attend(batch, q, out=out, lse=numbers(q, 8).view(torch.float32).view(2, 4)),
+                 lambda: cache.attend(batch, q, out=out, lse=numbers(out, 8).view(torch.float32).view(2, 4)),
+                 lambda: cache.attend_selected(batch, q, budget=2, out=out, pages=numbers(q, 16).view(2, 4, 2)),
+                 lambda: cache.attend_selected(batch, q, budget=2, out=out, pages=numbers(out, 16).view(2, 4, 2)),
+                 lambda: cache.attend_selected(batch, q, budget=1, recent=0, out=out, lse=lse, pages=lse.view(torch.int32).view(2, 4, 1))):
+        with pytest.raises(ValueError, match="overlap"):
+            call()

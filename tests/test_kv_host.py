@@ -173,3 +173,76 @@ def test_addresses_that_no_kernel_could_read_are_refused(lib):
         assert b"4-byte aligned" in lib.tv_last_error(None)
         assert lib.tv_kv_attend_selected(cache, batch, 1, 4, rows, 2, 1, 1, 0.1, out, lse, at, at, 1 << 40, None) == 90
         assert b"4-byte aligned" in lib.tv_last_error(None)
+
+
+def chunks(at, tokens, heads, token_stride, head_stride, dim):
+    """16-byte pieces of a view (strides in elements of two bytes)."""
+    return {(at + 2 * (t * token_stride + h * head_stride)) // 16 + i for t in range(tokens) for h in range(heads) for i in range(dim // 8)}
+
+
+def refused_for_overlap(lib, rc):
+    assert rc != 0
+    return rc == 90 and b"overlap" in lib.tv_last_error(None)
+
+
+@pytest.mark.parametrize("seed", range(3))
+def test_views_of_one_buffer_that_interleave_are_told_from_those_that_overlap(lib, seed):
+    """q and out, or k and the rotated queries, as heads of one buffer, in rows of tokens or of heads: refused where they share a byte."""
+    import random
+    rng = random.Random(seed)
+    dim, seen = 64, {True: 0, False: 0}
+    buf, at, cache, batch, row = views(device=63, head_dim=dim, k_head_stride=1024, k_token_stride=64, v_head_stride=1024, v_token_stride=64)     # no machine has so many devices
+    Row = type(row)
+    for _ in range(600):
+        tokens, heads = rng.choice([1, 2, 3, 5]), 4
+        by_heads = rng.random() < 0.3
+        outer = 8 * rng.choice([32, 40, 64, 96, 97])
+
+        def view(n):
+            rows, runs = (n, tokens) if by_heads else (tokens, n)
+            inner = 8 * rng.choice([8, 8, 9, 12, 16])
+            if (runs - 1) * inner + dim > outer:
+                inner = 64
+            if (runs - 1) * inner + dim > outer:
+                return None
+            where = at + 16 * rng.choice([0, rng.randrange(0, 8 * tokens), rng.randrange(0, 200), 8 * rng.randrange(0, 30)])
+            ts, hs = (inner, outer) if by_heads else (outer, inner)
+            return Row(where, ts, hs), chunks(where, tokens, n, ts, hs, dim)
+        a, b, k = view(heads), view(heads), view(2)
+        if not a or not b or not k:
+            continue
+        rc = lib.tv_kv_attend(cache, batch, tokens, heads, a[0], at, 2, 20, 0.1, b[0], None, at, 1 << 40, None)
+        assert refused_for_overlap(lib, rc) == bool(a[1] & b[1])
+        seen[bool(a[1] & b[1])] += 1
+        same = (a[0].data, a[0].token_stride, a[0].head_stride)
+        for first, second in ((a, a), (a, b)):
+            rc = lib.tv_kv_append(cache, batch, tokens, heads, k[0], k[0], first[0], second[0], at, at, 8, 64, 0, 0, None)
+            apart = (second[0].data, second[0].token_stride, second[0].head_stride) == same or not first[1] & second[1]
+            assert refused_for_overlap(lib, rc) == (not apart or bool(k[1] & second[1]))
+    assert min(seen.values()) > 50
+
+
+@pytest.mark.parametrize("seed", range(2))
+def test_views_that_share_bytes_are_never_let_through(lib, seed):
+    """Any strides: what overlaps is refused, and what lies in ranges of its own is not."""
+    import random
+    rng = random.Random(10 + seed)
+    dim = 64
+    buf, at, cache, batch, row = views(device=63, head_dim=dim, k_head_stride=1024, k_token_stride=64, v_head_stride=1024, v_token_stride=64)
+    hit = 0
+    for _ in range(600):
+        tokens, heads = rng.choice([1, 2, 3, 7]), rng.choice([2, 4])
+        a, b = ((at + 16 * rng.randrange(0, 300), 8 * rng.randrange(1, 120), 8 * rng.randrange(1, 120)) for _ in range(2))
+        ca, cb = chunks(a[0], tokens, heads, *a[1:], dim), chunks(b[0], tokens, heads, *b[1:], dim)
+        rc = lib.tv_kv_attend(cache, batch, tokens, heads, type(row)(*a), at, 2, 20, 0.1, type(row)(*b), None, at, 1 << 40, None)
+        refused = refused_for_overlap(lib, rc)
+        hit += bool(ca & cb)
+        assert refused if ca & cb else not (refused and (max(ca) < min(cb) or max(cb) < min(ca)))
+    assert hit > 100
+    # sums are contiguous
+    q, out = type(row)(at, 512, 128), type(row)(at + 16384, 512, 128)
+    for lse in (at, at + 64, at + 16384 + 1020):
+        assert refused_for_overlap(lib, lib.tv_kv_attend(cache, batch, 2, 4, q, at, 2, 20, 0.1, out, lse, at, 1 << 40, None))
+    # strides that no memory has do not wrap
+    far = type(row)(at, (1 << 38) - 8, 128)
+    assert lib.tv_kv_attend(cache, batch, 1 << 29, 4, far, at, 2, 20, 0.1, type(row)(at + 4096, 512, 128), None, at, 1 << 40, None) == 90

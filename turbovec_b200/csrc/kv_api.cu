@@ -3,6 +3,7 @@
 #include <atomic>
 #include <cmath>
 #include <cstdio>
+#include <utility>
 
 #include "kv_cache.cuh"
 #include "search.cuh"
@@ -80,13 +81,52 @@ int check_rows(const tv_kv_rows *r, const char *message) {
     if (!r || !r->data || !aligned(r->data, 16) || !stride_ok(r->token_stride) || !stride_ok(r->head_stride)) return refuse(message);
     return TV_OK;
 }
-// Bytes from the first to the last element of a [tokens][heads][dim] view
-int64_t extent(const tv_kv_rows *r, int64_t tokens, int64_t heads, int64_t dim) {
-    return 2 * ((tokens - 1) * r->token_stride + (heads - 1) * r->head_stride + dim);
+// Runs of `run` bytes: count[0] times stride[0] apart, each time count[1] of them stride[1] apart, the larger stride first.
+struct Runs {
+    intptr_t at;
+    int64_t count[2], stride[2], run;
+};
+Runs runs_of(const tv_kv_rows *r, int64_t tokens, int64_t heads, int64_t dim) {
+    Runs v{reinterpret_cast<intptr_t>(r->data), {tokens, heads}, {2 * r->token_stride, 2 * r->head_stride}, 2 * dim};
+    for (int i = 0; i < 2; ++i)
+        if (v.count[i] == 1) v.stride[i] = 0;                  // whatever it says
+    if (v.stride[0] < v.stride[1]) { std::swap(v.count[0], v.count[1]); std::swap(v.stride[0], v.stride[1]); }
+    return v;
 }
-bool overlap(const void *a, int64_t na, const void *b, int64_t nb) {
-    const char *x = static_cast<const char *>(a), *y = static_cast<const char *>(b);
-    return x < y + nb && y < x + na;
+Runs bytes_of(const void *p, size_t bytes) { return {reinterpret_cast<intptr_t>(p), {1, 1}, {0, 0}, int64_t(bytes)}; }
+// Whether `na` runs sa apart from 0 on and `nb` runs sb apart from `at` on share a byte.
+bool meet(int64_t na, int64_t sa, int64_t ra, __int128 at, int64_t nb, int64_t sb, int64_t rb) {
+    constexpr int64_t kMost = 1 << 18;
+    if (na > kMost || nb > kMost) return true;                 // not worth the time
+    for (int64_t i = 0, j = 0; i < na && j < nb;) {
+        const __int128 x = __int128(i) * sa, y = at + __int128(j) * sb;
+        if (x + ra <= y) ++i;
+        else if (y + rb <= x) ++j;
+        else return true;
+    }
+    return false;
+}
+// Whether two views share a byte.  Views of one buffer that interleave (heads of a fused projection, say) do not; where strides
+// have nothing in common and the views lie in the same range, they are taken to.
+bool overlap(const Runs &a, const Runs &b) {
+    auto extent = [](const Runs &v) { return __int128(v.count[0] - 1) * v.stride[0] + __int128(v.count[1] - 1) * v.stride[1] + v.run; };
+    if (a.at + extent(a) <= b.at || b.at + extent(b) <= a.at) return false;
+    const int64_t outer = a.stride[0] > b.stride[0] ? a.stride[0] : b.stride[0];
+    if (outer == 0) return true;                               // a run each
+    // rows `outer` apart, of runs within a row
+    struct Rows { int64_t rows, count, stride; bool ok; };
+    auto rows_in = [&](const Runs &v) {
+        const Rows r = v.stride[0] == outer ? Rows{v.count[0], v.count[1], v.stride[1], true} : Rows{1, v.count[0], v.stride[0], v.count[1] == 1};
+        return Rows{r.rows, r.count, r.stride, r.ok && __int128(r.count - 1) * r.stride + v.run <= outer};
+    };
+    const Rows ra = rows_in(a), rb = rows_in(b);
+    if (!ra.ok || !rb.ok) return true;
+    int64_t apart = (b.at - a.at) / outer, within = (b.at - a.at) % outer;
+    if (within < 0) { within += outer; --apart; }
+    // row j of b begins `within` after row j + apart of a, and ends in that or the next
+    auto both = [&](int64_t shift) { return shift < ra.rows && shift > -rb.rows; };
+    return (both(apart) && meet(ra.count, ra.stride, a.run, within, rb.count, rb.stride, b.run)) ||
+           (both(apart + 1) && meet(ra.count, ra.stride, a.run, __int128(within) - outer, rb.count, rb.stride, b.run));
 }
 KvRows rows_of(const tv_kv_rows *r) { return r ? KvRows{r->data, r->token_stride, r->head_stride} : KvRows{nullptr, 0, 0}; }
 KvBatch batch_of(const tv_kv_batch *b) { return {b->table, b->lens, b->offsets, b->table_stride, int(b->table_width), int(b->sequences)}; }
@@ -176,8 +216,12 @@ int fill_attend(KvAttendParams &p, const tv_kv_cache *c, const tv_kv_batch *b, i
     int rc = check_rows(q, "q must be given, 16-byte aligned, with strides that are positive multiples of 8 elements");
     if (rc == TV_OK) rc = check_rows(out, "out must be given, 16-byte aligned, with strides that are positive multiples of 8 elements");
     if (rc != TV_OK) return rc;
-    if (overlap(q->data, extent(q, tokens, heads, c->head_dim), out->data, extent(out, tokens, heads, c->head_dim))) return refuse("out must not overlap q");
+    if (overlap(runs_of(q, tokens, heads, c->head_dim), runs_of(out, tokens, heads, c->head_dim))) return refuse("out must not overlap q");
     if (!aligned(lse, 4)) return refuse("lse must be 4-byte aligned");
+    if (lse) {
+        const Runs sums = bytes_of(lse, size_t(tokens) * heads * 4);
+        if (overlap(sums, runs_of(q, tokens, heads, c->head_dim)) || overlap(sums, runs_of(out, tokens, heads, c->head_dim))) return refuse("lse must not overlap q or out");
+    }
     if (!(scale > 0.0f) || !std::isfinite(scale)) return refuse("scale must be positive and finite");
     p.batch = batch_of(b);
     p.q = rows_of(q);
@@ -215,9 +259,13 @@ int tv_kv_append(const tv_kv_cache *c, const tv_kv_batch *b, int64_t tokens, int
     if (rc == TV_OK && q) rc = check_rows(q, "q must be 16-byte aligned, with strides that are positive multiples of 8 elements");
     if (rc == TV_OK && q) rc = check_rows(q_out, "q_out must be 16-byte aligned, with strides that are positive multiples of 8 elements");
     if (rc != TV_OK) return rc;
-    if (q && !(q->data == q_out->data && q->token_stride == q_out->token_stride && q->head_stride == q_out->head_stride) &&
-        overlap(q->data, extent(q, tokens, heads, c->head_dim), q_out->data, extent(q_out, tokens, heads, c->head_dim)))
-        return refuse("q_out must be q itself or not overlap it");
+    if (q) {
+        const Runs to = runs_of(q_out, tokens, heads, c->head_dim);
+        if (!(q->data == q_out->data && q->token_stride == q_out->token_stride && q->head_stride == q_out->head_stride) && overlap(runs_of(q, tokens, heads, c->head_dim), to))
+            return refuse("q_out must be q itself or not overlap it");
+        if (overlap(runs_of(k_new, tokens, c->kv_heads, c->head_dim), to) || overlap(runs_of(v_new, tokens, c->kv_heads, c->head_dim), to))
+            return refuse("q_out must not overlap k_new or v_new");
+    }
     if (rotary < 0 || rotary > c->head_dim || rotary % 16 != 0) return refuse("rotary must be a multiple of 16 up to head_dim");
     if (rotary > 0 && (!cos || !sin || !aligned(cos, 16) || !aligned(sin, 16) || positions < 0 || positions > (int64_t(1) << 40)))
         return refuse("cos and sin must be given and 16-byte aligned, and positions not negative");
@@ -321,6 +369,10 @@ int tv_kv_attend_selected(const tv_kv_cache *c, const tv_kv_batch *b, int64_t to
     rc = check_workspace(workspace, workspace_bytes,
                          carve_chosen(p, s, static_cast<char *>(workspace), slots, tokens, tokens * heads, tokens * c->kv_heads * budget, c));
     if (rc != TV_OK) return rc;
+    const Runs list = bytes_of(pages_out, size_t(tokens) * c->kv_heads * budget * 4);
+    if (overlap(list, runs_of(q, tokens, heads, c->head_dim)) || overlap(list, runs_of(out, tokens, heads, c->head_dim)) ||
+        (lse && overlap(list, bytes_of(lse, size_t(tokens) * heads * 4))))
+        return refuse("pages_out must not overlap q, out or lse");
     s.batch = p.batch; s.q = p.q; s.bounds = c->bounds; s.scales = c->scales; s.chosen = pages_out;
     s.tokens = p.tokens; s.group = p.group; s.kv_heads = p.kv_heads; s.page_shift = p.page_shift; s.pages = p.pages;
     s.budget = int(budget); s.first = int(first); s.recent = int(recent);
