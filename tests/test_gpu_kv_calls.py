@@ -54,3 +54,32 @@ def test_results_over_one_another_are_refused():
                  lambda: cache.attend_selected(batch, q, budget=1, recent=0, out=out, lse=lse, pages=lse.view(torch.int32).view(2, 4, 1))):
         with pytest.raises(ValueError, match="overlap"):
             call()
+
+
+def test_gradients_are_refused_and_not_dropped():
+    from turbovec_b200.kvcache import PagedKVCache
+    s = R.Setup(602, dtype=BF, dim=64, page=16, heads=4, kv_heads=2, new=[1, 1], lens=[5, 40])
+    cache, batch = handles(s)
+    q, k, v = s.q.cuda(), s.k_new.cuda(), s.v_new.cuda()
+    cos = torch.rand(60, 32, device="cuda")
+
+    def asks(t):
+        return t.detach().clone().requires_grad_()
+    calls = [lambda: cache.attend(batch, asks(q)), lambda: cache.attend_selected(batch, asks(q), budget=2), lambda: cache.attend(batch, q, out=asks(q)),
+             lambda: cache.attend(batch, q, lse=asks(torch.zeros(2, 4, device="cuda"))),
+             lambda: cache.append(batch, asks(k), v), lambda: cache.append(batch, k, asks(v)), lambda: cache.append(batch, k, v, q=asks(q)),
+             lambda: cache.append(batch, k, v, cos=asks(cos), sin=cos), lambda: cache.append(batch, k, v, cos=cos, sin=asks(cos))]
+    k_pool, v_pool = asks(cache.k), asks(cache.v)
+    for pools in ((k_pool, cache.v), (cache.k, v_pool)):
+        other = PagedKVCache(*pools, cache.bounds, cache.scales)
+        calls += [lambda o=other: o.attend(batch, q), lambda o=other: o.attend_selected(batch, q, budget=2), lambda o=other: o.append(batch, k, v)]
+    kept = cache.k.clone()
+    for call in calls:
+        with pytest.raises(RuntimeError, match="gradient"):
+            call()
+    assert torch.equal(cache.k, kept)
+    want = cache.attend(batch, q)
+    with torch.no_grad():                               # nobody asks for one
+        assert torch.equal(cache.attend(batch, asks(q)), want)
+        assert torch.equal(PagedKVCache(k_pool, v_pool).attend(batch, asks(q)), want)
+        cache.append(batch, asks(k), asks(v), q=asks(q), cos=asks(cos), sin=asks(cos))

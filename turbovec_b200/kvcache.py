@@ -12,7 +12,8 @@ offsets[b]) + j of the sequence's own pages, table[b][position // page_size].  R
 
 Everything runs on torch's current stream of the cache's device, without a synchronisation, and may be captured into a CUDA graph;
 results and workspaces come from torch's allocator.  Tensors are read when the kernels run: table, lens and offsets may be changed
-in place between calls, and a captured graph sees the new values.  There is no CPU path, and no gradient passes through.
+in place between calls, and a captured graph sees the new values.  There is no CPU path.  No gradient passes through: tensors
+that require one are refused unless gradients are off (torch.no_grad, torch.inference_mode).
 """
 from __future__ import annotations
 
@@ -52,6 +53,10 @@ def _tensor(name: str, t, dtype, ndim: int, device=None) -> torch.Tensor:
     if device is not None and t.device != device:
         raise ValueError(f"{name} must be on {device}, got {t.device}")
     return t
+
+
+def _no_gradient(name: str):
+    raise RuntimeError(f"{name} requires a gradient, and none passes through the cache: detach it, or call under torch.no_grad()")
 
 
 def _last_adjacent(name: str, t: torch.Tensor) -> None:
@@ -181,6 +186,8 @@ class PagedKVCache:
         st = t.stride()
         if st[2] != 1:
             raise ValueError(f"{name}: the elements of the last dimension must be adjacent")
+        if t.requires_grad and torch.is_grad_enabled():
+            _no_gradient(name)
         return n, h, _native.KvRowsView(t.data_ptr(), st[0] if n > 1 else h * d, st[1] if h > 1 else d)
 
     def _query(self, q, tokens: int | None = None):
@@ -194,6 +201,8 @@ class PagedKVCache:
             raise TypeError(f"batch must be a KVBatch, got {type(batch).__name__}")
         if batch.device != self.device:
             raise ValueError(f"batch must be on {self.device}, got {batch.device}")
+        if (self.k.requires_grad or self.v.requires_grad) and torch.is_grad_enabled():
+            _no_gradient("the pool")
         return batch._view
 
     def _array(self, name: str, t, dtype, shape) -> int:
@@ -206,6 +215,8 @@ class PagedKVCache:
             raise ValueError(f"{name} must be contiguous with {'one dimension' if shape is None else f'shape {tuple(shape)}'}, got {tuple(t.shape)}")
         if t.get_device() != self._index:
             raise ValueError(f"{name} must be on {self.device}, got {t.device}")
+        if t.requires_grad and torch.is_grad_enabled():
+            _no_gradient(name)
         return t.data_ptr()
 
     def _workspace(self, op: str, batch, *sizes) -> torch.Tensor:
