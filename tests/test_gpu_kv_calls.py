@@ -83,3 +83,37 @@ def test_gradients_are_refused_and_not_dropped():
         assert torch.equal(cache.attend(batch, asks(q)), want)
         assert torch.equal(PagedKVCache(k_pool, v_pool).attend(batch, asks(q)), want)
         cache.append(batch, asks(k), asks(v), q=asks(q), cos=asks(cos), sin=asks(cos))
+
+
+def test_a_reported_error_does_not_wait_for_the_next_call():
+    """A device number that no machine has: the call says so, and torch's next call meets no error."""
+    from turbovec_b200 import _native
+    s = R.Setup(603, dtype=BF, dim=64, page=16, heads=4, kv_heads=2, new=[1, 1], lens=[5, 40])
+    cache, batch = handles(s)
+    q, k = s.q.cuda(), s.k_new.cuda()
+    clean = cache.attend(batch, q)
+    index, cache._view.device = cache._view.device, 63
+    calls = (lambda: cache.append(batch, k, k), lambda: cache.attend(batch, q), lambda: cache.attend_selected(batch, q, budget=2))
+    for call in calls:
+        cache._sizes.clear()
+        with pytest.raises(RuntimeError, match="no such CUDA device"):
+            call()
+        assert float((q.float() * 0 + 1).sum()) == q.numel()
+    assert _native.load().tv_kv_status(63) != 0
+    torch.cuda.synchronize()
+    cache._view.device = index
+    assert torch.cuda.current_device() == index and torch.equal(cache.attend(batch, q), clean)
+
+
+@pytest.mark.skipif(torch.cuda.device_count() < 2, reason="two devices are needed")
+def test_the_callers_device_stays_the_current_one():
+    s = R.Setup(604, dtype=BF, dim=64, page=16, heads=4, kv_heads=2, new=[1, 1], lens=[5, 40], prefix=30)
+    cache, batch = handles(s)
+    q, k, pre = s.q.cuda(), s.k_new.cuda(), s.prefix_pages.cuda()
+    want = cache.attend(batch, q, prefix_pages=pre, prefix_len=30)
+    with torch.cuda.device(1):
+        assert torch.equal(cache.attend(batch, q, prefix_pages=pre, prefix_len=30), want)
+        cache.attend_selected(batch, q, budget=2)
+        cache.append(batch, k, k)
+        cache.check()
+        assert torch.cuda.current_device() == 1

@@ -246,3 +246,32 @@ def test_views_that_share_bytes_are_never_let_through(lib, seed):
     # strides that no memory has do not wrap
     far = type(row)(at, (1 << 38) - 8, 128)
     assert lib.tv_kv_attend(cache, batch, 1 << 29, 4, far, at, 2, 20, 0.1, type(row)(at + 4096, 512, 128), None, at, 1 << 40, None) == 90
+
+
+def host_cache(monkeypatch, lib, **change):
+    """The Python class over host memory: its calls reach the C entries, which refuse them."""
+    from turbovec_b200 import kvcache
+    buf, at, view, batch_view, _ = views(head_dim=64, k_head_stride=1024, k_token_stride=64, v_head_stride=1024, v_token_stride=64, **change)
+    cache = object.__new__(kvcache.PagedKVCache)
+    k = torch.zeros(4, 2, 16, 64, dtype=torch.bfloat16)
+    bounds, scales = torch.zeros(4, 2, 2, 64, dtype=torch.int8), torch.zeros(4, 2)
+    for name, x in dict(k=k, v=k.clone(), bounds=bounds, scales=scales).items():
+        object.__setattr__(cache, "_" + name if hasattr(kvcache.PagedKVCache, name) else name, x)
+    cache._lib, cache._view, cache._buf = lib, view, buf
+    cache.device, cache.dtype, cache.pages, cache.kv_heads, cache.page_size, cache.head_dim = torch.device("cpu"), torch.bfloat16, 4, 2, 16, 64
+    cache._index, cache._scale, cache._sizes = -1, 0.125, {}
+    monkeypatch.setattr(kvcache, "_stream", lambda index: 0)
+    batch = kvcache.KVBatch(torch.zeros(1, 2, dtype=torch.int32), torch.ones(1, dtype=torch.int32))
+    return cache, batch, torch.zeros(1, 4, 64, dtype=torch.bfloat16)
+
+
+def test_a_device_that_fails_is_no_wrong_argument(monkeypatch, lib):
+    """Also where the size of a workspace is asked for first; sizes that are refused stay wrong arguments."""
+    cache, batch, q = host_cache(monkeypatch, lib, device=63)
+    kv = torch.zeros(1, 2, 64, dtype=torch.bfloat16)
+    for call in (lambda: cache.attend(batch, q), lambda: cache.attend_selected(batch, q, budget=2), lambda: cache.append(batch, kv, kv)):
+        with pytest.raises(RuntimeError, match="no such CUDA device"):
+            call()
+    for call in (lambda: cache.attend(batch, q, scale=-1.0), lambda: cache.attend_selected(batch, q, budget=40_000)):
+        with pytest.raises(ValueError):
+            call()

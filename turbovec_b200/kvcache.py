@@ -219,14 +219,14 @@ class PagedKVCache:
             _no_gradient(name)
         return t.data_ptr()
 
-    def _workspace(self, op: str, batch, *sizes) -> torch.Tensor:
-        """A workspace for an operator; its size for these sizes is asked for once."""
+    def _workspace(self, op: str, batch, *sizes):
+        """A workspace for an operator; its size for these sizes is asked for once.  None where there is none: the operator says why."""
         key = (op, _options, batch._view.sequences, *sizes)
         n = self._sizes.get(key)
         if n is None:
             n = getattr(self._lib, f"tv_kv_{op}_workspace")(self._view, batch._view, *sizes)
             if n == 0:
-                _fail(self._lib, 90)
+                return None
             if len(self._sizes) >= 256:
                 self._sizes.clear()
             self._sizes[key] = n
@@ -287,7 +287,8 @@ class PagedKVCache:
         ws_at, ws_n = None, 0
         if tokens and len(batch):
             ws = self._workspace("attend", batch, tokens, heads, prefix_len)
-            ws_at, ws_n = ws.data_ptr(), ws.shape[0]
+            if ws is not None:
+                ws_at, ws_n = ws.data_ptr(), ws.shape[0]
         rc = self._lib.tv_kv_attend(self._view, b, tokens, heads, qr, pages_at, width, prefix_len, self._scale if scale is None else scale,
                                     orow, lse_at, ws_at, ws_n, _stream(self._index))
         if rc:
@@ -315,7 +316,8 @@ class PagedKVCache:
         ws_at, ws_n = None, 0
         if tokens and len(batch):
             ws = self._workspace("attend_selected", batch, tokens, heads, budget)
-            ws_at, ws_n = ws.data_ptr(), ws.shape[0]
+            if ws is not None:
+                ws_at, ws_n = ws.data_ptr(), ws.shape[0]
         rc = self._lib.tv_kv_attend_selected(self._view, b, tokens, heads, qr, budget, first, recent, self._scale if scale is None else scale,
                                              orow, lse_at, pages_at, ws_at, ws_n, _stream(self._index))
         if rc:
