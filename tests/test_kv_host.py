@@ -275,3 +275,21 @@ def test_a_device_that_fails_is_no_wrong_argument(monkeypatch, lib):
     for call in (lambda: cache.attend(batch, q, scale=-1.0), lambda: cache.attend_selected(batch, q, budget=40_000)):
         with pytest.raises(ValueError):
             call()
+
+
+def test_tensors_that_calls_use_are_changed_in_place_and_not_replaced(monkeypatch, lib):
+    """A call reads the tensors that a batch or a cache was made of: another one in their place would be passed over in silence."""
+    cache, batch, _ = host_cache(monkeypatch, lib)
+    address = batch.lens.data_ptr()
+    batch.lens += 1
+    batch.table[0, 1] = 3
+    assert batch.lens.tolist() == [2] and batch.table.tolist() == [[0, 3]] and batch.lens.data_ptr() == address == batch._view.lens
+    for name in ("table", "lens", "offsets"):
+        with pytest.raises(AttributeError, match="in place"):
+            setattr(batch, name, getattr(batch, name).clone())
+    for name in ("k", "v", "bounds", "scales"):
+        t = getattr(cache, name)
+        setattr(cache, name, t)
+        with pytest.raises(AttributeError, match="in place"):
+            setattr(cache, name, t.clone())
+        assert getattr(cache, name) is t

@@ -74,10 +74,25 @@ def set_option(option: int, value: int) -> None:
     _options += 1
 
 
+def _kept(name: str) -> property:
+    """A tensor whose address calls use: what it holds may be changed, it may not be replaced."""
+    place = "_" + name
+
+    def get(self):
+        return getattr(self, place)
+
+    def put(self, t):
+        if t is not getattr(self, place):               # (`batch.lens += 1` gives the tensor itself)
+            raise AttributeError(f"{name} is changed in place; for another tensor make another {type(self).__name__}")
+    return property(get, put)
+
+
 class KVBatch:
     """The sequences of a call: `table` int32 [sequences, width], page numbers of each; `lens` int32 [sequences], tokens in its own
     pages, those of the call among them; `offsets` int32 [sequences + 1], first row of each (None: one row each).  The tensors
-    are kept and read when the kernels run."""
+    are kept and read when the kernels run: change them in place."""
+
+    table, lens, offsets = _kept("table"), _kept("lens"), _kept("offsets")
 
     def __init__(self, table: torch.Tensor, lens: torch.Tensor, offsets: torch.Tensor | None = None):
         _tensor("lens", lens, torch.int32, 1)
@@ -94,7 +109,7 @@ class KVBatch:
         _tensor("offsets", offsets, torch.int32, 1, self.device)
         if offsets.numel() != n + 1 or not offsets.is_contiguous():
             raise ValueError(f"offsets must hold {n + 1} adjacent numbers, got {offsets.numel()}")
-        self.table, self.lens, self.offsets = table, lens, offsets
+        self._table, self._lens, self._offsets = table, lens, offsets
         width = table.shape[1]
         stride = table.stride(0) if n > 1 else width
         if stride < width:
@@ -102,7 +117,7 @@ class KVBatch:
         self._view = _native.KvBatchView(n, width, stride, table.data_ptr(), lens.data_ptr(), offsets.data_ptr())
 
     def __len__(self) -> int:
-        return self.lens.numel()
+        return self._view.sequences
 
 
 class PagedKVCache:
@@ -110,6 +125,8 @@ class PagedKVCache:
     channels (a pool laid out [pages, page_size, kv_heads, head_dim] is passed as its transpose(1, 2)), bfloat16 or float16, head_dim
     64 or 128, page_size 16, 32, 64 or 128.  bounds int8 [pages, kv_heads, 2, head_dim] and scales float32 [pages, kv_heads] hold
     the lowest and highest key of every channel of a page, as multiples of scales; both None where no pages are selected by score."""
+
+    k, v, bounds, scales = _kept("k"), _kept("v"), _kept("bounds"), _kept("scales")
 
     def __init__(self, k: torch.Tensor, v: torch.Tensor, bounds: torch.Tensor | None = None, scales: torch.Tensor | None = None):
         if not isinstance(k, torch.Tensor):
@@ -141,7 +158,7 @@ class PagedKVCache:
         self._lib = _native.load()
         if k.device.type != "cuda":
             raise RuntimeError("turbovec_b200 has no CPU path: the cache must be in the memory of a CUDA device")
-        self.k, self.v, self.bounds, self.scales = k, v, bounds, scales
+        self._k, self._v, self._bounds, self._scales = k, v, bounds, scales
         self.device, self.dtype = k.device, k.dtype
         self.pages, self.kv_heads, self.page_size, self.head_dim = pages, heads, page_size, dim
         self._index, self._scale, self._sizes = k.device.index, dim ** -0.5, {}
@@ -201,7 +218,7 @@ class PagedKVCache:
             raise TypeError(f"batch must be a KVBatch, got {type(batch).__name__}")
         if batch.device != self.device:
             raise ValueError(f"batch must be on {self.device}, got {batch.device}")
-        if (self.k.requires_grad or self.v.requires_grad) and torch.is_grad_enabled():
+        if (self._k.requires_grad or self._v.requires_grad) and torch.is_grad_enabled():
             _no_gradient("the pool")
         return batch._view
 
@@ -300,7 +317,7 @@ class PagedKVCache:
         """Attention of every row over at most `budget` pages of its sequence: the `first` and the `recent` ones and the best of the others by
         the bound of what their keys can score (include/turbovec_b200.h), chosen for each token and key head.  Returns (out, pages): the
         chosen page numbers within the sequence, int32 [tokens, kv_heads, budget], ascending, then -1."""
-        if self.bounds is None:
+        if self._bounds is None:
             raise ValueError("the cache has no bounds to choose pages by")
         b = self._batch(batch)
         tokens, heads, qr = self._query(q)
