@@ -119,3 +119,26 @@ def test_prefix_kernels_of_several_parts_on_two_streams(prefix_kernel):  # noqa:
         for i, (run, alone, graph, got, stream, cache) in enumerate(work):
             assert torch.equal(got, alone) and torch.equal(eager[2 * i], alone) and torch.equal(eager[2 * i + 1], alone)
             cache.check()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("offsets", [[0, 3, 1, 3], [2, 0, 3, 1], [0, 2, 0, 3], [-5, 9, -5, 9]])
+def test_blocks_of_a_choice_agree_where_sequences_overlap(offsets):
+    """Offsets that do not ascend put a row into several sequences, some with fewer pages than the budget: all blocks take the lowest of them."""
+    s = R.Setup(750, dtype=BF, dim=64, page=16, heads=2, kv_heads=1, new=[1, 1, 1], lens=[30, 16 * 700, 16 * 500], padding=0)
+    cache, batch = handles(s)
+    batch.offsets.copy_(torch.tensor(offsets, dtype=torch.int32))
+    spans = [(max(0, min(a, 3)), max(max(0, min(a, 3)), min(b, 3))) for a, b in zip(offsets, offsets[1:])]
+    q = s.q.cuda()
+    for _ in range(3):
+        pages = torch.full((3, 1, 6), 7, dtype=torch.int32, device="cuda")
+        cache.attend_selected(batch, q, budget=6, first=1, recent=2, pages=pages)
+        cache.check()
+        for t in range(3):
+            mine = [b for b, (first, last) in enumerate(spans) if first <= t < last]
+            if not mine:
+                assert (pages[t] == 7).all()
+                continue
+            b = mine[0]
+            want = R.choose(s, t, 0, b, s.lens[b] - spans[b][1] + t, 6, 1, 2)
+            assert pages[t, 0].tolist() == want + [-1] * (6 - len(want)), (t, b)

@@ -81,13 +81,21 @@ __global__ void __launch_bounds__(kSelectThreads, 2) kv_select_kernel(const KvSe
     };
     uint32_t q_first[D / 64] = {};
     if (warp < p.group) query(warp, q_first);
-    if (tid == 0) sh.seq[2] = 0;
+    if (tid == 0) { sh.seq[0] = INT_MAX; sh.seq[2] = 0; }
     __syncthreads();
-    for (int i = tid; i < p.batch.sequences; i += kSelectThreads) {        // (of sequences that overlap, which offsets that decrease give, any)
-        const int from = p.batch.offsets[i], to = p.batch.offsets[i + 1], len = p.batch.lens[i];
-        const KvSpan sp = kv_span(from, to, p.tokens);
-        if (token >= sp.first && token < sp.first + sp.count) { sh.seq[0] = i; sh.seq[1] = sp.first; sh.seq[2] = sp.count; sh.seq[3] = len; }
+    // Offsets that decrease give sequences that overlap: the lowest of them, for the blocks of a cluster must all take the same one (a block
+    // that had nothing to score would have left when the others write into its memory).
+    int mine = INT_MAX, len_of_mine = 0;
+    KvSpan span_of_mine{0, 0};
+    for (int i = tid; i < p.batch.sequences && mine == INT_MAX; i += kSelectThreads) {
+        const int from = p.batch.offsets[i], to = p.batch.offsets[i + 1];
+        len_of_mine = p.batch.lens[i];
+        span_of_mine = kv_span(from, to, p.tokens);
+        if (token >= span_of_mine.first && token < span_of_mine.first + span_of_mine.count) mine = i;
     }
+    if (mine != INT_MAX) atomicMin(&sh.seq[0], mine);
+    __syncthreads();
+    if (mine != INT_MAX && mine == sh.seq[0]) { sh.seq[1] = span_of_mine.first; sh.seq[2] = span_of_mine.count; sh.seq[3] = len_of_mine; }
     __syncthreads();
     const int b = sh.seq[0], first_row = sh.seq[1], count = sh.seq[2], len = sh.seq[3];
     if (count == 0) {                                                      // behind the last sequence
