@@ -6,7 +6,8 @@
 // ends inside an item leaves partial results, (base of the weights, their sum, weighted sum of values), in slot
 // item + block, a number that is different for every pair of the two that meet; a second kernel joins them.
 //
-// Bound by memory: a tile of 128 channels is 32 KB and 4 * 64 * 128 * 16 multiply-adds, most of them padding where rows are few.  One warp
+// Bound by memory: a tile of 128 channels is 32 KB and 3 * 64 * 128 * 16 multiply-adds (Q K^T, the weights times V, and what rounding the
+// weights left times V), most of them padding where rows are few.  One warp
 // keeps the ring of tiles full by tensor copies; four warps take 16 keys of each tile: no exchange between warps until the end of a
 // part.  What a part costs beside its tiles is weighed as four tiles when the list is divided (2, 3, 4, 5, 6: attend_48_ragged 60.0, 54.2, 54.8,
 // 55.4, 55.7 us a call, attend_24_drafts_prefix_8200 57.1, 55.4, 52.8, 53.0, 52.5).  attend_48_ragged, 48 sequences of 1 to 12,000 keys,
@@ -76,9 +77,6 @@ struct Walk {
     }
     __device__ __forceinline__ int row_tiles(int count) const { return int((int64_t(count) * p.group + kKvRows - 1) / kKvRows); }
     __device__ __forceinline__ KvSpan span(int i) const { return kv_span(p.batch.offsets[i], p.batch.offsets[i + 1], p.tokens); }
-    __device__ __forceinline__ int64_t cost(int i) const {
-        return int64_t(row_tiles(span(i).count)) * p.kv_heads * (p.item_cost + tiles_of(p.batch.lens[i]));
-    }
     __device__ __forceinline__ int64_t items(int i) const { return int64_t(row_tiles(span(i).count)) * p.kv_heads; }
 
     // the next part; false when the run is over

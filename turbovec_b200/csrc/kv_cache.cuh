@@ -65,7 +65,6 @@ template <> struct KvType<__nv_bfloat16> {
         return d;
     }
     static constexpr uint32_t kExponents = 0x7f807f80u;
-    static constexpr CUtensorMapDataType kMapType = CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
 };
 template <> struct KvType<__half> {
     static constexpr float kLift = 11.0f, kRescaleAt = 4.0f;
@@ -76,7 +75,6 @@ template <> struct KvType<__half> {
         return d;
     }
     static constexpr uint32_t kExponents = 0x7c007c00u;
-    static constexpr CUtensorMapDataType kMapType = CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
 };
 
 // Smallest e in [kKvScaleMin, kKvScaleMax] with amax <= 127 * 2^e; amax >= 0 (infinite: the largest).
@@ -109,8 +107,10 @@ inline cudaError_t kv_allow_shared(Kernel *kern, std::atomic<uint64_t> &done, in
     return e;
 }
 
-// Launches a kernel that may begin before the one in front of it in the stream has ended: each of them waits (griddepcontrol.wait)
-// before it touches memory.
+// Launches a kernel that may begin before the one in front of it in the stream has ended.  Every block of every kernel waits
+// (griddepcontrol.wait) before it ends, so that what follows a kernel that has ended follows all before it too, and waits before it touches
+// memory, with one exception: a kernel may read and write first if the kernel in front of it waits before it lets this one begin
+// (griddepcontrol.launch_dependents) and neither touches what the other writes.  The attention behind a prefix kernel does.
 template <typename... Params, typename... Args>
 inline cudaError_t kv_launch(void (*kern)(Params...), dim3 grid, int threads, size_t smem, cudaStream_t s, const Args &...args) {
     cudaLaunchAttribute early;

@@ -1,10 +1,10 @@
-// Which pages of its sequence a token attends to: the first ones, the most recent ones, and the best of the others by a score that
-// bounds what any key of a page can give.
+// Which pages of its sequence a token attends to: the first ones, the most recent ones, and the best of the others by a score: what a key at
+// the page's bounds would give the query, rounded to int8.  (Not quite a bound of what its keys give: the query's rounding may go either way.)
 //
 // The score of a page for a key head is the largest, over the query heads that share it, of sum_d max(q_d lo_d, q_d hi_d) with q in
 // int8 (multiples of a power of two per head, nearest, ties to even) and the page's int8 bounds: a contraction of (min(q, 0), max(q, 0))
-// with (lo, hi), exact in whole numbers below 2^22, times powers of two (2^-24 to 2^40 each): no rounding anywhere, so the choice does not depend on the
-// order of any sum, and equal scores go to the lower page.
+// with (lo, hi), exact in whole numbers below 2^22, times powers of two (2^-24 to 2^40 each): nothing is rounded after the query, so the choice does
+// not depend on the order of any sum, and equal scores go to the lower page.
 //
 // The kernel is a chain of dependent steps (sequence, quantised queries, scores, histogram, list), each a latency of its own; the bounds alone
 // (2 D bytes a page and head) would be a fraction of its time.  selected_48x65536, 830 pages to each of 192 (token, head) pairs, 41 MB of

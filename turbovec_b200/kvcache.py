@@ -8,7 +8,8 @@ a long prefix, and attention over pages that a cheap score selects (tv_kv_* of i
     out, pages = cache.attend_selected(batch, q, budget=64, first=1, recent=4)
 
 Row t of a call is token j of sequence b, offsets[b] <= t < offsets[b + 1]; it stands at position lens[b] - (offsets[b + 1] -
-offsets[b]) + j of the sequence's own pages, table[b][position // page_size].  Rows behind the last sequence are left as they are.
+offsets[b]) + j of the sequence's own pages, table[b][position // page_size].  Rows behind the last sequence are left as they are: in a
+result that the call makes itself they hold anything.
 
 Everything runs on torch's current stream of the cache's device, without a synchronisation, and may be captured into a CUDA graph;
 results and workspaces come from torch's allocator.  Tensors are read when the kernels run: table, lens and offsets may be changed
@@ -255,7 +256,8 @@ class PagedKVCache:
         """Writes the rows of k and v [tokens, kv_heads, head_dim] into the pages of their sequences, keys rotated by the angles of
         position + position_offset; rotates q [tokens, heads, head_dim] into q_out (a new tensor by default; q itself is allowed) and
         returns it.  cos and sin: float32 [positions, rotary / 2], rotary a multiple of 16 up to head_dim; None: no rotation.  Pairs are
-        channels i and i + rotary / 2, or 2i and 2i + 1 where `interleaved`.  Tokens at positions below 0 or without an angle are left out."""
+        channels i and i + rotary / 2, or 2i and 2i + 1 where `interleaved`.  Tokens at positions below 0 or without an angle are left out: their
+        pages, bounds and rows of q_out stay as they are."""
         b = self._batch(batch)
         tokens, heads, kr = self._rows("k", k, None, self.kv_heads)
         vr = self._rows("v", v, tokens, heads)[2]
@@ -315,7 +317,7 @@ class PagedKVCache:
     def attend_selected(self, batch: KVBatch, q: torch.Tensor, *, budget: int, first: int = 1, recent: int = 1, scale: float | None = None,
                         out: torch.Tensor | None = None, lse: torch.Tensor | None = None, pages: torch.Tensor | None = None):
         """Attention of every row over at most `budget` pages of its sequence: the `first` and the `recent` ones and the best of the others by
-        the bound of what their keys can score (include/turbovec_b200.h), chosen for each token and key head.  Returns (out, pages): the
+        a score, what a key at a page's bounds would give the query rounded to int8 (include/turbovec_b200.h), chosen for each token and key head.  Returns (out, pages): the
         chosen page numbers within the sequence, int32 [tokens, kv_heads, budget], ascending, then -1."""
         if self._bounds is None:
             raise ValueError("the cache has no bounds to choose pages by")
