@@ -117,3 +117,29 @@ def test_the_callers_device_stays_the_current_one():
         cache.append(batch, k, k)
         cache.check()
         assert torch.cuda.current_device() == 1
+
+
+@pytest.mark.parametrize("tensor", [0, 1])
+def test_a_batch_without_pages_of_its_own(tensor):
+    """Tables of no width: rows see the prefix alone, choose nothing, and append nothing."""
+    from turbovec_b200 import kvcache
+    s = R.Setup(605, dtype=BF, dim=128, page=16, heads=4, kv_heads=2, new=[1, 2], lens=[0, 0], prefix=150)
+    cache, _ = handles(s)
+    batch = kvcache.KVBatch(torch.zeros(2, 0, dtype=torch.int32, device="cuda"), torch.tensor([0, 9], dtype=torch.int32, device="cuda"),
+                            torch.tensor([0, 1, 3], dtype=torch.int32, device="cuda"))
+    s.lens, s.table = [-5, -5], s.table[:, :0]
+    q, k = s.q.cuda(), s.k_new.cuda()
+    kvcache.set_option(kvcache.OPT_TENSOR_PREFIX, tensor)
+    try:
+        out = cache.attend(batch, q, prefix_pages=s.prefix_pages.cuda(), prefix_len=150)
+    finally:
+        kvcache.set_option(kvcache.OPT_TENSOR_PREFIX, -1)
+    want = R.attend(s)
+    check_rows(s, out, None, {t: want[t] for t in range(3)})
+    assert (cache.attend(batch, q) == 0).all()
+    out, pages = cache.attend_selected(batch, q, budget=3)
+    assert (out == 0).all() and (pages == -1).all()
+    before = cache.k.clone()
+    cache.append(batch, k, k)
+    cache.check()
+    assert torch.equal(cache.k, before)
