@@ -293,3 +293,14 @@ def test_tensors_that_calls_use_are_changed_in_place_and_not_replaced(monkeypatc
         with pytest.raises(AttributeError, match="in place"):
             setattr(cache, name, t.clone())
         assert getattr(cache, name) is t
+
+
+def test_position_offsets_beyond_64_bits_do_not_wrap(monkeypatch, lib):
+    cache, batch, _ = host_cache(monkeypatch, lib, device=63)
+    kv = torch.zeros(1, 2, 64, dtype=torch.bfloat16)
+    cos = torch.zeros(4, 32)
+    for offset in (1 << 41, 1 << 64, -(1 << 64), (1 << 65) + 3):
+        with pytest.raises(ValueError, match="position_offset"):
+            cache.append(batch, kv, kv, cos=cos, sin=cos, position_offset=offset)
+    with pytest.raises(RuntimeError, match="no such CUDA device"):
+        cache.append(batch, kv, kv, cos=cos, sin=cos, position_offset=1 << 40)

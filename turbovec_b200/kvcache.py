@@ -278,6 +278,8 @@ class PagedKVCache:
                 raise ValueError("cos must be a tensor of two dimensions")
             cos_at, sin_at = self._array("cos", cos, torch.float32, cos.shape), self._array("sin", sin, torch.float32, cos.shape)
             positions, rotary = cos.shape[0], 2 * cos.shape[1]
+        if not -(1 << 40) <= position_offset <= 1 << 40:         # (ctypes cuts to 64 bits what is more)
+            raise ValueError(f"position_offset is out of range: {position_offset}")
         rc = self._lib.tv_kv_append(self._view, b, tokens, heads, kr, vr, qr, qo, cos_at, sin_at, positions, rotary,
                                     1 if interleaved else 0, position_offset, _stream(self._index))
         if rc:
