@@ -19,11 +19,12 @@
 // the same time, so that the second and later ones find them in L2.
 //
 // What bounds it is the weights.  A step (256 rows x 128 keys x 128 channels) is 2,048 cycles of MMAs (2,480 measured: halves of S
-// are MMAs of N = 64, which shared memory feeds in 48 cycles and not in 32), and it takes 3,700 (211,000 cycles for 56 steps, beginning and end
-// included); when it took 3,800, 3,630 with the MMAs left out and 2,500 with the weights left out.  1,536 cycles of it are the exponential unit (8 cycles an instruction; a quarter of the weights go by the
-// multiply-add pipe, 0, 1/8 and 3/8 are 5, 1 and 1 % slower), 960 multiply-adds, 770 maxima and conversions, per scheduler, and two
-// warps do not overlap them well.  Tried and slower: tiles of 128 keys without halves (3,650 a step, but 8,000 cycles
-// more around the loop), two threads to a row on 16 warps (4,600), one warp for all MMAs with halves (4,300).
+// are MMAs of N = 64, which shared memory feeds in 48 cycles and not in 32), and it takes 3,700 (211,000 cycles for 56 steps, beginning and
+// end included); when it took 3,800, 3,630 with the MMAs left out and 2,500 with the weights left out.  1,536 cycles of it are the
+// exponential unit (8 cycles an instruction; a quarter of the weights go by the multiply-add pipe, 0, 1/8 and 3/8 are 5, 1 and 1 %
+// slower), 960 multiply-adds, 770 maxima and conversions, per scheduler, and two warps do not overlap them well.  Tried and slower: tiles of
+// 128 keys without halves (3,650 a step, but 8,000 cycles more around the loop), two threads to a row on 16 warps (4,600), one warp for
+// all MMAs with halves (4,300).
 // attend_128_prefix_32768 (1,024 rows of 8 key heads, 32,768 keys, 137 GFLOP): 129 us from the end of
 // the kernel before it to its own end, in a row of calls: 1.06 PFLOP/s.
 #include "kv_cache.cuh"

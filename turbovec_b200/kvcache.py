@@ -319,8 +319,8 @@ class PagedKVCache:
     def attend_selected(self, batch: KVBatch, q: torch.Tensor, *, budget: int, first: int = 1, recent: int = 1, scale: float | None = None,
                         out: torch.Tensor | None = None, lse: torch.Tensor | None = None, pages: torch.Tensor | None = None):
         """Attention of every row over at most `budget` pages of its sequence: the `first` and the `recent` ones and the best of the others by
-        a score, what a key at a page's bounds would give the query rounded to int8 (include/turbovec_b200.h), chosen for each token and key head.  Returns (out, pages): the
-        chosen page numbers within the sequence, int32 [tokens, kv_heads, budget], ascending, then -1."""
+        a score, what a key at a page's bounds would give the query rounded to int8 (include/turbovec_b200.h), chosen for each token and
+        key head.  Returns (out, pages): the chosen page numbers within the sequence, int32 [tokens, kv_heads, budget], ascending, then -1."""
         if self._bounds is None:
             raise ValueError("the cache has no bounds to choose pages by")
         b = self._batch(batch)
